@@ -60,6 +60,7 @@ typedef struct spmm_csr_host {
 
 #define SPMM_DTYPE_F16 0
 #define SPMM_DTYPE_BF16 1
+#define SPMM_DTYPE_F32 2 /* dense operands of the grouped-row operators only, where they say so */
 
 /* BSR with 16x16 blocks; block b holds values[b*256 .. b*256+255], row-major inside the
  * block, as FP16 or BF16 bits. (reference: src/bsr.h:22-60, BSR_BLOCK / BSR_host / BSR) */
@@ -307,6 +308,100 @@ int spmm_bsr16_algo(const spmm_bsr_view* A, const void* B16, float* C, int32_t N
  * bad index, device wait timeout. Synchronises the device. *detail gets the offending
  * index / site. clear != 0 resets the record. */
 int spmm_device_error(int32_t device, int32_t* code, int64_t* detail, int32_t clear);
+
+/* ---------------------------------------------------------------- rows grouped by an index
+ *
+ * Products over rows that belong to groups: tokens routed to experts, the experts' products,
+ * low-rank adapters of many requests. None has a counterpart in the reference. All pointers are
+ * device pointers on the current device; calls are asynchronous on `stream`, allocate nothing,
+ * use no atomics on results (the same inputs give the same bits) and can be captured in a CUDA
+ * graph (after a first call on the device, which sets up the library's device state). Row strides
+ * (ld*) count elements and are at least the row's length; outputs must not overlap inputs except
+ * where said. Index arrays are read on the device: a bad entry never leads out of a buffer, is
+ * recorded (SPMM_ERR_BAD_INDEX, spmm_device_error) and its row is left as described below. */
+
+/* The rows of `tokens * topk` pairs sorted by group. ids[t * topk + j] in [0, groups) is the group of
+ * token t's j-th pair; a negative id means the pair has no row (its group lives elsewhere), an id past
+ * groups counts the same and is recorded. The sort is stable: pairs of one group keep their order.
+ * offsets[groups + 1]: group g's rows are [offsets[g], offsets[g+1]); order[tokens * topk]: the pair of
+ * each sorted row, -1 behind the last (NULL: not wanted); pos[tokens * topk]: each pair's sorted row, -1 if
+ * it has none. tokens * topk <= 2^31 - 4096 and groups <= 4096 (SPMM_ERR_TOO_LARGE above). A workspace of
+ * spmm_route_workspace_size bytes (0 for small inputs; any contents) belongs to the call until it has run. */
+#define SPMM_MAX_GROUPS 4096
+int spmm_route_workspace_size(int32_t tokens, int32_t topk, int32_t groups, size_t* bytes);
+int spmm_route_build(const int32_t* ids, int32_t tokens, int32_t topk, int32_t groups, int32_t* offsets, int32_t* order,
+                     int32_t* pos, void* ws, size_t ws_bytes, void* stream);
+
+/* The routing matrix as the operators below read it: pos as spmm_route_build writes it, and the number of
+ * rows of the sorted buffers. A position outside [-1, rows) is recorded and treated as -1 (no row). */
+typedef struct spmm_route_view {
+    int32_t tokens, topk;
+    int32_t rows;       /* rows of xs / ys / dys; tokens * topk always suffices */
+    const int32_t* pos; /* tokens * topk */
+} spmm_route_view;
+
+/* Tokens to their groups: xs[pos[t, j], :] = x[t, :] for every pair that has a row. Other rows of xs are left
+ * as they were. H columns; dtype F16, BF16 or F32 (bits are copied). The gradient of x is
+ * spmm_route_combine of the gradient of xs with w = NULL. */
+int spmm_route_gather(const spmm_route_view* r, const void* x, int64_t ldx, void* xs, int64_t ldxs, int32_t H,
+                      int32_t dtype, void* stream);
+
+/* And back, with weights applied: y[t, :] = sum over j in order of w[t, j] * ys[pos[t, j], :] over the pairs that
+ * have a row (FP32 FMA, one rounding at the end; 0 for a token without any). w: tokens * topk FP32, NULL = all 1.
+ * Rows of ys that no pair has are not read. With F32 rows this is spmm_csr_f32 on the routing matrix. */
+int spmm_route_combine(const spmm_route_view* r, const void* ys, int64_t ldys, const float* w, void* y, int64_t ldy,
+                       int32_t H, int32_t dtype, void* stream);
+
+/* Gradients of spmm_route_combine: dys[pos[t, j], :] = w[t, j] * dy[t, :], dw[t, j] = <dy[t, :], ys[pos[t, j], :]>
+ * (FP32 sums in a fixed order; 0 for a pair without a row). Rows of dys that no pair has are left as they were.
+ * dys or dw may be NULL (not wanted); ys is read for dw only, w for dys only (NULL = all 1). */
+int spmm_route_combine_grad(const spmm_route_view* r, const void* dy, int64_t lddy, const void* ys, int64_t ldys,
+                            const float* w, void* dys, int64_t lddys, float* dw, int32_t H, int32_t dtype,
+                            void* stream);
+
+/* Products of row groups with their own matrices, on the tensor cores: y[p, :] = w[g] * x[p, :] for
+ * offsets[g] <= p < offsets[g+1], w = groups x N x K contiguous (a block-diagonal sparse matrix with dense N x K
+ * blocks). x is rows x K, y rows x N; rows in no group are left as they were. offsets (groups + 1, non-decreasing,
+ * within [0, rows]) stays on the device; an offset out of order is clamped to its neighbours and recorded.
+ * dtype F16 or BF16 (x, w); out_dtype the same or F32; sums in FP32. 16-byte aligned pointers and rows (N and K
+ * multiples of 8, ldx/ldy * size multiples of 16) run on tcgen05; other operands on a slower kernel.
+ * groups <= 4096 (SPMM_ERR_TOO_LARGE above). */
+int spmm_grouped_mm(const int32_t* offsets, int32_t groups, int32_t rows, const void* x, int64_t ldx, const void* w,
+                    void* y, int64_t ldy, int32_t N, int32_t K, int32_t dtype, int32_t out_dtype, void* stream);
+
+/* Its gradients. dx[p, :] = w[g]^T * dy[p, :] (dy rows x N, dx rows x K; rows in no group left as they were) and
+ * dw[g] = sum of dy[p, :] * x[p, :]^T over the group's rows (groups x N x K contiguous; zero for an empty group).
+ * Rows in no group are never read into a result, whatever they hold. */
+int spmm_grouped_mm_dx(const int32_t* offsets, int32_t groups, int32_t rows, const void* dy, int64_t lddy,
+                       const void* w, void* dx, int64_t lddx, int32_t N, int32_t K, int32_t dtype, int32_t out_dtype,
+                       void* stream);
+int spmm_grouped_mm_dw(const int32_t* offsets, int32_t groups, int32_t rows, const void* dy, int64_t lddy,
+                       const void* x, int64_t ldx, void* dw, int32_t N, int32_t K, int32_t dtype, int32_t out_dtype,
+                       void* stream);
+
+/* Low-rank adapters: adapter i adds scale[i] * b[i] * (a[i] * x) to a row x of K values. */
+typedef struct spmm_lora_view {
+    int32_t adapters, rank;
+    int32_t N, K;       /* features out, features in              */
+    int32_t dtype;      /* F16 / BF16, of a, b, x, base and out   */
+    const void* a;      /* adapters x rank x K, contiguous        */
+    const void* b;      /* adapters x N x rank, contiguous        */
+    const float* scale; /* adapters, or NULL: all 1               */
+} spmm_lora_view;
+
+/* Many requests at once, beside a shared projection: for the rows p of request r (offsets[r] <= p < offsets[r+1])
+ * out[p, :] = base[p, :] + scale * b * (a * x[p, :]) with the matrices of adapter[r]; out = base for a negative adapter
+ * (none); an adapter past l->adapters counts as none and is recorded. offsets: requests + 1, on the device, as
+ * in spmm_grouped_mm; NULL = every row is a request of its own (requests == rows, single tokens). base: rows x N
+ * (the shared projection's output), NULL = 0; out may be base itself (same stride). Rows in no request are left as
+ * they were. One rounding of the result; the rank-wide intermediate is held in FP32 or as a sum of two 16-bit
+ * terms (F16: |a * x| up to 131008). rank <= 256, requests <= 4096 (SPMM_ERR_TOO_LARGE above). A workspace of
+ * spmm_lora_workspace_size bytes (any contents, 256-byte aligned) belongs to the call until it has run: calls that
+ * overlap on the GPU need one each. */
+int spmm_lora_workspace_size(const spmm_lora_view* l, int32_t requests, int32_t rows, size_t* bytes);
+int spmm_lora(const spmm_lora_view* l, const int32_t* offsets, const int32_t* adapter, int32_t requests, int32_t rows,
+              const void* x, int64_t ldx, const void* base, int64_t ldbase, void* out, int64_t ldout, void* ws,
+              size_t ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------- hybrid dispatch */
 

@@ -1,0 +1,546 @@
+// Tokens routed to groups (experts) and back.
+//
+// The routing matrix R (tokens x sorted rows) has one 1 (or w[t, j]) at (t, pos[t, j]) for every pair that has a
+// row. spmm_route_build sorts the pairs by group (a counting sort, stable), spmm_route_gather computes R1^T x,
+// spmm_route_combine R_w ys, spmm_route_combine_grad the gradients R_w^T dy and (dy ys^T) at R's nonzeros.
+// The three row kernels move rows and compute next to nothing: the rows' bytes through HBM bound them.
+// All three walk tokens, not sorted rows, so that a token's own row crosses HBM once for its topk pairs.
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+
+#include "rows.cuh"
+
+namespace spmm_b200 {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+// ------------------------------------------------------------------ sort
+//
+// Counting sort over blocks of `per_block` pairs. With one block the histogram, its scan and the placement are one
+// launch; with more, a first launch leaves each block's histogram in the workspace and every block of the second
+// adds up what it needs (blocks x groups ints from L2), so there is no wait between blocks.
+
+constexpr int kSortThreads = 1024;
+constexpr int kPairsPerBlock = 4096;
+constexpr int kMaxSortBlocks = 128;  // blocks grow beyond kPairsPerBlock instead
+
+struct SortShape {
+    int warps;      // warps with a histogram of their own
+    int blocks;
+    int per_block;  // a multiple of 32 * warps
+    size_t smem;
+};
+
+SortShape sort_shape(int pairs, int groups) {
+    SortShape s{};
+    // Per-warp histograms (ints) within 128 KiB, totals and block prefixes behind them.
+    s.warps = groups <= 1024 ? 32 : (groups <= 2048 ? 16 : 8);
+    const int unit = 32 * s.warps;
+    const long long want = std::max<long long>(kPairsPerBlock, (static_cast<long long>(pairs) + kMaxSortBlocks - 1) / kMaxSortBlocks);
+    s.per_block = static_cast<int>((want + unit - 1) / unit * unit);
+    s.blocks = std::max(1, static_cast<int>((static_cast<long long>(pairs) + s.per_block - 1) / s.per_block));
+    s.smem = sizeof(int) * (static_cast<size_t>(s.warps) * groups + 2 * static_cast<size_t>(groups) + 1 + 32);
+    return s;
+}
+
+// A pair's group, -1 for none.
+__device__ __forceinline__ int group_of(const int* __restrict__ ids, int i, int groups, DeviceErrorRecord* err) {
+    const int id = __ldg(ids + i);
+    if (id >= groups) record_device_error(err, SPMM_ERR_BAD_INDEX, i);
+    return id < 0 || id >= groups ? -1 : id;
+}
+
+__global__ void __launch_bounds__(kSortThreads) route_count_kernel(const int* __restrict__ ids, int pairs, int groups,
+                                                                   int per_block, int* __restrict__ counts,
+                                                                   DeviceErrorRecord* err) {
+    extern __shared__ int sm[];
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) sm[g] = 0;
+    __syncthreads();
+    grid_dependency_wait();
+    allow_dependent_launch();
+    const int begin = blockIdx.x * per_block, end = begin + min(per_block, pairs - begin);
+    for (int i = begin + threadIdx.x; i < end; i += blockDim.x) {
+        const int g = group_of(ids, i, groups, err);
+        if (g >= 0) atomicAdd(sm + g, 1);
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) counts[static_cast<size_t>(blockIdx.x) * groups + g] = sm[g];
+}
+
+__global__ void __launch_bounds__(kSortThreads)
+    route_place_kernel(const int* __restrict__ ids, int pairs, int groups, int warps, int per_block,
+                       const int* __restrict__ counts, int* __restrict__ offsets, int* __restrict__ order,
+                       int* __restrict__ pos, DeviceErrorRecord* err) {
+    extern __shared__ int sm[];
+    int* hist = sm;                       // [warps][groups]: counts, then each warp's next row
+    int* total = hist + warps * groups;   // [groups + 1]: counts over all blocks, then offsets
+    int* before = total + groups + 1;     // [groups]: counts of the blocks before this one
+    int* part = before + groups;          // [32]: scan of the warps' sums
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool alone = gridDim.x == 1;
+
+    for (int i = threadIdx.x; i < warps * groups + 2 * groups + 1; i += blockDim.x) sm[i] = 0;
+    __syncthreads();
+    grid_dependency_wait();
+    allow_dependent_launch();
+
+    // Warp w owns the w-th run of per_block / warps pairs: pairs of one group keep their order.
+    const int per_warp = per_block / warps;
+    const int begin = static_cast<int>(min(static_cast<long long>(pairs),
+                                           static_cast<long long>(blockIdx.x) * per_block + static_cast<long long>(warp) * per_warp));
+    const int end = warp < warps ? begin + min(per_warp, pairs - begin) : begin;
+    int* mine = hist + warp * groups;
+    for (int i = begin + lane; i < end; i += 32) {
+        const int g = group_of(ids, i, groups, alone ? err : nullptr);
+        if (g >= 0) atomicAdd(mine + g, 1);
+    }
+    if (!alone) {
+        const int parts = max(1, static_cast<int>(blockDim.x) / groups);
+        for (int u = threadIdx.x; u < parts * groups; u += blockDim.x) {
+            const int g = u % groups;
+            int all = 0, prev = 0;
+#pragma unroll 8
+            for (int b = u / groups; b < static_cast<int>(gridDim.x); b += parts) {
+                const int c = __ldg(counts + static_cast<size_t>(b) * groups + g);
+                all += c;
+                prev += b < static_cast<int>(blockIdx.x) ? c : 0;
+            }
+            atomicAdd(total + g, all);
+            atomicAdd(before + g, prev);
+        }
+    }
+    __syncthreads();
+    if (alone) {
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+            int all = 0;
+            for (int w = 0; w < warps; ++w) all += hist[w * groups + g];
+            total[g] = all;
+        }
+        __syncthreads();
+    }
+    // Exclusive scan of the totals: each thread a run of them, warps by shuffles, then the warps' sums.
+    const int run = (groups + blockDim.x - 1) / blockDim.x;
+    const int g0 = min(groups, static_cast<int>(threadIdx.x) * run), g1 = min(groups, g0 + run);
+    int sum = 0;
+    for (int g = g0; g < g1; ++g) sum += total[g];
+    int incl = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int v = __shfl_up_sync(kFull, incl, d);
+        if (lane >= d) incl += v;
+    }
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        int v = lane < static_cast<int>(blockDim.x >> 5) ? part[lane] : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int u = __shfl_up_sync(kFull, v, d);
+            if (lane >= d) v += u;
+        }
+        part[lane] = v;
+    }
+    __syncthreads();
+    int at = incl - sum + (warp > 0 ? part[warp - 1] : 0);
+    for (int g = g0; g < g1; ++g) {
+        const int c = total[g];
+        total[g] = at;
+        at += c;
+    }
+    const int rows = part[31];
+    __syncthreads();
+    // Each warp's first row of each group.
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+        int next = total[g] + before[g];
+        if (blockIdx.x == 0) offsets[g] = total[g];
+        for (int w = 0; w < warps; ++w) {
+            const int c = hist[w * groups + g];
+            hist[w * groups + g] = next;
+            next += c;
+        }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) offsets[groups] = rows;
+    __syncthreads();
+    for (int base = begin; base < end; base += 32) {
+        const int i = base + lane;
+        const int g = i < end ? group_of(ids, i, groups, nullptr) : -1;
+        const unsigned peers = __match_any_sync(kFull, g);
+        const int first = g >= 0 ? mine[g] : 0;
+        __syncwarp();
+        if (g >= 0 && lane == __ffs(peers) - 1) mine[g] = first + __popc(peers);
+        __syncwarp();
+        const int p = g >= 0 ? first + __popc(peers & ((1u << lane) - 1u)) : -1;
+        if (i < end) {
+            pos[i] = p;
+            if (p >= 0 && order) order[p] = i;
+        }
+    }
+    if (order)
+        for (long long p = rows + static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; p < pairs;
+             p += static_cast<long long>(gridDim.x) * blockDim.x)
+            order[p] = -1;
+}
+
+// ------------------------------------------------------------------ rows
+
+struct RouteArgs {
+    int tokens, topk, rows;
+    const int* __restrict__ pos;
+    int nvec;         // vectors of a row
+    int chunks;       // blocks along a row
+    DeviceErrorRecord* err;
+};
+
+// The sorted row of a pair, -1 for none.
+__device__ __forceinline__ int row_of(const RouteArgs& a, long long pair) {
+    const int p = __ldg(a.pos + pair);
+    if (p < -1 || p >= a.rows) record_device_error(a.err, SPMM_ERR_BAD_INDEX, pair);
+    return p < 0 || p >= a.rows ? -1 : p;
+}
+
+// Threads (tx along a row, ty tokens): tx the power of two that covers a row, at most `most`.
+dim3 row_block(int nvec, int most) {
+    int tx = 1;
+    while (tx < nvec && tx < most) tx *= 2;
+    return dim3(tx, std::max(1, 128 / tx));
+}
+
+// xs[pos[t, j]] = x[t]: a thread holds U vectors of the token's row and writes them to its topk places.
+template <int VB, int U>
+__global__ void __launch_bounds__(128) route_gather_kernel(RouteArgs a, const char* __restrict__ x, long long ldx,
+                                                           char* __restrict__ xs, long long ldxs) {
+    using V = typename VecOf<VB>::type;
+    grid_dependency_wait();
+    allow_dependent_launch();
+    const int chunk = blockIdx.x % a.chunks;
+    const long long t = static_cast<long long>(blockIdx.x / a.chunks) * blockDim.y + threadIdx.y;
+    if (t >= a.tokens) return;
+    const int v0 = chunk * blockDim.x * U + threadIdx.x;
+    V v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = v0 + u * blockDim.x;
+        if (c < a.nvec) v[u] = __ldg(reinterpret_cast<const V*>(x + t * ldx) + c);
+    }
+    for (int j = 0; j < a.topk; ++j) {
+        const int p = row_of(a, t * a.topk + j);
+        if (p < 0) continue;
+        V* dst = reinterpret_cast<V*>(xs + p * ldxs);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = v0 + u * blockDim.x;
+            if (c < a.nvec) dst[c] = v[u];
+        }
+    }
+}
+
+// y[t] = sum_j w[t, j] ys[pos[t, j]]: a thread sums one vector over the pairs, J loads in flight. FP32 FMA in the
+// order of j, as spmm_csr_f32 sums a row's nonzeros; one rounding at the end.
+template <int DT, int VB, int J>
+__global__ void __launch_bounds__(128) route_combine_kernel(RouteArgs a, const char* __restrict__ ys, long long ldys,
+                                                            const float* __restrict__ w, char* __restrict__ y, long long ldy) {
+    using R = RowVec<DT, VB>;
+    using V = typename R::V;
+    grid_dependency_wait();
+    allow_dependent_launch();
+    const int chunk = blockIdx.x % a.chunks;
+    const long long t = static_cast<long long>(blockIdx.x / a.chunks) * blockDim.y + threadIdx.y;
+    const int c = chunk * blockDim.x + threadIdx.x;
+    if (t >= a.tokens || c >= a.nvec) return;
+    float acc[R::N];
+#pragma unroll
+    for (int i = 0; i < R::N; ++i) acc[i] = 0.f;
+    for (int j0 = 0; j0 < a.topk; j0 += J) {
+        V v[J];
+        float wj[J];
+        int p[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            p[j] = -1;
+            if (j0 + j >= a.topk) continue;
+            const long long pair = t * a.topk + j0 + j;
+            p[j] = row_of(a, pair);
+            wj[j] = w ? __ldg(w + pair) : 1.f;
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (p[j] >= 0) v[j] = __ldg(reinterpret_cast<const V*>(ys + p[j] * ldys) + c);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (p[j] < 0) continue;
+            float f[R::N];
+            R::unpack(v[j], f);
+#pragma unroll
+            for (int i = 0; i < R::N; ++i) acc[i] = fmaf(wj[j], f[i], acc[i]);
+        }
+    }
+    reinterpret_cast<V*>(y + t * ldy)[c] = R::pack(acc);
+}
+
+// dys[pos[t, j]] = w[t, j] dy[t], dw[t, j] = <dy[t], ys[pos[t, j]]>: one block row (blockDim.x threads) takes a whole
+// token, J pairs at a time, so that a dot product is one tree in a fixed order and needs no second pass.
+template <int DT, int VB, int J>
+__global__ void __launch_bounds__(256)
+    route_combine_grad_kernel(RouteArgs a, const char* __restrict__ dy, long long lddy, const char* __restrict__ ys, long long ldys,
+                              const float* __restrict__ w, char* __restrict__ dys, long long lddys, float* __restrict__ dw) {
+    using R = RowVec<DT, VB>;
+    using V = typename R::V;
+    __shared__ float sums[8][J];  // [ty * warps along a row][J]; rows of one warp or less use shuffles only
+    grid_dependency_wait();
+    allow_dependent_launch();
+    const long long t = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const bool real = t < a.tokens;
+    const int tx = blockDim.x;
+    for (int j0 = 0; j0 < a.topk; j0 += J) {
+        int p[J];
+        float wj[J], dot[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            p[j] = -1;
+            dot[j] = 0.f;
+            wj[j] = 1.f;
+            if (!real || j0 + j >= a.topk) continue;
+            const long long pair = t * a.topk + j0 + j;
+            p[j] = row_of(a, pair);
+            if (w) wj[j] = __ldg(w + pair);
+        }
+        if (real) {
+            for (int c = threadIdx.x; c < a.nvec; c += tx) {
+                const V dv = __ldg(reinterpret_cast<const V*>(dy + t * lddy) + c);
+                V v[J];
+                if (dw) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+                        if (p[j] >= 0) v[j] = __ldg(reinterpret_cast<const V*>(ys + p[j] * ldys) + c);
+                }
+                float g[R::N];
+                R::unpack(dv, g);
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    if (p[j] < 0) continue;
+                    if (dys) {
+                        float o[R::N];
+#pragma unroll
+                        for (int i = 0; i < R::N; ++i) o[i] = wj[j] * g[i];
+                        reinterpret_cast<V*>(dys + p[j] * lddys)[c] = R::pack(o);
+                    }
+                    if (dw) {
+                        float f[R::N];
+                        R::unpack(v[j], f);
+#pragma unroll
+                        for (int i = 0; i < R::N; ++i) dot[j] = fmaf(g[i], f[i], dot[j]);
+                    }
+                }
+            }
+        }
+        if (!dw) continue;
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            for (int d = min(tx, 32) / 2; d > 0; d /= 2) dot[j] += __shfl_xor_sync(kFull, dot[j], d);
+        if (tx <= 32) {
+            if (real && threadIdx.x == 0) {
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    if (j0 + j < a.topk) dw[t * a.topk + j0 + j] = dot[j];
+            }
+        } else {
+            const int warps = tx / 32;  // along a row
+            const int slot = threadIdx.y * warps + threadIdx.x / 32;
+            __syncthreads();
+            if (threadIdx.x % 32 == 0) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) sums[slot][j] = dot[j];
+            }
+            __syncthreads();
+            if (real && threadIdx.x < J && j0 + static_cast<int>(threadIdx.x) < a.topk) {
+                float s = 0.f;
+                for (int k = 0; k < warps; ++k) s += sums[threadIdx.y * warps + k][threadIdx.x];
+                dw[t * a.topk + j0 + threadIdx.x] = s;
+            }
+        }
+    }
+}
+
+int route_args(const spmm_route_view* r, int32_t H, int32_t dtype) {
+    if (!r || r->tokens < 0 || r->topk < 1 || r->rows < 0 || H < 0) return SPMM_ERR_INVALID_ARG;
+    if (dtype != SPMM_DTYPE_F16 && dtype != SPMM_DTYPE_BF16 && dtype != SPMM_DTYPE_F32) return SPMM_ERR_INVALID_ARG;
+    if (r->tokens > 0 && !r->pos) return SPMM_ERR_INVALID_ARG;
+    if (static_cast<int64_t>(r->tokens) * r->topk > INT32_MAX - 4095) return SPMM_ERR_TOO_LARGE;
+    return SPMM_OK;
+}
+
+// An operand of `rows` rows: there when it has any, stride at least its length, elements on their own boundaries.
+int check_rows(const void* p, int64_t ld, int32_t rows, int32_t H, int32_t dtype) {
+    if (rows == 0 || H == 0) return SPMM_OK;
+    if (!p || ld < H || ld > (INT64_C(1) << 40)) return SPMM_ERR_INVALID_ARG;
+    return reinterpret_cast<uintptr_t>(p) % dtype_bytes(dtype) ? SPMM_ERR_MISALIGNED : SPMM_OK;
+}
+
+RouteArgs make_args(const spmm_route_view* r, int32_t H, int32_t dtype, int vb, DeviceState* st) {
+    RouteArgs a{};
+    a.tokens = r->tokens;
+    a.topk = r->topk;
+    a.rows = r->rows;
+    a.pos = r->pos;
+    a.nvec = static_cast<int>(static_cast<int64_t>(H) * dtype_bytes(dtype) / vb);
+    a.err = st->err;
+    return a;
+}
+
+// Blocks of a launch over tokens x chunks.
+int row_grid(const RouteArgs& a, dim3 block, unsigned* grid) {
+    const int64_t n = (static_cast<int64_t>(a.tokens) + block.y - 1) / block.y * a.chunks;
+    if (n > INT32_MAX) return SPMM_ERR_TOO_LARGE;
+    *grid = static_cast<unsigned>(n);
+    return SPMM_OK;
+}
+
+template <int VB>
+int gather_launch(RouteArgs a, const void* x, int64_t ldx, void* xs, int64_t ldxs, cudaStream_t s) {
+    constexpr int U = 4;
+    const dim3 block = row_block(a.nvec, 128);
+    a.chunks = (a.nvec + block.x * U - 1) / (block.x * U);
+    unsigned grid = 0;
+    SPMM_TRY(row_grid(a, block, &grid));
+    return launch_dependent(route_gather_kernel<VB, U>, dim3(grid), block, 0, s, a, static_cast<const char*>(x),
+                            static_cast<long long>(ldx), static_cast<char*>(xs), static_cast<long long>(ldxs));
+}
+
+template <int DT, int VB>
+int combine_launch(RouteArgs a, const void* ys, int64_t ldys, const float* w, void* y, int64_t ldy, cudaStream_t s) {
+    const dim3 block = row_block(a.nvec, 128);
+    a.chunks = (a.nvec + block.x - 1) / block.x;
+    unsigned grid = 0;
+    SPMM_TRY(row_grid(a, block, &grid));
+    return launch_dependent(route_combine_kernel<DT, VB, 8>, dim3(grid), block, 0, s, a, static_cast<const char*>(ys),
+                            static_cast<long long>(ldys), w, static_cast<char*>(y), static_cast<long long>(ldy));
+}
+
+template <int DT, int VB>
+int combine_grad_launch(RouteArgs a, const void* dy, int64_t lddy, const void* ys, int64_t ldys, const float* w, void* dys,
+                        int64_t lddys, float* dw, cudaStream_t s) {
+    const dim3 block = row_block(a.nvec, 256);
+    a.chunks = 1;
+    unsigned grid = 0;
+    SPMM_TRY(row_grid(a, block, &grid));
+    return launch_dependent(route_combine_grad_kernel<DT, VB, 8>, dim3(grid), block, 0, s, a, static_cast<const char*>(dy),
+                            static_cast<long long>(lddy), static_cast<const char*>(ys), static_cast<long long>(ldys), w,
+                            static_cast<char*>(dys), static_cast<long long>(lddys), dw);
+}
+
+#define SPMM_ROUTE_DISPATCH(fn, ...)                                                     \
+    switch (dtype * 32 + vb) {                                                           \
+        case SPMM_DTYPE_F16 * 32 + 16: return fn<SPMM_DTYPE_F16, 16>(__VA_ARGS__);       \
+        case SPMM_DTYPE_F16 * 32 + 4: return fn<SPMM_DTYPE_F16, 4>(__VA_ARGS__);         \
+        case SPMM_DTYPE_F16 * 32 + 2: return fn<SPMM_DTYPE_F16, 2>(__VA_ARGS__);         \
+        case SPMM_DTYPE_BF16 * 32 + 16: return fn<SPMM_DTYPE_BF16, 16>(__VA_ARGS__);     \
+        case SPMM_DTYPE_BF16 * 32 + 4: return fn<SPMM_DTYPE_BF16, 4>(__VA_ARGS__);       \
+        case SPMM_DTYPE_BF16 * 32 + 2: return fn<SPMM_DTYPE_BF16, 2>(__VA_ARGS__);       \
+        case SPMM_DTYPE_F32 * 32 + 16: return fn<SPMM_DTYPE_F32, 16>(__VA_ARGS__);       \
+        default: return fn<SPMM_DTYPE_F32, 4>(__VA_ARGS__);                              \
+    }
+
+}  // namespace
+}  // namespace spmm_b200
+
+using namespace spmm_b200;
+
+extern "C" {
+
+int spmm_route_workspace_size(int32_t tokens, int32_t topk, int32_t groups, size_t* bytes) {
+    if (!bytes || tokens < 0 || topk < 1 || groups < 1) return SPMM_ERR_INVALID_ARG;
+    const int64_t pairs = static_cast<int64_t>(tokens) * topk;
+    if (groups > SPMM_MAX_GROUPS || pairs > INT32_MAX - 4095) return SPMM_ERR_TOO_LARGE;
+    const SortShape h = sort_shape(static_cast<int>(pairs), groups);
+    *bytes = h.blocks == 1 ? 0 : sizeof(int) * static_cast<size_t>(h.blocks) * groups;
+    return SPMM_OK;
+}
+
+int spmm_route_build(const int32_t* ids, int32_t tokens, int32_t topk, int32_t groups, int32_t* offsets, int32_t* order,
+                     int32_t* pos, void* ws, size_t ws_bytes, void* stream) {
+    size_t need = 0;
+    SPMM_TRY(spmm_route_workspace_size(tokens, topk, groups, &need));
+    if (!offsets || (tokens > 0 && (!ids || !pos)) || (need > 0 && (!ws || ws_bytes < need))) return SPMM_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(ws) % 4) return SPMM_ERR_MISALIGNED;
+    DeviceState* st = nullptr;
+    SPMM_TRY(current_device_state(&st));
+    const cudaStream_t s = as_stream(stream);
+    const int pairs = tokens * topk;
+    const SortShape h = sort_shape(pairs, groups);
+    if (h.smem > 48 * 1024)
+        SPMM_CUDA_TRY(cudaFuncSetAttribute(route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(h.smem)));
+    int* counts = static_cast<int*>(ws);
+    if (h.blocks > 1)
+        SPMM_TRY(launch_dependent(route_count_kernel, dim3(h.blocks), dim3(kSortThreads), sizeof(int) * groups, s, ids, pairs, groups,
+                                  h.per_block, counts, st->err));
+    return launch_dependent(route_place_kernel, dim3(h.blocks), dim3(kSortThreads), h.smem, s, ids, pairs, groups, h.warps, h.per_block,
+                            counts, offsets, order, pos, st->err);
+}
+
+int spmm_route_gather(const spmm_route_view* r, const void* x, int64_t ldx, void* xs, int64_t ldxs, int32_t H, int32_t dtype,
+                      void* stream) {
+    SPMM_TRY(route_args(r, H, dtype));
+    SPMM_TRY(check_rows(x, ldx, r->tokens, H, dtype));
+    SPMM_TRY(check_rows(xs, ldxs, r->rows, H, dtype));
+    DeviceState* st = nullptr;
+    SPMM_TRY(current_device_state(&st));
+    if (r->tokens == 0 || r->rows == 0 || H == 0) return SPMM_OK;
+    const int e = dtype_bytes(dtype);
+    RowAlign al;
+    al.add(x, ldx * e);
+    al.add(xs, ldxs * e);
+    al.add(nullptr, static_cast<int64_t>(H) * e);
+    const int vb = al.vector_bytes();
+    const RouteArgs a = make_args(r, H, dtype, vb, st);
+    if (vb == 16) return gather_launch<16>(a, x, ldx * e, xs, ldxs * e, as_stream(stream));
+    if (vb == 4) return gather_launch<4>(a, x, ldx * e, xs, ldxs * e, as_stream(stream));
+    return gather_launch<2>(a, x, ldx * e, xs, ldxs * e, as_stream(stream));
+}
+
+int spmm_route_combine(const spmm_route_view* r, const void* ys, int64_t ldys, const float* w, void* y, int64_t ldy, int32_t H,
+                       int32_t dtype, void* stream) {
+    SPMM_TRY(route_args(r, H, dtype));
+    SPMM_TRY(check_rows(ys, ldys, r->rows, H, dtype));
+    SPMM_TRY(check_rows(y, ldy, r->tokens, H, dtype));
+    if (reinterpret_cast<uintptr_t>(w) % 4) return SPMM_ERR_MISALIGNED;
+    DeviceState* st = nullptr;
+    SPMM_TRY(current_device_state(&st));
+    if (r->tokens == 0 || H == 0) return SPMM_OK;
+    const int e = dtype_bytes(dtype);
+    RowAlign al;
+    if (r->rows > 0) al.add(ys, ldys * e);
+    al.add(y, ldy * e);
+    al.add(nullptr, static_cast<int64_t>(H) * e);
+    const int vb = al.vector_bytes();
+    const RouteArgs a = make_args(r, H, dtype, vb, st);
+    SPMM_ROUTE_DISPATCH(combine_launch, a, ys, ldys * e, w, y, ldy * e, as_stream(stream))
+}
+
+int spmm_route_combine_grad(const spmm_route_view* r, const void* dy, int64_t lddy, const void* ys, int64_t ldys, const float* w,
+                            void* dys, int64_t lddys, float* dw, int32_t H, int32_t dtype, void* stream) {
+    SPMM_TRY(route_args(r, H, dtype));
+    if (!dys && !dw) return SPMM_ERR_INVALID_ARG;
+    SPMM_TRY(check_rows(dy, lddy, r->tokens, H, dtype));
+    if (dw) SPMM_TRY(check_rows(ys, ldys, r->rows, H, dtype));
+    if (dys) SPMM_TRY(check_rows(dys, lddys, r->rows, H, dtype));
+    if (reinterpret_cast<uintptr_t>(w) % 4 || reinterpret_cast<uintptr_t>(dw) % 4) return SPMM_ERR_MISALIGNED;
+    DeviceState* st = nullptr;
+    SPMM_TRY(current_device_state(&st));
+    if (r->tokens == 0 || (H == 0 && !dw)) return SPMM_OK;
+    const int e = dtype_bytes(dtype);
+    RowAlign al;
+    if (H > 0) al.add(dy, lddy * e);
+    if (H > 0 && r->rows > 0 && dw) al.add(ys, ldys * e);
+    if (H > 0 && r->rows > 0 && dys) al.add(dys, lddys * e);
+    al.add(nullptr, static_cast<int64_t>(H) * e);
+    const int vb = al.vector_bytes();
+    const RouteArgs a = make_args(r, H, dtype, vb, st);
+    SPMM_ROUTE_DISPATCH(combine_grad_launch, a, dy, lddy * e, ys, ldys * e, w, dys, lddys * e, dw, as_stream(stream))
+}
+
+}  // extern "C"

@@ -24,7 +24,7 @@ ERR = {
     -9: "SPMM_ERR_IO", -10: "SPMM_ERR_TOO_LARGE",
 }
 CSR_AUTO, CSR_ROWWARP, CSR_MERGE = 0, 1, 2
-DTYPE_F16, DTYPE_BF16 = 0, 1
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 BACKEND_CSR, BACKEND_TC = 0, 1
 
 # Every symbol include/spmm_c.h declares (checked by the CPU test suite).
@@ -45,6 +45,9 @@ EXPORTS = [
     "spmm_rank_plan_create", "spmm_rank_plan_info", "spmm_rank_run", "spmm_rank_submit", "spmm_rank_wait",
     "spmm_rank_execute", "spmm_rank_gather_b",
     "spmm_rank_plan_buffers", "spmm_rank_plan_destroy",
+    "spmm_route_workspace_size", "spmm_route_build", "spmm_route_gather", "spmm_route_combine",
+    "spmm_route_combine_grad", "spmm_grouped_mm", "spmm_grouped_mm_dx", "spmm_grouped_mm_dw",
+    "spmm_lora_workspace_size", "spmm_lora",
 ]
 
 
@@ -90,6 +93,15 @@ class CsrTuning(C.Structure):
 class HybridPlan(C.Structure):
     _fields_ = [("backend", C.c_int32), ("fill_in_ratio", C.c_double), ("block_density", C.c_double),
                 ("threshold", C.c_float), ("n_aligned", C.c_int32), ("reason", C.c_char_p)]
+
+
+class RouteView(C.Structure):
+    _fields_ = [("tokens", C.c_int32), ("topk", C.c_int32), ("rows", C.c_int32), ("pos", C.c_void_p)]
+
+
+class LoraView(C.Structure):
+    _fields_ = [("adapters", C.c_int32), ("rank", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("dtype", C.c_int32),
+                ("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p)]
 
 
 _lib: C.CDLL | None = None
@@ -172,6 +184,16 @@ def lib() -> C.CDLL:
         "spmm_rank_gather_b": (C.c_int, [vp, vp]),
         "spmm_rank_plan_buffers": (C.c_int, [vp, C.POINTER(vp), C.POINTER(vp)]),
         "spmm_rank_plan_destroy": (None, [vp]),
+        "spmm_route_workspace_size": (C.c_int, [i32, i32, i32, C.POINTER(C.c_size_t)]),
+        "spmm_route_build": (C.c_int, [vp, i32, i32, i32, vp, vp, vp, vp, C.c_size_t, vp]),
+        "spmm_route_gather": (C.c_int, [C.POINTER(RouteView), vp, i64, vp, i64, i32, i32, vp]),
+        "spmm_route_combine": (C.c_int, [C.POINTER(RouteView), vp, i64, vp, vp, i64, i32, i32, vp]),
+        "spmm_route_combine_grad": (C.c_int, [C.POINTER(RouteView), vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, vp]),
+        "spmm_grouped_mm": (C.c_int, [vp, i32, i32, vp, i64, vp, vp, i64, i32, i32, i32, i32, vp]),
+        "spmm_grouped_mm_dx": (C.c_int, [vp, i32, i32, vp, i64, vp, vp, i64, i32, i32, i32, i32, vp]),
+        "spmm_grouped_mm_dw": (C.c_int, [vp, i32, i32, vp, i64, vp, i64, vp, i32, i32, i32, i32, vp]),
+        "spmm_lora_workspace_size": (C.c_int, [C.POINTER(LoraView), i32, i32, C.POINTER(C.c_size_t)]),
+        "spmm_lora": (C.c_int, [C.POINTER(LoraView), vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp, C.c_size_t, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -639,3 +661,214 @@ class RankPlan:
             self.close()
         except Exception:  # noqa: BLE001 - interpreter shutdown
             pass
+
+
+# ------------------------------------------------------------------ rows grouped by an index
+#
+# Routing to experts and back, the experts' products, low-rank adapters (include/spmm_c.h says what each computes).
+# Operands are torch tensors on the current CUDA device: rows may be strided, the elements of a row may not; index
+# tensors (int32), weights (float32) and matrices are contiguous. Outputs are the caller's. A tensor of another
+# type, shape or device raises ValueError, a refusal of the library SpmmError. `stream`: None is the legacy default
+# stream, as everywhere here.
+
+_DTYPES: dict = {}
+
+
+def _dtypes() -> dict:
+    if not _DTYPES:
+        import torch
+
+        _DTYPES.update({torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32})
+    return _DTYPES
+
+
+def _here() -> int:
+    import torch
+
+    return torch.cuda.current_device() if torch.cuda.is_available() else -1
+
+
+def _rows(t, what: str, shape: tuple, dtype) -> int:
+    """Row stride of a (rows, columns) tensor whose rows are contiguous."""
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_cuda or t.device.index != _here():
+        raise ValueError(f"{what}: want {shape} {dtype} on cuda:{_here()}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    ld, step = t.stride()
+    if (step != 1 and shape[1] > 1) or (shape[0] > 1 and ld < shape[1]):
+        raise ValueError(f"{what}: the elements of a row must be adjacent and rows must not overlap, got strides {t.stride()}")
+    return max(ld, shape[1])
+
+
+def _flat(t, what: str, shape: tuple, dtype) -> int:
+    """Address of a contiguous tensor (0 for None)."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_cuda or t.device.index != _here() or not t.is_contiguous():
+        raise ValueError(f"{what}: want contiguous {shape} {dtype} on cuda:{_here()}, got {tuple(t.shape)} {t.dtype} "
+                         f"strides {t.stride()} on {t.device}")
+    return t.data_ptr()
+
+
+def _value_dtype(t, what: str, allowed=(DTYPE_F16, DTYPE_BF16)) -> int:
+    dt = _dtypes().get(t.dtype)
+    if dt not in allowed:
+        raise ValueError(f"{what}: unsupported type {t.dtype}")
+    return dt
+
+
+def _workspace(ws, need: int, stream):
+    """(tensor that owns the workspace, address, bytes). Without one from the caller, memory of torch's allocator in the
+    order of `stream`: reused by a later allocation only behind this call's kernels, also under graph capture."""
+    if need == 0:
+        return None, 0, 0
+    if ws is not None:
+        if not ws.is_cuda or ws.device.index != _here() or not ws.is_contiguous():
+            raise ValueError("ws: want a contiguous CUDA tensor on the current device")
+        return ws, ws.data_ptr(), ws.numel() * ws.element_size()
+    import torch
+
+    sp = stream_ptr(stream)
+    if sp == torch.cuda.current_stream().cuda_stream:
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    else:
+        with torch.cuda.stream(torch.cuda.ExternalStream(sp) if sp else torch.cuda.default_stream()):
+            ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    return ws, ws.data_ptr(), need
+
+
+def route_workspace_size(tokens: int, topk: int, groups: int) -> int:
+    n = C.c_size_t()
+    check(lib().spmm_route_workspace_size(tokens, topk, groups, C.byref(n)), "spmm_route_workspace_size")
+    return int(n.value)
+
+
+def route_build(ids, groups: int, offsets, order, pos, ws=None, stream=None) -> None:
+    """Sort the pairs of ids (tokens, topk) by group: offsets (groups + 1), order (tokens * topk, or None), pos (tokens, topk)."""
+    import torch
+
+    tokens, topk = ids.shape
+    need = route_workspace_size(tokens, topk, groups)
+    _ws, wp, wn = _workspace(ws, need, stream)
+    check(lib().spmm_route_build(_flat(ids, "ids", (tokens, topk), torch.int32), tokens, topk, groups,
+                                 _flat(offsets, "offsets", (groups + 1,), torch.int32),
+                                 _flat(order, "order", (tokens * topk,), torch.int32),
+                                 _flat(pos, "pos", (tokens, topk), torch.int32), wp, wn, stream_ptr(stream)), "spmm_route_build")
+
+
+def _route_view(pos, rows: int) -> RouteView:
+    import torch
+
+    tokens, topk = pos.shape
+    return RouteView(tokens, topk, rows, _flat(pos, "pos", (tokens, topk), torch.int32))
+
+
+def route_gather(pos, x, xs, stream=None) -> None:
+    """xs[pos[t, j]] = x[t] (rows of xs without a pair stay as they are)."""
+    rows, H = xs.shape
+    dt = _value_dtype(x, "x", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
+    v = _route_view(pos, rows)
+    check(lib().spmm_route_gather(C.byref(v), x.data_ptr(), _rows(x, "x", (v.tokens, H), x.dtype), xs.data_ptr(),
+                                  _rows(xs, "xs", (rows, H), x.dtype), H, dt, stream_ptr(stream)), "spmm_route_gather")
+
+
+def route_combine(pos, ys, y, w=None, stream=None) -> None:
+    """y[t] = sum_j w[t, j] ys[pos[t, j]] (w None: all 1, the gradient of route_gather)."""
+    import torch
+
+    rows, H = ys.shape
+    dt = _value_dtype(ys, "ys", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
+    v = _route_view(pos, rows)
+    check(lib().spmm_route_combine(C.byref(v), ys.data_ptr(), _rows(ys, "ys", (rows, H), ys.dtype),
+                                   _flat(w, "w", (v.tokens, v.topk), torch.float32), y.data_ptr(),
+                                   _rows(y, "y", (v.tokens, H), ys.dtype), H, dt, stream_ptr(stream)), "spmm_route_combine")
+
+
+def route_combine_grad(pos, dy, ys=None, w=None, dys=None, dw=None, stream=None) -> None:
+    """Gradients of route_combine: dys[pos[t, j]] = w[t, j] dy[t] and dw[t, j] = <dy[t], ys[pos[t, j]]>; either may be left out
+    (None; ys is needed for dw only)."""
+    import torch
+
+    H = dy.shape[1]
+    dt = _value_dtype(dy, "dy", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
+    if dys is None and dw is None:
+        raise ValueError("route_combine_grad: neither dys nor dw is wanted")
+    if dw is not None and ys is None:
+        raise ValueError("route_combine_grad: dw needs ys")
+    if dw is not None and dys is not None and ys.shape[0] != dys.shape[0]:
+        raise ValueError("route_combine_grad: ys and dys must have the same rows")
+    ys = ys if dw is not None else None
+    rows = (dys if dys is not None else ys).shape[0]
+    v = _route_view(pos, rows)
+    check(lib().spmm_route_combine_grad(
+        C.byref(v), dy.data_ptr(), _rows(dy, "dy", (v.tokens, H), dy.dtype), ptr(ys),
+        _rows(ys, "ys", (rows, H), dy.dtype) if ys is not None else 0, _flat(w, "w", (v.tokens, v.topk), torch.float32), ptr(dys),
+        _rows(dys, "dys", (rows, H), dy.dtype) if dys is not None else 0, _flat(dw, "dw", (v.tokens, v.topk), torch.float32), H, dt,
+        stream_ptr(stream)), "spmm_route_combine_grad")
+
+
+def grouped_mm(offsets, x, w, y, stream=None) -> None:
+    """y[p] = w[g] x[p] for offsets[g] <= p < offsets[g + 1]; x (rows, K), w (groups, N, K), y (rows, N) of x's type or float32."""
+    import torch
+
+    groups, N, K = w.shape
+    rows = x.shape[0]
+    dt, odt = _value_dtype(x, "x"), _value_dtype(y, "y", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
+    check(lib().spmm_grouped_mm(_flat(offsets, "offsets", (groups + 1,), torch.int32), groups, rows, x.data_ptr(),
+                                _rows(x, "x", (rows, K), x.dtype), _flat(w, "w", (groups, N, K), x.dtype), y.data_ptr(),
+                                _rows(y, "y", (rows, N), y.dtype), N, K, dt, odt, stream_ptr(stream)), "spmm_grouped_mm")
+
+
+def grouped_mm_dx(offsets, dy, w, dx, stream=None) -> None:
+    """dx[p] = w[g]^T dy[p]; dy (rows, N), w (groups, N, K), dx (rows, K) of dy's type or float32."""
+    import torch
+
+    groups, N, K = w.shape
+    rows = dy.shape[0]
+    dt, odt = _value_dtype(dy, "dy"), _value_dtype(dx, "dx", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
+    check(lib().spmm_grouped_mm_dx(_flat(offsets, "offsets", (groups + 1,), torch.int32), groups, rows, dy.data_ptr(),
+                                   _rows(dy, "dy", (rows, N), dy.dtype), _flat(w, "w", (groups, N, K), dy.dtype), dx.data_ptr(),
+                                   _rows(dx, "dx", (rows, K), dx.dtype), N, K, dt, odt, stream_ptr(stream)), "spmm_grouped_mm_dx")
+
+
+def grouped_mm_dw(offsets, dy, x, dw, stream=None) -> None:
+    """dw[g] = sum over the group's rows of dy[p] x[p]^T; dw (groups, N, K) of x's type or float32."""
+    import torch
+
+    groups, N, K = dw.shape
+    rows = x.shape[0]
+    dt, odt = _value_dtype(x, "x"), _value_dtype(dw, "dw", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
+    check(lib().spmm_grouped_mm_dw(_flat(offsets, "offsets", (groups + 1,), torch.int32), groups, rows, dy.data_ptr(),
+                                   _rows(dy, "dy", (rows, N), x.dtype), x.data_ptr(), _rows(x, "x", (rows, K), x.dtype),
+                                   _flat(dw, "dw", (groups, N, K), dw.dtype), N, K, dt, odt, stream_ptr(stream)), "spmm_grouped_mm_dw")
+
+
+def _lora_view(a, b, scale) -> LoraView:
+    import torch
+
+    adapters, rank, K = a.shape
+    N = b.shape[1]
+    dt = _value_dtype(a, "a")
+    return LoraView(adapters, rank, N, K, dt, _flat(a, "a", (adapters, rank, K), a.dtype), _flat(b, "b", (adapters, N, rank), a.dtype),
+                    _flat(scale, "scale", (adapters,), torch.float32))
+
+
+def lora_workspace_size(a, b, requests: int, rows: int) -> int:
+    v = _lora_view(a, b, None)
+    n = C.c_size_t()
+    check(lib().spmm_lora_workspace_size(C.byref(v), requests, rows, C.byref(n)), "spmm_lora_workspace_size")
+    return int(n.value)
+
+
+def lora(offsets, adapter, x, a, b, out, base=None, scale=None, ws=None, stream=None) -> None:
+    """out[p] = base[p] + scale * b (a x[p]) with the matrices of adapter[r], offsets[r] <= p < offsets[r + 1] (offsets None: every
+    row a request of its own); x (rows, K), a (adapters, rank, K), b (adapters, N, rank), base and out (rows, N)."""
+    import torch
+
+    v = _lora_view(a, b, scale)
+    rows, requests = x.shape[0], adapter.shape[0]
+    n = C.c_size_t()
+    check(lib().spmm_lora_workspace_size(C.byref(v), requests, rows, C.byref(n)), "spmm_lora_workspace_size")
+    _ws, wp, wn = _workspace(ws, int(n.value), stream)
+    check(lib().spmm_lora(C.byref(v), _flat(offsets, "offsets", (requests + 1,), torch.int32),
+                          _flat(adapter, "adapter", (requests,), torch.int32), requests, rows, x.data_ptr(),
+                          _rows(x, "x", (rows, v.K), a.dtype), ptr(base), _rows(base, "base", (rows, v.N), a.dtype) if base is not None else 0,
+                          out.data_ptr(), _rows(out, "out", (rows, v.N), a.dtype), wp, wn, stream_ptr(stream)), "spmm_lora")
