@@ -42,7 +42,7 @@
 #include <new>
 #include <vector>
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 // A BSR-16 plan: the view, the tile group size, the per-CTA schedule (device memory, NULL when
 // the schedule would be too large or the tensor-core path does not apply) and A's tensor map.
@@ -76,7 +76,6 @@ constexpr int kTcThreads = 192;       // warp 0 TMA, warp 1 MMA + TMEM, warps 2.
 constexpr unsigned kFullMask = 0xffffffffu;
 constexpr int kDone = -1;
 constexpr uint32_t kFullArrivals = 1;  // the lane that claims the stage (arrive + expect_tx)
-constexpr unsigned long long kWaitNs = 500ull * 1000 * 1000;  // 0.5 s per wait
 
 struct BsrArgs {
     int M, K, N;
@@ -125,148 +124,8 @@ struct Layout {
     static constexpr int kDynamic = kBytes + 1024;         // room to align the base to 1 KB
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ unsigned long long global_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// Non-blocking test of a phase.
-__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// Bounded wait, slow path: polls with the abort flag and the clock checked every 64 polls
-// (the clock is read only once a wait has lasted that long: a %globaltimer read costs
-// hundreds of nanoseconds, which at one read per wait dominated the producer's step time).
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    unsigned long long t0 = 0;
-    for (uint32_t it = 0; it < (1u << 26); ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63) == 63) {
-            if (*abort_flag) return false;
-            const unsigned long long t = global_ns();
-            if (t0 == 0) t0 = t;
-            else if (t - t0 > kWaitNs) return false;
-        }
-    }
-    return false;
-}
-
-// Bounded wait: true when the phase completed; false on timeout or when another role of the
-// CTA has already given up (abort flag). One poll inline, the rest out of line.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    if (mbar_try_wait(bar, parity)) return true;
-    return mbar_wait_slow(bar, parity, abort_flag);
-}
-
-__device__ __forceinline__ void mbar_arrive_count(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z,
-                                            int w) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(ncols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
-        : "memory");
-}
-
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-        "[%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor (tcgen05 "version 1" format): start address, leading and
-// stride byte offsets (16-byte units), swizzle mode in bits 61..63.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, uint64_t swizzle) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr & 0x3ffffu) >> 4);
-    d |= static_cast<uint64_t>((lbo >> 4) & 0x3fffu) << 16;
-    d |= static_cast<uint64_t>((sbo >> 4) & 0x3fffu) << 32;
-    d |= 1ull << 46;
-    d |= swizzle << 61;
-    return d;
-}
-
-constexpr uint64_t kSwizzle128 = 2;
-constexpr uint64_t kSwizzle32 = 6;
-
-// Instruction descriptor for kind::f16: D = F32, A and B the same 16-bit type, A MN-major,
-// B K-major, M = 128, N = n (16 .. 256, a multiple of 16).
-__device__ __forceinline__ uint32_t instr_desc(int dtype, uint32_t n) {
-    const uint32_t fmt = dtype == SPMM_DTYPE_BF16 ? 1u : 0u;
-    return (1u << 4) | (fmt << 7) | (fmt << 10) | (1u << 15) | (0u << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
-}
+// The MMA's A (the B tile) is MN-major, its B (the blocks) K-major, M = 128, N = n (16 .. 256, a multiple of 16).
+__device__ __forceinline__ uint32_t instr_desc(int dtype, uint32_t n) { return instr_desc_f16(dtype, n, true, false); }
 
 template <int G, bool SCHED>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -611,34 +470,6 @@ __global__ void __launch_bounds__(128) bsr_cudacore_kernel(BsrArgs a) {
             if (row < a.M) a.C[static_cast<size_t>(row) * a.N + n] = acc[r];
         }
     }
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-        cudaGetLastError();
-    });
-    return fn;
-}
-
-int encode_2d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t outer, uint64_t row_bytes, uint32_t box_inner,
-              uint32_t box_outer, CUtensorMapSwizzle swz) {
-    auto enc = tensor_map_encoder();
-    if (!enc) return SPMM_ERR_UNSUPPORTED;
-    const cuuint64_t dims[2] = {inner, outer};
-    const cuuint64_t strides[1] = {row_bytes};
-    const cuuint32_t box[2] = {box_inner, box_outer};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(ptr), dims, strides, box, estr,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? SPMM_OK : SPMM_ERR_INVALID_ARG;
 }
 
 int encode_b_map(CUtensorMap* tb, const BsrArgs& a) {

@@ -8,10 +8,12 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstdint>
 
 #include "groups.cuh"
+#include "tcgen05.cuh"
 
 namespace spmm_b200 {
 namespace {
@@ -135,6 +137,391 @@ int any_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st)
     return launch_dependent(grouped_any_kernel<FORM, SPMM_DTYPE_F16>, dim3(grid), dim3(256), smem, s, a);
 }
 
+// ------------------------------------------------------------------ tcgen05
+//
+// A persistent block takes 128 x TN tiles of D, 64 of k a step: one warp issues TMA copies into a ring of stages, one
+// issues the MMAs (M = 128, N = TN, FP32 accumulators in TMEM, two of them so that the next tile's MMAs run under this
+// one's epilogue), four move TMEM -> registers -> shared memory -> 16-byte stores of whole 128-byte row pieces.
+// x, dy and w are read as they lie: K-major where k is the contiguous index (both operands of the forward product,
+// dx's A), MN-major where it is not (dx's B, both of dw's), so nothing is transposed in memory.
+// Ragged groups: a row tile may reach past its group. Rows of D past it are computed and not stored (rows do not mix
+// in the MMA); in dw, where rows are summed, the last step issues only the MMAs that hold rows of the group (16 rows
+// each) and the up to 15 rows past it are cleared in shared memory first, A's and B's, so NaN there cannot get in.
+
+constexpr int kTileM = 128;
+constexpr int kStepK = 64;
+constexpr int kBand = 8;          // row tiles that run together down a band (their A and the band's B stay in L2)
+constexpr int kTcThreads = 192;   // warp 0 TMA, warp 1 MMA, warps 2..5 epilogue
+constexpr int kSmallRows = 32;    // groups with no more rows left load a box of this many
+
+template <int TN>
+struct TcLayout {
+    static constexpr int kA = kTileM * kStepK * 2;
+    static constexpr int kB = TN * kStepK * 2;
+    static constexpr int kStage = kA + kB;
+    static constexpr int kStages = TN == 256 ? 4 : (TN == 128 ? 6 : 8);
+    static constexpr int kOut = kStages * kStage;    // 4 warps x 32 rows x 128 bytes
+    static constexpr int kBars = kOut + 4 * 4096;    // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
+    static constexpr int kTable = kBars + 8 * (2 * kStages + 5) + 16;
+    static constexpr int kFixed = kTable + 1024;     // room to align the base to 1 KB; then int[groups + 1]
+};
+
+struct TcArgs {
+    const int* __restrict__ offsets;
+    int groups, rows;
+    int outs;          // columns of D
+    int ms;            // dw: rows of D of each group
+    int sum;           // not dw: length of the sum
+    int mtiles;        // dw: row tiles of a group
+    int ntiles;
+    void* out;
+    long long ldo;     // row stride of out
+    int out_f32, dtype;
+    DeviceErrorRecord* err;
+};
+
+struct Tile {
+    int g, m0, n0;     // group, first row of D in the group, first column
+    int begin, end;    // the group's rows
+    int steps;         // k steps
+};
+
+template <int FORM, int TN>
+__device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, int t) {
+    Tile r;
+    int local, mtiles;
+    if constexpr (FORM == kDw) {
+        const int per = a.mtiles * a.ntiles;
+        r.g = t / per;
+        local = t - r.g * per;
+        mtiles = a.mtiles;
+    } else {
+        r.g = tile_group(start, a.groups, t / a.ntiles);
+        local = t - start[r.g] * a.ntiles;
+        mtiles = start[r.g + 1] - start[r.g];
+    }
+    const int band = local / (kBand * a.ntiles);
+    const int high = min(kBand, mtiles - band * kBand);
+    local -= band * kBand * a.ntiles;
+    r.m0 = (band * kBand + local % high) * kTileM;
+    r.n0 = local / high * TN;
+    const GroupRange range = group_range(a.offsets, r.g, a.rows, nullptr);
+    r.begin = range.begin;
+    r.end = range.end;
+    const int sum = FORM == kDw ? r.end - r.begin : a.sum;
+    r.steps = (sum + kStepK - 1) / kStepK;
+    return r;
+}
+
+template <int FORM, int TN>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    grouped_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_small,
+                      const __grid_constant__ CUtensorMap map_b, TcArgs a) {
+    using L = TcLayout<TN>;
+    constexpr int kStages = L::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_addr(smem_raw);
+    uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // 1 KB: the 128-byte swizzle's atoms
+    const uint32_t sbase = smem_addr(base);
+    const uint32_t full0 = sbase + L::kBars, empty0 = full0 + 8 * kStages, acc_full0 = empty0 + 8 * kStages, acc_empty0 = acc_full0 + 16,
+                   drain = acc_empty0 + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kBars + 8 * (2 * kStages + 5));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* start = reinterpret_cast<int*>(base + L::kTable);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(acc_full0 + 8 * s, 1);
+            mbar_init(acc_empty0 + 8 * s, 4);
+        }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_tensormap(&map_a);
+        prefetch_tensormap(&map_b);
+    }
+    if (warp == 1) tmem_alloc(smem_addr(tmem_slot), 2 * TN);
+    grid_dependency_wait();
+    allow_dependent_launch();
+    int tiles;
+    if constexpr (FORM == kDw) {
+        if (blockIdx.x == 0)
+            for (int g = threadIdx.x; g < a.groups; g += kTcThreads) group_range(a.offsets, g, a.rows, a.err);  // records bad ones
+        tiles = a.groups * a.mtiles * a.ntiles;
+    } else {
+        build_tile_table(start, a.offsets, a.groups, a.rows, kTileM, blockIdx.x == 0 ? a.err : nullptr);
+        tiles = start[a.groups] * a.ntiles;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        // ---------------- producer
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+                const Tile r = tile_of<FORM, TN>(a, start, t);
+                const bool small = FORM != kDw && r.end - r.begin - r.m0 <= kSmallRows;
+                // Boxes of 64 columns that lie wholly past the operand are not loaded; their part of D is not stored.
+                const int nb = min(TN / 64, (a.outs - r.n0 + 63) / 64);
+                const int na = min(2, (a.ms - r.m0 + 63) / 64);  // dw
+                const uint32_t bytes = (FORM == kDw ? na * 8192 : (small ? kSmallRows * 128 : L::kA)) + (FORM == kForward ? L::kB : nb * 8192);
+                for (int ks = 0; ks < r.steps; ++ks, ++it) {
+                    const int s = it % kStages;
+                    const uint32_t bar = full0 + 8 * s, sa = sbase + s * L::kStage, sb = sa + L::kA;
+                    if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_expect_tx(bar, bytes);
+                    const int k0 = ks * kStepK;
+                    if constexpr (FORM == kDw) {
+                        for (int j = 0; j < na; ++j) tma_load_2d(sa + j * 8192, &map_a, bar, r.m0 + 64 * j, r.begin + k0);
+                        for (int j = 0; j < nb; ++j) tma_load_2d(sb + j * 8192, &map_b, bar, r.n0 + 64 * j, r.begin + k0);
+                    } else {
+                        tma_load_2d(sa, small ? &map_a_small : &map_a, bar, k0, r.begin + r.m0);
+                        if constexpr (FORM == kForward) {
+                            tma_load_3d(sb, &map_b, bar, k0, r.n0, r.g);
+                        } else {
+                            for (int j = 0; j < nb; ++j) tma_load_3d(sb + j * 8192, &map_b, bar, r.n0 + 64 * j, k0, r.g);
+                        }
+                    }
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                record_device_error(a.err, SPMM_ERR_TIMEOUT, 11);
+            }
+            // The block's shared memory outlives every copy into it and every arrival on its barriers.
+            for (int i = max(0, it - kStages); i < it; ++i) {
+                const unsigned long long t0 = global_ns();
+                while (!mbar_try_wait(full0 + 8 * (i % kStages), (i / kStages) & 1u) && global_ns() - t0 < kWaitNs) {
+                }
+                if (ok) mbar_wait(empty0 + 8 * (i % kStages), (i / kStages) & 1u, abort_flag);
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (lane 0; the whole warp clears rows past a group's end in dw)
+        const uint32_t idesc = instr_desc_f16(a.dtype, TN, FORM == kDw, FORM != kForward);
+        int it = 0, n = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++n) {
+            const Tile r = tile_of<FORM, TN>(a, start, t);
+            const int buf = n & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * TN;
+            const int sum = FORM == kDw ? r.end - r.begin : a.sum;
+            for (int ks = 0; ks < r.steps; ++ks, ++it) {
+                const int s = it % kStages;
+                if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag))) {
+                    ok = false;
+                    break;
+                }
+                const int left = min(kStepK, sum - ks * kStepK), slices = (left + 15) / 16;
+                if constexpr (FORM == kDw) {
+                    if (left % 16) {
+                        const int nb = min(TN / 64, (a.outs - r.n0 + 63) / 64), na = min(2, (a.ms - r.m0 + 63) / 64);
+                        const int pieces = (slices * 16 - left) * 8;  // 16-byte pieces of a box's rows to clear
+                        uint8_t* st = base + s * L::kStage;
+                        for (int b = 0; b < na + nb; ++b) {
+                            uint4* rows = reinterpret_cast<uint4*>(st + (b < na ? b * 8192 : L::kA + (b - na) * 8192) + left * 128);
+                            for (int i = lane; i < pieces; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                }
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t sa = sbase + s * L::kStage, sb = sa + L::kA;
+                    for (int j = 0; j < slices; ++j) {
+                        const uint64_t da = FORM == kDw ? smem_desc(sa + 2048 * j, 8192, 1024, kSwizzle128)
+                                                        : smem_desc(sa + 32 * j, 16, 1024, kSwizzle128);
+                        const uint64_t db = FORM == kForward ? smem_desc(sb + 32 * j, 16, 1024, kSwizzle128)
+                                                             : smem_desc(sb + 2048 * j, 8192, 1024, kSwizzle128);
+                        umma_f16(acc, da, db, idesc, ks + j > 0 ? 1u : 0u);
+                    }
+                    umma_commit(empty0 + 8 * s);
+                }
+                __syncwarp();
+            }
+            if (lane == 0) umma_commit(acc_full0 + 8 * buf);
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_device_error(a.err, SPMM_ERR_TIMEOUT, 12);
+        }
+    } else {
+        // ---------------- epilogue
+        const int q = warp & 3;  // TMEM lane quarter this warp may access
+        uint8_t* stage = base + L::kOut + q * 4096;
+        const int size = a.out_f32 ? 4 : 2, per = 128 / size;  // columns of a 128-byte row piece
+        int n = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
+            const Tile r = tile_of<FORM, TN>(a, start, t);
+            const int buf = n & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * TN + (static_cast<uint32_t>(q * 32) << 16);
+            const int rows = min(32, (FORM == kDw ? a.ms : r.end - r.begin) - r.m0 - q * 32);
+            const long long first = FORM == kDw ? static_cast<long long>(r.g) * a.ms + r.m0 + q * 32 : r.begin + r.m0 + q * 32;
+            char* out = static_cast<char*>(a.out) + (first * a.ldo + r.n0) * size;
+            const int cols = min(TN, a.outs - r.n0);
+            if (rows > 0) {
+                for (int c0 = 0; c0 < cols; c0 += per) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (a.out_f32 && h) continue;
+                        uint32_t v[32];
+                        if (FORM == kDw && r.steps == 0) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = 0u;
+                        } else {
+                            tmem_ld32(acc + c0 + 32 * h, v);
+                        }
+                        if (a.out_f32) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+                                *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+                                    make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float lo = __uint_as_float(v[8 * c + 2 * i]), hi = __uint_as_float(v[8 * c + 2 * i + 1]);
+                                    w[i] = a.dtype == SPMM_DTYPE_BF16 ? pack_half2<SPMM_DTYPE_BF16>(lo, hi) : pack_half2<SPMM_DTYPE_F16>(lo, hi);
+                                }
+                                *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * h + c) ^ (lane & 7)) << 4)) =
+                                    make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    const int c = lane & 7, col = c0 + c * (16 / size);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int row = 4 * i + (lane >> 3);
+                        if (row < rows && col < cols)
+                            *reinterpret_cast<uint4*>(out + (row * a.ldo + col) * size) =
+                                *reinterpret_cast<const uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+                    }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_count(acc_empty0 + 8 * buf, 1);
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_device_error(a.err, SPMM_ERR_TIMEOUT, 13);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        if (*abort_flag) {
+            // MMAs still in flight end before their accumulators are given back.
+            if (lane == 0) {
+                umma_commit(drain);
+                const unsigned long long t0 = global_ns();
+                while (!mbar_try_wait(drain, 0) && global_ns() - t0 < kWaitNs) {
+                }
+            }
+            __syncwarp();
+        }
+        tmem_dealloc(tmem, 2 * TN);
+    }
+}
+
+template <int FORM, int TN>
+int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap& mb, const TcArgs& a, long long tiles, cudaStream_t s,
+              DeviceState* st) {
+    using L = TcLayout<TN>;
+    // The attribute belongs to the device's context: set once a device, for the largest table.
+    static std::atomic<unsigned long long> attr_set{0};
+    const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
+    if (!bit || !(attr_set.load(std::memory_order_acquire) & bit)) {
+        SPMM_CUDA_TRY(cudaFuncSetAttribute(grouped_tc_kernel<FORM, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           L::kFixed + 4 * (SPMM_MAX_GROUPS + 1)));
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const size_t smem = L::kFixed + (FORM == kDw ? 0 : 4 * (static_cast<size_t>(a.groups) + 1));
+    const unsigned grid = static_cast<unsigned>(std::min<long long>(tiles, st->sm_count));
+    return launch_dependent(grouped_tc_kernel<FORM, TN>, dim3(grid), dim3(kTcThreads), smem, s, ma, small, mb, a);
+}
+
+bool fits16(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
+
+// Whether TMA and 16-byte stores can address the operands.
+template <int FORM>
+bool tc_fits(const GroupedArgs& a, DeviceState* st) {
+    if (st->cc_major != 10 || a.N % 8 || a.K % 8 || a.rows == 0 || a.N == 0 || a.K == 0) return false;
+    const int size = a.out_f32 ? 4 : 2;
+    if (!fits16(a.a, a.lda, 2) || !fits16(a.b, FORM == kDw ? a.ldb : 8, 2)) return false;
+    return fits16(a.out, FORM == kDw ? 8 : a.ldo, size);
+}
+
+template <int FORM>
+int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st) {
+    if (!tc_fits<FORM>(a, st)) return any_launch<FORM>(a, dtype, s, st);
+    TcArgs t{};
+    t.offsets = a.offsets;
+    t.groups = a.groups;
+    t.rows = a.rows;
+    t.outs = FORM == kForward ? a.N : a.K;
+    t.ms = a.N;
+    t.sum = FORM == kForward ? a.K : a.N;
+    t.mtiles = (a.N + kTileM - 1) / kTileM;
+    t.out = a.out;
+    t.ldo = FORM == kDw ? a.K : a.ldo;
+    t.out_f32 = a.out_f32;
+    t.dtype = dtype;
+    t.err = a.err;
+    // Row tiles: exact for dw, else as many as the groups can have (how many they do have is on the device).
+    const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * t.mtiles : a.rows / kTileM + std::min(a.groups, a.rows);
+    // The widest tile that still gives every SM one: a wide tile reads A less often, narrow ones spread few rows.
+    int tn = 256;
+    while (tn > 64 && (mtiles * ((t.outs + tn - 1) / tn) < st->sm_count || t.outs <= tn / 2)) tn /= 2;
+    t.ntiles = (t.outs + tn - 1) / tn;
+    const int64_t tiles = mtiles * t.ntiles;
+    if (tiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
+
+    CUtensorMap ma, small, mb;
+    const uint64_t rows = a.rows, N = a.N, K = a.K;
+    const uint64_t wide = FORM == kForward ? K : N;  // columns of A's operand
+    SPMM_TRY(encode_2d(&ma, a.a, wide, rows, a.lda * 2, 64, FORM == kDw ? 64 : kTileM, CU_TENSOR_MAP_SWIZZLE_128B));
+    SPMM_TRY(encode_2d(&small, a.a, wide, rows, a.lda * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
+    if constexpr (FORM == kDw) {
+        SPMM_TRY(encode_2d(&mb, a.b, K, rows, a.ldb * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+    } else {
+        SPMM_TRY(encode_3d(&mb, a.b, {K, N, static_cast<uint64_t>(a.groups)}, {K * 2, N * K * 2},
+                           {64, static_cast<uint32_t>(FORM == kForward ? tn : 64), 1}, CU_TENSOR_MAP_SWIZZLE_128B));
+    }
+    if (tn == 256) return tc_launch<FORM, 256>(ma, small, mb, t, tiles, s, st);
+    if (tn == 128) return tc_launch<FORM, 128>(ma, small, mb, t, tiles, s, st);
+    return tc_launch<FORM, 64>(ma, small, mb, t, tiles, s, st);
+}
+
 int check_common(const int32_t* offsets, int32_t groups, int32_t rows, int32_t N, int32_t K, int32_t dtype, int32_t out_dtype) {
     if (groups < 1 || rows < 0 || N < 0 || K < 0 || !offsets) return SPMM_ERR_INVALID_ARG;
     if (dtype != SPMM_DTYPE_F16 && dtype != SPMM_DTYPE_BF16) return SPMM_ERR_INVALID_ARG;
@@ -182,7 +569,7 @@ int spmm_grouped_mm(const int32_t* offsets, int32_t groups, int32_t rows, const 
     a.ldo = ldy;
     a.out_f32 = out_dtype == SPMM_DTYPE_F32;
     a.err = st->err;
-    return any_launch<kForward>(a, dtype, as_stream(stream), st);
+    return grouped_launch<kForward>(a, dtype, as_stream(stream), st);
 }
 
 int spmm_grouped_mm_dx(const int32_t* offsets, int32_t groups, int32_t rows, const void* dy, int64_t lddy, const void* w, void* dx,
@@ -211,7 +598,7 @@ int spmm_grouped_mm_dx(const int32_t* offsets, int32_t groups, int32_t rows, con
     a.ldo = lddx;
     a.out_f32 = out_dtype == SPMM_DTYPE_F32;
     a.err = st->err;
-    return any_launch<kDx>(a, dtype, as_stream(stream), st);
+    return grouped_launch<kDx>(a, dtype, as_stream(stream), st);
 }
 
 int spmm_grouped_mm_dw(const int32_t* offsets, int32_t groups, int32_t rows, const void* dy, int64_t lddy, const void* x, int64_t ldx,
@@ -240,7 +627,7 @@ int spmm_grouped_mm_dw(const int32_t* offsets, int32_t groups, int32_t rows, con
     a.ldb = ldx;
     a.out_f32 = out_dtype == SPMM_DTYPE_F32;
     a.err = st->err;
-    return any_launch<kDw>(a, dtype, as_stream(stream), st);
+    return grouped_launch<kDw>(a, dtype, as_stream(stream), st);
 }
 
 }  // extern "C"
