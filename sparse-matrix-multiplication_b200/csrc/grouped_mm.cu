@@ -177,39 +177,61 @@ struct TcArgs {
     void* out;
     long long ldo;     // row stride of out
     int out_f32, dtype;
+    // Forward only: the sum over k cut into `splits` ranges of split_steps steps, each with a result of its own
+    // (split_stride elements apart), and the groups' matrices by index (NULL: group g has matrix g).
+    int splits, split_steps;
+    long long split_stride;
+    const int* __restrict__ which;
+    int matrices;
     DeviceErrorRecord* err;
 };
 
 struct Tile {
-    int g, m0, n0;     // group, first row of D in the group, first column
+    int g, m0, n0;     // matrix, first row of D in the group, first column
     int begin, end;    // the group's rows
+    int split;         // forward: the range of the sum,
+    int first;         // its first step
     int steps;         // k steps
 };
 
 template <int FORM, int TN>
 __device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, int t) {
     Tile r;
-    int local, mtiles;
+    int g, local, mtiles;
+    r.split = 0;
+    if constexpr (FORM == kForward) {
+        if (a.splits > 1) {
+            const int whole = t / a.splits;
+            r.split = t - whole * a.splits;
+            t = whole;
+        }
+    }
     if constexpr (FORM == kDw) {
         const int per = a.mtiles * a.ntiles;
-        r.g = t / per;
-        local = t - r.g * per;
+        g = t / per;
+        local = t - g * per;
         mtiles = a.mtiles;
     } else {
-        r.g = tile_group(start, a.groups, t / a.ntiles);
-        local = t - start[r.g] * a.ntiles;
-        mtiles = start[r.g + 1] - start[r.g];
+        g = tile_group(start, a.groups, t / a.ntiles);
+        local = t - start[g] * a.ntiles;
+        mtiles = start[g + 1] - start[g];
     }
     const int band = local / (kBand * a.ntiles);
     const int high = min(kBand, mtiles - band * kBand);
     local -= band * kBand * a.ntiles;
     r.m0 = (band * kBand + local % high) * kTileM;
     r.n0 = local / high * TN;
-    const GroupRange range = group_range(a.offsets, r.g, a.rows, nullptr);
+    const GroupRange range = group_range(a.offsets, g, a.rows, nullptr);
     r.begin = range.begin;
     r.end = range.end;
+    r.g = FORM == kForward ? max(0, group_matrix(a.which, g, a.matrices, nullptr)) : g;
     const int sum = FORM == kDw ? r.end - r.begin : a.sum;
     r.steps = (sum + kStepK - 1) / kStepK;
+    r.first = 0;
+    if constexpr (FORM == kForward) {
+        r.first = r.split * a.split_steps;
+        r.steps = min(a.split_steps, r.steps - r.first);
+    }
     return r;
 }
 
@@ -254,8 +276,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int g = threadIdx.x; g < a.groups; g += kTcThreads) group_range(a.offsets, g, a.rows, a.err);  // records bad ones
         tiles = a.groups * a.mtiles * a.ntiles;
     } else {
-        build_tile_table(start, a.offsets, a.groups, a.rows, kTileM, blockIdx.x == 0 ? a.err : nullptr);
-        tiles = start[a.groups] * a.ntiles;
+        build_tile_table(start, a.offsets, a.groups, a.rows, kTileM, blockIdx.x == 0 ? a.err : nullptr,
+                         FORM == kForward ? a.which : nullptr, a.matrices);
+        tiles = start[a.groups] * a.ntiles * (FORM == kForward ? a.splits : 1);
     }
     tc_fence_before();
     __syncthreads();
@@ -282,7 +305,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         break;
                     }
                     mbar_arrive_expect_tx(bar, bytes);
-                    const int k0 = ks * kStepK;
+                    const int k0 = (r.first + ks) * kStepK;
                     if constexpr (FORM == kDw) {
                         for (int j = 0; j < na; ++j) tma_load_2d(sa + j * 8192, &map_a, bar, r.m0 + 64 * j, r.begin + k0);
                         for (int j = 0; j < nb; ++j) tma_load_2d(sb + j * 8192, &map_b, bar, r.n0 + 64 * j, r.begin + k0);
@@ -329,7 +352,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     ok = false;
                     break;
                 }
-                const int left = min(kStepK, sum - ks * kStepK), slices = (left + 15) / 16;
+                const int left = min(kStepK, sum - (r.first + ks) * kStepK), slices = (left + 15) / 16;
                 if constexpr (FORM == kDw) {
                     if (left % 16) {
                         const int nb = min(TN / 64, (a.outs - r.n0 + 63) / 64), na = min(2, (a.ms - r.m0 + 63) / 64);
@@ -381,7 +404,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t acc = tmem + buf * TN + (static_cast<uint32_t>(q * 32) << 16);
             const int rows = min(32, (FORM == kDw ? a.ms : r.end - r.begin) - r.m0 - q * 32);
             const long long first = FORM == kDw ? static_cast<long long>(r.g) * a.ms + r.m0 + q * 32 : r.begin + r.m0 + q * 32;
-            char* out = static_cast<char*>(a.out) + (first * a.ldo + r.n0) * size;
+            char* out = static_cast<char*>(a.out) + (first * a.ldo + r.n0 + r.split * a.split_stride) * size;
             const int cols = min(TN, a.outs - r.n0);
             if (rows > 0) {
                 for (int c0 = 0; c0 < cols; c0 += per) {
@@ -496,6 +519,8 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     t.ldo = FORM == kDw ? a.K : a.ldo;
     t.out_f32 = a.out_f32;
     t.dtype = dtype;
+    t.splits = 1;
+    t.split_steps = (t.sum + kStepK - 1) / kStepK;
     t.err = a.err;
     // Row tiles: exact for dw, else as many as the groups can have (how many they do have is on the device).
     const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * t.mtiles : a.rows / kTileM + std::min(a.groups, a.rows);
@@ -537,6 +562,39 @@ int check_operand(const void* p, int64_t ld, int64_t cols, int bytes) {
 }
 
 }  // namespace
+
+int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st) {
+    TcArgs t{};
+    t.offsets = p.offsets;
+    t.groups = p.groups;
+    t.rows = p.rows;
+    t.outs = p.rank;
+    t.sum = p.K;
+    t.ntiles = 1;
+    t.out = p.parts;
+    t.ldo = p.rank;
+    t.out_f32 = 1;
+    t.dtype = p.dtype;
+    t.splits = p.splits;
+    t.split_steps = p.steps_per_split;
+    t.split_stride = static_cast<long long>(p.rows) * p.rank;
+    t.which = p.which;
+    t.matrices = p.matrices;
+    t.err = st->err;
+    const int tn = p.rank <= 64 ? 64 : (p.rank <= 128 ? 128 : 256);
+    const int64_t tiles = (p.rows / kTileM + std::min<int64_t>(p.groups, p.rows)) * p.splits;
+    if (tiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
+    CUtensorMap ma, small, mb;
+    const uint64_t rows = p.rows, K = p.K, rank = p.rank;
+    SPMM_TRY(encode_2d(&ma, p.x, K, rows, p.ldx * 2, 64, kTileM, CU_TENSOR_MAP_SWIZZLE_128B));
+    SPMM_TRY(encode_2d(&small, p.x, K, rows, p.ldx * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
+    SPMM_TRY(encode_3d(&mb, p.a, {K, rank, static_cast<uint64_t>(p.matrices)}, {K * 2, rank * K * 2}, {64, static_cast<uint32_t>(tn), 1},
+                       CU_TENSOR_MAP_SWIZZLE_128B));
+    if (tn == 256) return tc_launch<kForward, 256>(ma, small, mb, t, tiles, s, st);
+    if (tn == 128) return tc_launch<kForward, 128>(ma, small, mb, t, tiles, s, st);
+    return tc_launch<kForward, 64>(ma, small, mb, t, tiles, s, st);
+}
+
 }  // namespace spmm_b200
 
 using namespace spmm_b200;

@@ -18,13 +18,21 @@ __device__ __forceinline__ GroupRange group_range(const int* __restrict__ offset
     return {begin, max(begin, min(e, rows))};
 }
 
-// start[g] = number of row tiles (tile rows each) of the groups before g, start[groups] = all of them. Called by every
-// thread of the block; ends with a barrier.
+// The matrix of group g: g itself, or which[g], -1 for none (negative or, recorded, past `matrices`).
+__device__ __forceinline__ int group_matrix(const int* __restrict__ which, int g, int matrices, DeviceErrorRecord* err) {
+    if (!which) return g;
+    const int i = __ldg(which + g);
+    if (i >= matrices) record_device_error(err, SPMM_ERR_BAD_INDEX, g);
+    return i < 0 || i >= matrices ? -1 : i;
+}
+
+// start[g] = number of row tiles (tile rows each) of the groups before g, start[groups] = all of them. Groups that
+// `which` gives no matrix have none. Called by every thread of the block; ends with a barrier.
 __device__ __forceinline__ void build_tile_table(int* start, const int* __restrict__ offsets, int groups, int rows, int tile,
-                                                 DeviceErrorRecord* err) {
+                                                 DeviceErrorRecord* err, const int* __restrict__ which = nullptr, int matrices = 0) {
     for (int g = threadIdx.x; g < groups; g += blockDim.x) {
         const GroupRange r = group_range(offsets, g, rows, err);
-        start[g + 1] = (r.end - r.begin + tile - 1) / tile;
+        start[g + 1] = group_matrix(which, g, matrices, err) < 0 ? 0 : (r.end - r.begin + tile - 1) / tile;
     }
     if (threadIdx.x == 0) start[0] = 0;
     __syncthreads();
@@ -45,7 +53,7 @@ __device__ __forceinline__ void build_tile_table(int* start, const int* __restri
     __syncthreads();
 }
 
-// The group of row tile m < start[groups].
+// The group of row tile m, 0 <= m < start[groups].
 __device__ __forceinline__ int tile_group(const int* start, int groups, int m) {
     int lo = 0, hi = groups;  // start[lo] <= m < start[hi]
     while (hi - lo > 1) {
@@ -55,5 +63,20 @@ __device__ __forceinline__ int tile_group(const int* start, int groups, int m) {
     }
     return lo;
 }
+
+// Partial sums of x[p] a[which[g]]^T on the tensor cores (grouped_mm.cu), for lora.cu: parts[s][p][0 .. rank) for each of
+// `splits` ranges of steps_per_split * 64 of K. Rows of groups without a matrix are not written. Operands on 16-byte
+// boundaries, rank and K multiples of 8.
+struct PartialProducts {
+    const int* offsets;
+    const int* which;
+    int groups, rows, matrices, rank, K, dtype;
+    const void* x;
+    long long ldx;
+    const void* a;
+    float* parts;
+    int splits, steps_per_split;
+};
+int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st);
 
 }  // namespace spmm_b200

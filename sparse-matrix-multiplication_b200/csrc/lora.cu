@@ -1,14 +1,17 @@
 // Low-rank adapters of many requests at once: out_p = base_p + s_i B_i (A_i x_p), i = the adapter of p's request.
 //
 // Two launches: shrink u_p = A_i x_p (rank values a row, FP32 in the workspace), expand out_p = base_p + s_i B_i u_p.
+// Three forms of each: a few rows a request (CUDA cores, latency), many (tcgen05, the rows' bytes), any alignment.
 
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstdint>
 
 #include "groups.cuh"
+#include "tcgen05.cuh"
 
 namespace spmm_b200 {
 namespace {
@@ -107,6 +110,495 @@ __global__ void __launch_bounds__(256) lora_expand_any_kernel(LoraArgs a) {
     }
 }
 
+// ------------------------------------------------------------------ few rows a request: CUDA cores
+//
+// With a row or a few to a request nothing is reused: the adapters' bytes bound the work, at single tokens its latency.
+// Shrink: a block takes a row and four ranks, all its loads in flight at once. Expand: a thread takes one output, its
+// row of b and its base are under way before the kernel waits for the shrink.
+
+constexpr int kRanksPerBlock = 4;
+
+// Dot product of eight 16-bit pairs, added to s.
+template <int DT>
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
+    float x[8], y[8];
+    RowVec<DT, 16>::unpack(a, x);
+    RowVec<DT, 16>::unpack(b, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
+    return s;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) lora_shrink_rows_kernel(LoraArgs a, int rank_blocks) {
+    __shared__ float sums[8][kRanksPerBlock];
+    grid_dependency_wait();
+    allow_dependent_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int p = blockIdx.x / rank_blocks, q0 = (blockIdx.x - p * rank_blocks) * kRanksPerBlock;
+    const int r = request_of(a, p);
+    const int i = r < 0 ? -1 : adapter_of(a, r, threadIdx.x == 0 && q0 == 0 ? a.err : nullptr);
+    if (i < 0) return;
+    const uint4* x = reinterpret_cast<const uint4*>(a.x + p * a.ldx);
+    const uint4* rows = reinterpret_cast<const uint4*>(a.a + (static_cast<long long>(i) * a.rank + q0) * a.K);
+    const int nvec = a.K / 8;
+    float s[kRanksPerBlock] = {};
+#pragma unroll 2
+    for (int c = threadIdx.x; c < nvec; c += 256) {
+        const uint4 xv = __ldg(x + c);
+        uint4 v[kRanksPerBlock];
+#pragma unroll
+        for (int q = 0; q < kRanksPerBlock; ++q) v[q] = __ldg(rows + static_cast<long long>(q) * nvec + c);  // rank is a multiple of 8
+#pragma unroll
+        for (int q = 0; q < kRanksPerBlock; ++q) s[q] = dot8<DT>(xv, v[q], s[q]);
+    }
+#pragma unroll
+    for (int q = 0; q < kRanksPerBlock; ++q) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) s[q] += __shfl_xor_sync(0xffffffffu, s[q], d);
+        if (lane == 0) sums[warp][q] = s[q];
+    }
+    __syncthreads();
+    if (threadIdx.x < kRanksPerBlock) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += sums[w][threadIdx.x];
+        a.u[static_cast<long long>(p) * a.rank + q0 + threadIdx.x] = t;
+    }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) lora_expand_rows_kernel(LoraArgs a, int col_blocks) {
+    constexpr int kAhead = 2;  // vectors of b's row that are loaded before the wait
+    __shared__ __align__(16) float u[kMaxRank];
+    // Reached only behind the shrink of the same call, which has itself waited for everything before it and writes
+    // nothing but u: the rest may be read before this kernel's own wait.
+    allow_dependent_launch();
+    if (blockIdx.x == 0 && a.offsets)
+        for (int k = threadIdx.x; k < a.requests; k += 256) group_range(a.offsets, k, a.rows, a.err);  // records bad ones
+    const int p = blockIdx.x / col_blocks, n = (blockIdx.x - p * col_blocks) * 256 + threadIdx.x;
+    const int r = request_of(a, p);
+    const int i = r < 0 ? -1 : adapter_of(a, r, nullptr);
+    const bool mine = r >= 0 && n < a.N;
+    const uint4* row = reinterpret_cast<const uint4*>(a.b + (static_cast<long long>(max(i, 0)) * a.N + n) * a.rank);
+    const int nvec = a.rank / 8;
+    uint4 v[kAhead];
+    float base = 0.f, scale = 1.f;
+    if (mine) {
+        if (i >= 0) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (k < nvec) v[k] = __ldg(row + k);
+            if (a.scale) scale = __ldg(a.scale + i);
+        }
+        if (a.base) base = half_bits_to_float<DT>(a.base[p * a.ldbase + n]);
+    }
+    grid_dependency_wait();
+    if (i >= 0)
+        for (int q = threadIdx.x; q < a.rank; q += 256) u[q] = a.u[static_cast<long long>(p) * a.rank + q];
+    __syncthreads();
+    if (!mine) return;
+    float d = 0.f;
+    if (i >= 0) {
+        const auto add = [&](const uint4& w, int k) {
+            float f[8];
+            RowVec<DT, 16>::unpack(w, f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d = fmaf(f[e], u[8 * k + e], d);
+        };
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (k < nvec) add(v[k], k);
+#pragma unroll 4
+        for (int k = kAhead; k < nvec; ++k) add(__ldg(row + k), k);
+        d = a.base ? fmaf(d, scale, base) : d * scale;
+    } else {
+        d = base;
+    }
+    a.out[p * a.ldout + n] = float_to_half_bits<DT>(d);
+}
+
+// ------------------------------------------------------------------ many rows a request: tcgen05
+//
+// Shrink is the grouped product's kernel on 128-row tiles of the requests, its sum over K cut so that few tiles still
+// fill the GPU (partial_products; FP32 parts in the workspace). Expand moves base and out (2 x rows x N) and computes
+// little: a persistent block holds u of a 128-row tile in shared memory and streams b and base past it.
+//   warp 0      TMA: b (TN features x rank) and the base tile (128 x TN) into a ring of stages
+//   warp 1      MMA: D = u b^T in TMEM, two accumulators
+//   warps 2..5  D * scale + base -> the base's place in the stage -> 16-byte stores of 128-byte row pieces
+//   warps 6..9  the next tile's u: the parts' sum as two 16-bit terms, hi + lo, K-major under the 128-byte swizzle
+// The MMA needs 16-bit u; one term would cost half a step of 16 bits in every product (2^-8 in bf16), two leave 2^-16
+// for twice the MMAs, which still run under the copies.
+
+constexpr int kTileM = 128;
+constexpr int kExpandThreads = 320;
+constexpr int kSmallRows = 8;  // requests with no more rows load a base box of this many
+
+template <int RB>  // rank in blocks of 64
+struct ExpandLayout {
+    static constexpr int kTn = RB == 4 ? 64 : 128;
+    static constexpr int kU = 2 * RB * 16384;                 // hi blocks, lo blocks: 128 rows x 64 each
+    static constexpr int kUs = RB == 1 ? 2 : 1;
+    static constexpr int kB = RB * kTn * 128;
+    static constexpr int kBase = kTn / 64 * 16384;            // 64-column blocks of 128 rows
+    static constexpr int kStage = kB + kBase;
+    static constexpr int kStages = RB == 1 ? 3 : (RB == 2 ? 2 : 1);
+    static constexpr int kStage0 = kUs * kU;
+    static constexpr int kBars = kStage0 + kStages * kStage;  // full[], empty[], u_full[2], u_empty[2], acc_full[2], acc_empty[2], drain
+    static constexpr int kSlot = kBars + 8 * (2 * kStages + 9);
+    static constexpr int kTable = kSlot + 8;
+    static constexpr int kFixed = kTable + 1024;
+};
+
+struct ExpandArgs {
+    LoraArgs l;
+    int splits;
+    int ntiles, per_unit, chunks;  // column tiles, of which a unit takes per_unit, units along a row
+};
+
+struct Unit {
+    int i;             // adapter, -1 none
+    int row, rows;     // first row, rows of the tile
+    int nt0, nt1;      // column tiles
+};
+
+__device__ __forceinline__ Unit unit_of(const ExpandArgs& e, const int* start, int u) {
+    const int m = u / e.chunks, c = u - m * e.chunks;
+    const int r = tile_group(start, e.l.requests, m);
+    const GroupRange g = group_range(e.l.offsets, r, e.l.rows, nullptr);
+    Unit x;
+    x.row = g.begin + (m - start[r]) * kTileM;
+    x.rows = min(kTileM, g.end - x.row);
+    x.i = adapter_of(e.l, r, nullptr);
+    x.nt0 = c * e.per_unit;
+    x.nt1 = min(e.ntiles, x.nt0 + e.per_unit);
+    return x;
+}
+
+template <int DT, int RB>
+__global__ void __launch_bounds__(kExpandThreads, 1)
+    lora_expand_tc_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_base,
+                          const __grid_constant__ CUtensorMap map_base_small, ExpandArgs e) {
+    using L = ExpandLayout<RB>;
+    constexpr int kStages = L::kStages, kTn = L::kTn, kUs = L::kUs;
+    const LoraArgs& a = e.l;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_addr(smem_raw);
+    uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+    const uint32_t sbase = smem_addr(base);
+    const uint32_t full0 = sbase + L::kBars, empty0 = full0 + 8 * kStages, u_full0 = empty0 + 8 * kStages, u_empty0 = u_full0 + 16,
+                   acc_full0 = u_empty0 + 16, acc_empty0 = acc_full0 + 16, drain = acc_empty0 + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kSlot);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* start = reinterpret_cast<int*>(base + L::kTable);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 4);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(u_full0 + 8 * s, 4);
+            mbar_init(u_empty0 + 8 * s, 1);
+            mbar_init(acc_full0 + 8 * s, 1);
+            mbar_init(acc_empty0 + 8 * s, 4);
+        }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_tensormap(&map_b);
+        if (a.base) prefetch_tensormap(&map_base);
+    }
+    if (warp == 1) tmem_alloc(smem_addr(tmem_slot), 2 * kTn);
+    // Only the warps that read the shrink's parts wait for it (every block has them, so none ends before it): the shrink
+    // itself waited for everything before it, and writes nothing else.
+    allow_dependent_launch();
+    build_tile_table(start, a.offsets, a.requests, a.rows, kTileM, blockIdx.x == 0 ? a.err : nullptr);
+    const int units = start[a.requests] * e.chunks;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        // ---------------- producer
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+                const Unit x = unit_of(e, start, u);
+                const bool small = x.rows <= kSmallRows;
+                for (int nt = x.nt0; nt < x.nt1; ++nt, ++it) {
+                    const int s = it % kStages;
+                    const uint32_t bar = full0 + 8 * s, sb = sbase + L::kStage0 + s * L::kStage, sbs = sb + L::kB;
+                    if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const int n0 = nt * kTn, blocks = min(kTn / 64, (a.N - n0 + 63) / 64);
+                    const uint32_t bytes = (x.i >= 0 ? L::kB : 0) + (a.base ? blocks * (small ? kSmallRows * 128 : 16384) : 0);
+                    mbar_arrive_expect_tx(bar, bytes);
+                    if (x.i >= 0)
+                        for (int k = 0; k < RB; ++k) tma_load_3d(sb + k * kTn * 128, &map_b, bar, 64 * k, n0, x.i);
+                    if (a.base)
+                        for (int k = 0; k < blocks; ++k)
+                            tma_load_2d(sbs + k * 16384, small ? &map_base_small : &map_base, bar, n0 + 64 * k, x.row);
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                record_device_error(a.err, SPMM_ERR_TIMEOUT, 21);
+            }
+            for (int i = max(0, it - kStages); i < it; ++i) {
+                const unsigned long long t0 = global_ns();
+                while (!mbar_try_wait(full0 + 8 * (i % kStages), (i / kStages) & 1u) && global_ns() - t0 < kWaitNs) {
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer
+        if (lane == 0) {
+            const uint32_t idesc = instr_desc_f16(DT, kTn, false, false);
+            const int slices = (a.rank + 15) / 16;
+            int it = 0, nu = 0, n = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+                const Unit x = unit_of(e, start, u);
+                if (x.i < 0) {
+                    it += x.nt1 - x.nt0;
+                    continue;
+                }
+                const int ub = nu % kUs;
+                if (!mbar_wait(u_full0 + 8 * ub, (nu / kUs) & 1u, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                for (int nt = x.nt0; nt < x.nt1; ++nt, ++it, ++n) {
+                    const int s = it % kStages, buf = n & 1;
+                    if (!mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag) ||
+                        !mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t su = sbase + ub * L::kU, sb = sbase + L::kStage0 + s * L::kStage;
+                    for (int t = 0; t < 2; ++t)
+                        for (int k = 0; k < slices; ++k) {
+                            const uint64_t da = smem_desc(su + (t * RB + k / 4) * 16384 + 32 * (k % 4), 16, 1024, kSwizzle128);
+                            const uint64_t db = smem_desc(sb + k / 4 * kTn * 128 + 32 * (k % 4), 16, 1024, kSwizzle128);
+                            umma_f16(tmem + buf * kTn, da, db, idesc, t + k > 0 ? 1u : 0u);
+                        }
+                    umma_commit(acc_full0 + 8 * buf);
+                }
+                umma_commit(u_empty0 + 8 * ub);
+                ++nu;
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                record_device_error(a.err, SPMM_ERR_TIMEOUT, 22);
+            }
+        }
+        __syncwarp();
+    } else if (warp < 6) {
+        // ---------------- epilogue
+        const int q = warp & 3;
+        int it = 0, n = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+            const Unit x = unit_of(e, start, u);
+            const float scale = x.i >= 0 && a.scale ? __ldg(a.scale + x.i) : 1.f;
+            const int rows = min(32, x.rows - q * 32);
+            for (int nt = x.nt0; nt < x.nt1; ++nt, ++it) {
+                const int s = it % kStages, buf = n & 1;
+                bool got = mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag);
+                if (x.i >= 0) got = got && mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag);
+                if (!__all_sync(0xffffffffu, got)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const int cols = min(kTn, a.N - nt * kTn);
+                if (rows > 0) {
+                    for (int c0 = 0; c0 < cols; c0 += 64) {
+                        uint8_t* block = base + L::kStage0 + s * L::kStage + L::kB + c0 / 64 * 16384 + q * 4096;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t v[32];
+                            if (x.i >= 0) {
+                                tmem_ld32(tmem + buf * kTn + c0 + 32 * h + (static_cast<uint32_t>(q * 32) << 16), v);
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) v[k] = 0u;
+                            }
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint4* at = reinterpret_cast<uint4*>(block + lane * 128 + (((4 * h + c) ^ (lane & 7)) << 4));
+                                float f[8] = {};
+                                if (a.base) RowVec<DT, 16>::unpack(*at, f);
+                                if (x.i >= 0) {
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k) f[k] = fmaf(__uint_as_float(v[8 * c + k]), scale, f[k]);
+                                }
+                                *at = RowVec<DT, 16>::pack(f);
+                            }
+                        }
+                        __syncwarp();
+                        const int c = lane & 7, col = c0 + 8 * c;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int row = 4 * k + (lane >> 3);
+                            if (row < rows && col < cols)
+                                *reinterpret_cast<uint4*>(a.out + (x.row + q * 32 + row) * a.ldout + nt * kTn + col) =
+                                    *reinterpret_cast<const uint4*>(block + row * 128 + ((c ^ (row & 7)) << 4));
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA writes the stage again
+                }
+                __syncwarp();
+                tc_fence_before();
+                if (lane == 0) {
+                    mbar_arrive_count(empty0 + 8 * s, 1);
+                    if (x.i >= 0) mbar_arrive_count(acc_empty0 + 8 * buf, 1);
+                }
+                if (x.i >= 0) ++n;
+            }
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_device_error(a.err, SPMM_ERR_TIMEOUT, 23);
+        }
+    } else {
+        // ---------------- u: sum of the parts -> hi + lo
+        grid_dependency_wait();
+        const int row = (warp - 6) * 32 + lane;
+        const int pieces = (a.rank + 15) / 16 * 2;  // 8 ranks each; the last may lie past the rank and is zero
+        int nu = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+            const Unit x = unit_of(e, start, u);
+            if (x.i < 0) continue;
+            const int ub = nu % kUs;
+            if (!__all_sync(0xffffffffu, mbar_wait(u_empty0 + 8 * ub, ((nu / kUs) & 1u) ^ 1u, abort_flag))) {
+                ok = false;
+                break;
+            }
+            if (row < x.rows) {
+                uint8_t* hi = base + ub * L::kU + row * 128;
+                const float* part = a.u + static_cast<long long>(x.row + row) * a.rank;
+                const long long stride = static_cast<long long>(a.rows) * a.rank;
+                for (int c = 0; c < pieces; ++c) {
+                    float f[8] = {};
+                    if (8 * c < a.rank) {
+                        for (int k = 0; k < e.splits; ++k) {
+                            const float4* src = reinterpret_cast<const float4*>(part + k * stride + 8 * c);
+                            const float4 lo4 = src[0], hi4 = src[1];
+                            f[0] += lo4.x, f[1] += lo4.y, f[2] += lo4.z, f[3] += lo4.w;
+                            f[4] += hi4.x, f[5] += hi4.y, f[6] += hi4.z, f[7] += hi4.w;
+                        }
+                    }
+                    const uint4 top = RowVec<DT, 16>::pack(f);
+                    float g[8];
+                    RowVec<DT, 16>::unpack(top, g);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) g[k] = f[k] - g[k];
+                    const uint4 rest = RowVec<DT, 16>::pack(g);
+                    const int at = c / 8 * 16384 + (((c % 8) ^ (row & 7)) << 4);
+                    *reinterpret_cast<uint4*>(hi + at) = top;
+                    *reinterpret_cast<uint4*>(hi + RB * 16384 + at) = rest;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_count(u_full0 + 8 * ub, 1);
+            ++nu;
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_device_error(a.err, SPMM_ERR_TIMEOUT, 24);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        // The last commits' arrivals, and after a timeout the MMAs in flight, end before the block gives up its TMEM.
+        if (lane == 0) {
+            umma_commit(drain);
+            const unsigned long long t0 = global_ns();
+            while (!mbar_try_wait(drain, 0) && global_ns() - t0 < kWaitNs) {
+            }
+        }
+        __syncwarp();
+        tmem_dealloc(tmem, 2 * kTn);
+    }
+}
+
+template <int DT, int RB>
+int expand_launch(const CUtensorMap& mb, const CUtensorMap& ms, const CUtensorMap& small, const ExpandArgs& e, long long units,
+                  cudaStream_t s, DeviceState* st) {
+    using L = ExpandLayout<RB>;
+    static std::atomic<unsigned long long> attr_set{0};
+    const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
+    if (!bit || !(attr_set.load(std::memory_order_acquire) & bit)) {
+        SPMM_CUDA_TRY(cudaFuncSetAttribute(lora_expand_tc_kernel<DT, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           L::kFixed + 4 * (SPMM_MAX_GROUPS + 1)));
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    const size_t smem = L::kFixed + 4 * (static_cast<size_t>(e.l.requests) + 1);
+    const unsigned grid = static_cast<unsigned>(std::min<long long>(units, st->sm_count));
+    return launch_dependent(lora_expand_tc_kernel<DT, RB>, dim3(grid), dim3(kExpandThreads), smem, s, mb, ms, small, e);
+}
+
+template <int DT>
+int expand(const ExpandArgs& e0, int64_t mtiles, cudaStream_t s, DeviceState* st) {
+    ExpandArgs e = e0;
+    const LoraArgs& a = e.l;
+    const int rb = a.rank <= 64 ? 1 : (a.rank <= 128 ? 2 : 4);
+    const int tn = rb == 4 ? 64 : 128;
+    e.ntiles = (a.N + tn - 1) / tn;
+    // Column tiles of a unit: u is made once for all of them, but every SM should have two units.
+    e.per_unit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, mtiles * e.ntiles / (2 * st->sm_count))));
+    e.chunks = (e.ntiles + e.per_unit - 1) / e.per_unit;
+    const int64_t units = mtiles * e.chunks;
+    if (units > INT32_MAX) return SPMM_ERR_TOO_LARGE;
+    CUtensorMap mb, ms{}, small{};
+    const uint64_t N = a.N, rank = a.rank, rows = a.rows;
+    SPMM_TRY(encode_3d(&mb, a.b, {rank, N, static_cast<uint64_t>(a.adapters)}, {rank * 2, N * rank * 2}, {64, static_cast<uint32_t>(tn), 1},
+                       CU_TENSOR_MAP_SWIZZLE_128B));
+    if (a.base) {
+        SPMM_TRY(encode_2d(&ms, a.base, N, rows, a.ldbase * 2, 64, kTileM, CU_TENSOR_MAP_SWIZZLE_128B));
+        SPMM_TRY(encode_2d(&small, a.base, N, rows, a.ldbase * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
+    }
+    if (rb == 1) return expand_launch<DT, 1>(mb, ms, small, e, units, s, st);
+    if (rb == 2) return expand_launch<DT, 2>(mb, ms, small, e, units, s, st);
+    return expand_launch<DT, 4>(mb, ms, small, e, units, s, st);
+}
+
+// ------------------------------------------------------------------ host
+
+// How a call runs, by its sizes alone (the lengths are on the device). `fits`: 16-byte boundaries throughout.
+struct Shape {
+    bool rows;         // CUDA cores, a few rows a request
+    int splits, steps_per_split;
+    int64_t mtiles;
+};
+
+Shape shape_of(int32_t requests, int32_t rows, int32_t K) {
+    Shape h{};
+    h.rows = rows <= 4 * static_cast<int64_t>(requests);
+    h.mtiles = rows / kTileM + std::min(requests, rows);
+    // Ranges of the sum over K until about two tiles an SM (of 148) are there, each at least 8 steps of 64 long.
+    const int steps = (K + 63) / 64;
+    const int64_t want = h.rows ? 1 : std::max<int64_t>(1, std::min<int64_t>({8, 296 / std::max<int64_t>(1, h.mtiles), steps / 8}));
+    h.steps_per_split = static_cast<int>((steps + want - 1) / want);
+    h.splits = h.steps_per_split ? (steps + h.steps_per_split - 1) / h.steps_per_split : 1;
+    return h;
+}
+
+bool fits16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
+
 int check_view(const spmm_lora_view* l, int32_t requests, int32_t rows) {
     if (!l || l->adapters < 0 || l->rank < 0 || l->N < 0 || l->K < 0 || requests < 0 || rows < 0) return SPMM_ERR_INVALID_ARG;
     if (l->dtype != SPMM_DTYPE_F16 && l->dtype != SPMM_DTYPE_BF16) return SPMM_ERR_INVALID_ARG;
@@ -130,7 +622,7 @@ extern "C" {
 int spmm_lora_workspace_size(const spmm_lora_view* l, int32_t requests, int32_t rows, size_t* bytes) {
     SPMM_TRY(check_view(l, requests, rows));
     if (!bytes) return SPMM_ERR_INVALID_ARG;
-    *bytes = sizeof(float) * static_cast<size_t>(rows) * l->rank;
+    *bytes = sizeof(float) * static_cast<size_t>(rows) * l->rank * shape_of(requests, rows, l->K).splits;
     return SPMM_OK;
 }
 
@@ -181,8 +673,28 @@ int spmm_lora(const spmm_lora_view* l, const int32_t* offsets, const int32_t* ad
     a.u = static_cast<float*>(ws);
     a.err = st->err;
     const cudaStream_t s = as_stream(stream);
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, st->sm_count * 8)));
     const bool bf16 = l->dtype == SPMM_DTYPE_BF16;
+    const bool fits = adds && st->cc_major == 10 && l->K > 0 && l->K % 8 == 0 && l->N % 8 == 0 && l->rank % 8 == 0 && fits16(x, ldx) &&
+                      fits16(out, ldout) && (!base || fits16(base, ldbase)) && fits16(l->a, 8) && fits16(l->b, 8);
+    const Shape h = shape_of(requests, rows, l->K);
+    if (fits && h.rows) {
+        const int rank_blocks = l->rank / kRanksPerBlock, col_blocks = (l->N + 255) / 256;
+        const int64_t blocks = static_cast<int64_t>(rows) * std::max(rank_blocks, col_blocks);
+        if (blocks > INT32_MAX) return SPMM_ERR_TOO_LARGE;
+        SPMM_TRY(launch_dependent(bf16 ? lora_shrink_rows_kernel<SPMM_DTYPE_BF16> : lora_shrink_rows_kernel<SPMM_DTYPE_F16>,
+                                  dim3(static_cast<unsigned>(rows) * rank_blocks), dim3(256), 0, s, a, rank_blocks));
+        return launch_dependent(bf16 ? lora_expand_rows_kernel<SPMM_DTYPE_BF16> : lora_expand_rows_kernel<SPMM_DTYPE_F16>,
+                                dim3(static_cast<unsigned>(rows) * col_blocks), dim3(256), 0, s, a, col_blocks);
+    }
+    if (fits) {
+        PartialProducts p{offsets, adapter, requests, rows, l->adapters, l->rank, l->K, l->dtype, x, ldx, l->a, a.u, h.splits, h.steps_per_split};
+        SPMM_TRY(partial_products(p, s, st));
+        ExpandArgs e{};
+        e.l = a;
+        e.splits = h.splits;
+        return bf16 ? expand<SPMM_DTYPE_BF16>(e, h.mtiles, s, st) : expand<SPMM_DTYPE_F16>(e, h.mtiles, s, st);
+    }
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, st->sm_count * 8)));
     if (adds)
         SPMM_TRY(launch_dependent(bf16 ? lora_shrink_any_kernel<SPMM_DTYPE_BF16> : lora_shrink_any_kernel<SPMM_DTYPE_F16>, grid, dim3(256), 0,
                                   s, a));

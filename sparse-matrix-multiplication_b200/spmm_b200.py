@@ -671,68 +671,74 @@ class RankPlan:
 # type, shape or device raises ValueError, a refusal of the library SpmmError. `stream`: None is the legacy default
 # stream, as everywhere here.
 
+# The checks are a few attribute reads a tensor: at the sizes of single tokens they would otherwise cost more than the
+# launch (a whole call is about 6 us of host time).
+
+_torch = None  # the torch module, once a tensor has been seen
 _DTYPES: dict = {}
 
 
-def _dtypes() -> dict:
-    if not _DTYPES:
+def _device(t) -> int:
+    """The current device, on which `t` and every other operand must be."""
+    global _torch
+    if _torch is None:
         import torch
 
         _DTYPES.update({torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32})
-    return _DTYPES
+        _torch = torch
+    dev = t.get_device()
+    if dev < 0 or dev != _torch.cuda.current_device():
+        raise ValueError(f"operands must be on the current CUDA device, got {t.device}")
+    return dev
 
 
-def _here() -> int:
-    import torch
-
-    return torch.cuda.current_device() if torch.cuda.is_available() else -1
+def _refuse(t, what: str, shape: tuple, dtype, dev: int):
+    raise ValueError(f"{what}: want {shape} {dtype} on cuda:{dev}, got {tuple(t.shape)} {t.dtype}, strides {t.stride()}, on {t.device}")
 
 
-def _rows(t, what: str, shape: tuple, dtype) -> int:
-    """Row stride of a (rows, columns) tensor whose rows are contiguous."""
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_cuda or t.device.index != _here():
-        raise ValueError(f"{what}: want {shape} {dtype} on cuda:{_here()}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _rows(t, what: str, shape: tuple, dtype, dev: int) -> int:
+    """Row stride of a (rows, columns) tensor whose rows are contiguous and do not overlap."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
+        _refuse(t, what, shape, dtype, dev)
     ld, step = t.stride()
-    if (step != 1 and shape[1] > 1) or (shape[0] > 1 and ld < shape[1]):
-        raise ValueError(f"{what}: the elements of a row must be adjacent and rows must not overlap, got strides {t.stride()}")
+    if ld >= shape[1] and step == 1:
+        return ld
+    if (step != 1 and shape[1] > 1) or (ld < shape[1] and shape[0] > 1):
+        _refuse(t, what + " (the elements of a row adjacent, rows apart)", shape, dtype, dev)
     return max(ld, shape[1])
 
 
-def _flat(t, what: str, shape: tuple, dtype) -> int:
+def _flat(t, what: str, shape: tuple, dtype, dev: int) -> int:
     """Address of a contiguous tensor (0 for None)."""
     if t is None:
         return 0
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_cuda or t.device.index != _here() or not t.is_contiguous():
-        raise ValueError(f"{what}: want contiguous {shape} {dtype} on cuda:{_here()}, got {tuple(t.shape)} {t.dtype} "
-                         f"strides {t.stride()} on {t.device}")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        _refuse(t, what + " (contiguous)", shape, dtype, dev)
     return t.data_ptr()
 
 
-def _value_dtype(t, what: str, allowed=(DTYPE_F16, DTYPE_BF16)) -> int:
-    dt = _dtypes().get(t.dtype)
-    if dt not in allowed:
+def _value_dtype(t, what: str, f32: bool = False) -> int:
+    dt = _DTYPES.get(t.dtype)
+    if dt is None or (dt == DTYPE_F32 and not f32):
         raise ValueError(f"{what}: unsupported type {t.dtype}")
     return dt
 
 
-def _workspace(ws, need: int, stream):
+def _workspace(ws, need: int, stream: int, dev: int):
     """(tensor that owns the workspace, address, bytes). Without one from the caller, memory of torch's allocator in the
     order of `stream`: reused by a later allocation only behind this call's kernels, also under graph capture."""
     if need == 0:
         return None, 0, 0
-    if ws is not None:
-        if not ws.is_cuda or ws.device.index != _here() or not ws.is_contiguous():
-            raise ValueError("ws: want a contiguous CUDA tensor on the current device")
-        return ws, ws.data_ptr(), ws.numel() * ws.element_size()
-    import torch
-
-    sp = stream_ptr(stream)
-    if sp == torch.cuda.current_stream().cuda_stream:
-        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
-    else:
-        with torch.cuda.stream(torch.cuda.ExternalStream(sp) if sp else torch.cuda.default_stream()):
-            ws = torch.empty(need, dtype=torch.uint8, device="cuda")
-    return ws, ws.data_ptr(), need
+    if ws is None:
+        cuda = _torch.cuda
+        if stream == cuda.current_stream().cuda_stream:
+            ws = _torch.empty(need, dtype=_torch.uint8, device="cuda")
+        else:
+            with cuda.stream(cuda.ExternalStream(stream) if stream else cuda.default_stream()):
+                ws = _torch.empty(need, dtype=_torch.uint8, device="cuda")
+    elif ws.get_device() != dev or not ws.is_contiguous():
+        raise ValueError("ws: want a contiguous CUDA tensor on the current device")
+    return ws, ws.data_ptr(), ws.numel() * ws.element_size()
 
 
 def route_workspace_size(tokens: int, topk: int, groups: int) -> int:
@@ -743,132 +749,121 @@ def route_workspace_size(tokens: int, topk: int, groups: int) -> int:
 
 def route_build(ids, groups: int, offsets, order, pos, ws=None, stream=None) -> None:
     """Sort the pairs of ids (tokens, topk) by group: offsets (groups + 1), order (tokens * topk, or None), pos (tokens, topk)."""
-    import torch
+    dev = _device(ids)
+    i32 = _torch.int32
+    shape = tokens, topk = ids.shape
+    sp = stream_ptr(stream)
+    _ws, wp, wn = _workspace(ws, route_workspace_size(tokens, topk, groups), sp, dev)
+    check(lib().spmm_route_build(_flat(ids, "ids", shape, i32, dev), tokens, topk, groups,
+                                 _flat(offsets, "offsets", (groups + 1,), i32, dev),
+                                 _flat(order, "order", (tokens * topk,), i32, dev), _flat(pos, "pos", shape, i32, dev), wp, wn, sp),
+          "spmm_route_build")
 
-    tokens, topk = ids.shape
-    need = route_workspace_size(tokens, topk, groups)
-    _ws, wp, wn = _workspace(ws, need, stream)
-    check(lib().spmm_route_build(_flat(ids, "ids", (tokens, topk), torch.int32), tokens, topk, groups,
-                                 _flat(offsets, "offsets", (groups + 1,), torch.int32),
-                                 _flat(order, "order", (tokens * topk,), torch.int32),
-                                 _flat(pos, "pos", (tokens, topk), torch.int32), wp, wn, stream_ptr(stream)), "spmm_route_build")
 
-
-def _route_view(pos, rows: int) -> RouteView:
-    import torch
-
+def _route_view(pos, rows: int, dev: int) -> RouteView:
     tokens, topk = pos.shape
-    return RouteView(tokens, topk, rows, _flat(pos, "pos", (tokens, topk), torch.int32))
+    return RouteView(tokens, topk, rows, _flat(pos, "pos", (tokens, topk), _torch.int32, dev))
 
 
 def route_gather(pos, x, xs, stream=None) -> None:
     """xs[pos[t, j]] = x[t] (rows of xs without a pair stay as they are)."""
-    rows, H = xs.shape
-    dt = _value_dtype(x, "x", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
-    v = _route_view(pos, rows)
-    check(lib().spmm_route_gather(C.byref(v), x.data_ptr(), _rows(x, "x", (v.tokens, H), x.dtype), xs.data_ptr(),
-                                  _rows(xs, "xs", (rows, H), x.dtype), H, dt, stream_ptr(stream)), "spmm_route_gather")
+    dev = _device(pos)
+    shape = rows, H = xs.shape
+    v = _route_view(pos, rows, dev)
+    check(lib().spmm_route_gather(v, x.data_ptr(), _rows(x, "x", (v.tokens, H), x.dtype, dev), xs.data_ptr(),
+                                  _rows(xs, "xs", shape, x.dtype, dev), H, _value_dtype(x, "x", True), stream_ptr(stream)),
+          "spmm_route_gather")
 
 
 def route_combine(pos, ys, y, w=None, stream=None) -> None:
     """y[t] = sum_j w[t, j] ys[pos[t, j]] (w None: all 1, the gradient of route_gather)."""
-    import torch
-
-    rows, H = ys.shape
-    dt = _value_dtype(ys, "ys", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
-    v = _route_view(pos, rows)
-    check(lib().spmm_route_combine(C.byref(v), ys.data_ptr(), _rows(ys, "ys", (rows, H), ys.dtype),
-                                   _flat(w, "w", (v.tokens, v.topk), torch.float32), y.data_ptr(),
-                                   _rows(y, "y", (v.tokens, H), ys.dtype), H, dt, stream_ptr(stream)), "spmm_route_combine")
+    dev = _device(pos)
+    shape = rows, H = ys.shape
+    v = _route_view(pos, rows, dev)
+    check(lib().spmm_route_combine(v, ys.data_ptr(), _rows(ys, "ys", shape, ys.dtype, dev),
+                                   _flat(w, "w", pos.shape, _torch.float32, dev), y.data_ptr(),
+                                   _rows(y, "y", (v.tokens, H), ys.dtype, dev), H, _value_dtype(ys, "ys", True), stream_ptr(stream)),
+          "spmm_route_combine")
 
 
 def route_combine_grad(pos, dy, ys=None, w=None, dys=None, dw=None, stream=None) -> None:
     """Gradients of route_combine: dys[pos[t, j]] = w[t, j] dy[t] and dw[t, j] = <dy[t], ys[pos[t, j]]>; either may be left out
     (None; ys is needed for dw only)."""
-    import torch
-
-    H = dy.shape[1]
-    dt = _value_dtype(dy, "dy", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
+    dev = _device(pos)
     if dys is None and dw is None:
         raise ValueError("route_combine_grad: neither dys nor dw is wanted")
     if dw is not None and ys is None:
         raise ValueError("route_combine_grad: dw needs ys")
-    if dw is not None and dys is not None and ys.shape[0] != dys.shape[0]:
-        raise ValueError("route_combine_grad: ys and dys must have the same rows")
+    H = dy.shape[1]
     ys = ys if dw is not None else None
-    rows = (dys if dys is not None else ys).shape[0]
-    v = _route_view(pos, rows)
+    shape = ((dys if dys is not None else ys).shape[0], H)
+    v = _route_view(pos, shape[0], dev)
+    f32 = _torch.float32
     check(lib().spmm_route_combine_grad(
-        C.byref(v), dy.data_ptr(), _rows(dy, "dy", (v.tokens, H), dy.dtype), ptr(ys),
-        _rows(ys, "ys", (rows, H), dy.dtype) if ys is not None else 0, _flat(w, "w", (v.tokens, v.topk), torch.float32), ptr(dys),
-        _rows(dys, "dys", (rows, H), dy.dtype) if dys is not None else 0, _flat(dw, "dw", (v.tokens, v.topk), torch.float32), H, dt,
-        stream_ptr(stream)), "spmm_route_combine_grad")
+        v, dy.data_ptr(), _rows(dy, "dy", (v.tokens, H), dy.dtype, dev), ptr(ys),
+        _rows(ys, "ys", shape, dy.dtype, dev) if ys is not None else 0, _flat(w, "w", pos.shape, f32, dev), ptr(dys),
+        _rows(dys, "dys", shape, dy.dtype, dev) if dys is not None else 0, _flat(dw, "dw", pos.shape, f32, dev), H,
+        _value_dtype(dy, "dy", True), stream_ptr(stream)), "spmm_route_combine_grad")
 
 
 def grouped_mm(offsets, x, w, y, stream=None) -> None:
     """y[p] = w[g] x[p] for offsets[g] <= p < offsets[g + 1]; x (rows, K), w (groups, N, K), y (rows, N) of x's type or float32."""
-    import torch
-
+    dev = _device(offsets)
     groups, N, K = w.shape
     rows = x.shape[0]
-    dt, odt = _value_dtype(x, "x"), _value_dtype(y, "y", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
-    check(lib().spmm_grouped_mm(_flat(offsets, "offsets", (groups + 1,), torch.int32), groups, rows, x.data_ptr(),
-                                _rows(x, "x", (rows, K), x.dtype), _flat(w, "w", (groups, N, K), x.dtype), y.data_ptr(),
-                                _rows(y, "y", (rows, N), y.dtype), N, K, dt, odt, stream_ptr(stream)), "spmm_grouped_mm")
+    check(lib().spmm_grouped_mm(_flat(offsets, "offsets", (groups + 1,), _torch.int32, dev), groups, rows, x.data_ptr(),
+                                _rows(x, "x", (rows, K), x.dtype, dev), _flat(w, "w", w.shape, x.dtype, dev), y.data_ptr(),
+                                _rows(y, "y", (rows, N), y.dtype, dev), N, K, _value_dtype(x, "x"), _value_dtype(y, "y", True),
+                                stream_ptr(stream)), "spmm_grouped_mm")
 
 
 def grouped_mm_dx(offsets, dy, w, dx, stream=None) -> None:
     """dx[p] = w[g]^T dy[p]; dy (rows, N), w (groups, N, K), dx (rows, K) of dy's type or float32."""
-    import torch
-
+    dev = _device(offsets)
     groups, N, K = w.shape
     rows = dy.shape[0]
-    dt, odt = _value_dtype(dy, "dy"), _value_dtype(dx, "dx", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
-    check(lib().spmm_grouped_mm_dx(_flat(offsets, "offsets", (groups + 1,), torch.int32), groups, rows, dy.data_ptr(),
-                                   _rows(dy, "dy", (rows, N), dy.dtype), _flat(w, "w", (groups, N, K), dy.dtype), dx.data_ptr(),
-                                   _rows(dx, "dx", (rows, K), dx.dtype), N, K, dt, odt, stream_ptr(stream)), "spmm_grouped_mm_dx")
+    check(lib().spmm_grouped_mm_dx(_flat(offsets, "offsets", (groups + 1,), _torch.int32, dev), groups, rows, dy.data_ptr(),
+                                   _rows(dy, "dy", (rows, N), dy.dtype, dev), _flat(w, "w", w.shape, dy.dtype, dev), dx.data_ptr(),
+                                   _rows(dx, "dx", (rows, K), dx.dtype, dev), N, K, _value_dtype(dy, "dy"),
+                                   _value_dtype(dx, "dx", True), stream_ptr(stream)), "spmm_grouped_mm_dx")
 
 
 def grouped_mm_dw(offsets, dy, x, dw, stream=None) -> None:
     """dw[g] = sum over the group's rows of dy[p] x[p]^T; dw (groups, N, K) of x's type or float32."""
-    import torch
-
+    dev = _device(offsets)
     groups, N, K = dw.shape
     rows = x.shape[0]
-    dt, odt = _value_dtype(x, "x"), _value_dtype(dw, "dw", (DTYPE_F16, DTYPE_BF16, DTYPE_F32))
-    check(lib().spmm_grouped_mm_dw(_flat(offsets, "offsets", (groups + 1,), torch.int32), groups, rows, dy.data_ptr(),
-                                   _rows(dy, "dy", (rows, N), x.dtype), x.data_ptr(), _rows(x, "x", (rows, K), x.dtype),
-                                   _flat(dw, "dw", (groups, N, K), dw.dtype), N, K, dt, odt, stream_ptr(stream)), "spmm_grouped_mm_dw")
+    check(lib().spmm_grouped_mm_dw(_flat(offsets, "offsets", (groups + 1,), _torch.int32, dev), groups, rows, dy.data_ptr(),
+                                   _rows(dy, "dy", (rows, N), x.dtype, dev), x.data_ptr(), _rows(x, "x", (rows, K), x.dtype, dev),
+                                   _flat(dw, "dw", dw.shape, dw.dtype, dev), N, K, _value_dtype(x, "x"), _value_dtype(dw, "dw", True),
+                                   stream_ptr(stream)), "spmm_grouped_mm_dw")
 
 
-def _lora_view(a, b, scale) -> LoraView:
-    import torch
-
+def _lora_view(a, b, scale, dev: int) -> LoraView:
     adapters, rank, K = a.shape
     N = b.shape[1]
-    dt = _value_dtype(a, "a")
-    return LoraView(adapters, rank, N, K, dt, _flat(a, "a", (adapters, rank, K), a.dtype), _flat(b, "b", (adapters, N, rank), a.dtype),
-                    _flat(scale, "scale", (adapters,), torch.float32))
+    return LoraView(adapters, rank, N, K, _value_dtype(a, "a"), _flat(a, "a", a.shape, a.dtype, dev),
+                    _flat(b, "b", (adapters, N, rank), a.dtype, dev), _flat(scale, "scale", (adapters,), _torch.float32, dev))
 
 
 def lora_workspace_size(a, b, requests: int, rows: int) -> int:
-    v = _lora_view(a, b, None)
+    v = _lora_view(a, b, None, _device(a))
     n = C.c_size_t()
-    check(lib().spmm_lora_workspace_size(C.byref(v), requests, rows, C.byref(n)), "spmm_lora_workspace_size")
-    return int(n.value)
+    check(lib().spmm_lora_workspace_size(v, requests, rows, C.byref(n)), "spmm_lora_workspace_size")
+    return n.value
 
 
 def lora(offsets, adapter, x, a, b, out, base=None, scale=None, ws=None, stream=None) -> None:
     """out[p] = base[p] + scale * b (a x[p]) with the matrices of adapter[r], offsets[r] <= p < offsets[r + 1] (offsets None: every
     row a request of its own); x (rows, K), a (adapters, rank, K), b (adapters, N, rank), base and out (rows, N)."""
-    import torch
-
-    v = _lora_view(a, b, scale)
+    dev = _device(adapter)
+    v = _lora_view(a, b, scale, dev)
     rows, requests = x.shape[0], adapter.shape[0]
     n = C.c_size_t()
-    check(lib().spmm_lora_workspace_size(C.byref(v), requests, rows, C.byref(n)), "spmm_lora_workspace_size")
-    _ws, wp, wn = _workspace(ws, int(n.value), stream)
-    check(lib().spmm_lora(C.byref(v), _flat(offsets, "offsets", (requests + 1,), torch.int32),
-                          _flat(adapter, "adapter", (requests,), torch.int32), requests, rows, x.data_ptr(),
-                          _rows(x, "x", (rows, v.K), a.dtype), ptr(base), _rows(base, "base", (rows, v.N), a.dtype) if base is not None else 0,
-                          out.data_ptr(), _rows(out, "out", (rows, v.N), a.dtype), wp, wn, stream_ptr(stream)), "spmm_lora")
+    check(lib().spmm_lora_workspace_size(v, requests, rows, C.byref(n)), "spmm_lora_workspace_size")
+    sp, wide = stream_ptr(stream), (rows, v.N)
+    _ws, wp, wn = _workspace(ws, n.value, sp, dev)
+    check(lib().spmm_lora(v, _flat(offsets, "offsets", (requests + 1,), _torch.int32, dev),
+                          _flat(adapter, "adapter", (requests,), _torch.int32, dev), requests, rows, x.data_ptr(),
+                          _rows(x, "x", (rows, v.K), a.dtype, dev), ptr(base), _rows(base, "base", wide, a.dtype, dev) if base is not None else 0,
+                          out.data_ptr(), _rows(out, "out", wide, a.dtype, dev), wp, wn, sp), "spmm_lora")
