@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     if (warp == 0) {
         // ---------------- producer
-        if (lane == 0) {
+        if (elect_one()) {
             int it = 0;
             bool ok = true;
             for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
     } else if (warp == 1) {
-        // ---------------- MMA issuer (lane 0; the whole warp clears rows past a group's end in dw)
+        // ---------------- MMA issuer (one lane; the whole warp clears rows past a group's end in dw)
         const uint32_t idesc = instr_desc_f16(a.dtype, TN, FORM == kDw, FORM != kForward);
         int it = 0, n = 0;
         bool ok = true;
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
                 tc_fence_after();
-                if (lane == 0) {
+                if (elect_one()) {
                     const uint32_t sa = sbase + s * L::kStage, sb = sa + L::kA;
                     for (int j = 0; j < slices; ++j) {
                         const uint64_t da = FORM == kDw ? smem_desc(sa + 2048 * j, 8192, 1024, kSwizzle128)
@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 __syncwarp();
             }
-            if (lane == 0) umma_commit(acc_full0 + 8 * buf);
+            if (elect_one()) umma_commit(acc_full0 + 8 * buf);
+            __syncwarp();
         }
         if (!ok && lane == 0) {
             *abort_flag = 1;
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tc_fence_after();
         if (*abort_flag) {
             // MMAs still in flight end before their accumulators are given back.
-            if (lane == 0) {
+            if (elect_one()) {
                 umma_commit(drain);
                 const unsigned long long t0 = global_ns();
                 while (!mbar_try_wait(drain, 0) && global_ns() - t0 < kWaitNs) {

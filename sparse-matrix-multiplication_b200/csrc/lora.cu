@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
 
     if (warp == 0) {
         // ---------------- producer
-        if (lane == 0) {
+        if (elect_one()) {
             int it = 0;
             bool ok = true;
             for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer
-        if (lane == 0) {
+        if (elect_one()) {
             const uint32_t idesc = instr_desc_f16(DT, kTn, false, false);
             const int slices = (a.rank + 15) / 16;
             int it = 0, nu = 0, n = 0;
@@ -471,7 +471,6 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     } else {
         // ---------------- u: sum of the parts -> hi + lo
         grid_dependency_wait();
-        const int row = (warp - 6) * 32 + lane;
         const int pieces = (a.rank + 15) / 16 * 2;  // 8 ranks each; the last may lie past the rank and is zero
         int nu = 0;
         bool ok = true;
@@ -483,32 +482,49 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                 ok = false;
                 break;
             }
-            if (row < x.rows) {
-                uint8_t* hi = base + ub * L::kU + row * 128;
-                const float* part = a.u + static_cast<long long>(x.row + row) * a.rank;
-                const long long stride = static_cast<long long>(a.rows) * a.rank;
-                for (int c = 0; c < pieces; ++c) {
-                    float f[8] = {};
-                    if (8 * c < a.rank) {
-                        for (int k = 0; k < e.splits; ++k) {
-                            const float4* src = reinterpret_cast<const float4*>(part + k * stride + 8 * c);
-                            const float4 lo4 = src[0], hi4 = src[1];
-                            f[0] += lo4.x, f[1] += lo4.y, f[2] += lo4.z, f[3] += lo4.w;
-                            f[4] += hi4.x, f[5] += hi4.y, f[6] += hi4.z, f[7] += hi4.w;
-                        }
+            // Pieces of 8 ranks, taken by consecutive threads; four at a time so that their loads overlap.
+            uint8_t* hi = base + ub * L::kU;
+            const float* parts = a.u + static_cast<long long>(x.row) * a.rank;
+            const long long stride = static_cast<long long>(a.rows) * a.rank;
+            for (int first = (warp - 6) * 32 + lane; first < x.rows * pieces; first += 4 * 128) {
+                float f[4][8] = {};
+                int row[4], piece[4];
+                bool real[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    row[j] = (first + 128 * j) / pieces;
+                    piece[j] = first + 128 * j - row[j] * pieces;
+                    real[j] = row[j] < x.rows && 8 * piece[j] < a.rank;
+                }
+                for (int k = 0; k < e.splits; ++k) {
+                    float4 v[4][2];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float4* src = reinterpret_cast<const float4*>(parts + k * stride + static_cast<long long>(row[j]) * a.rank + 8 * piece[j]);
+                        if (real[j]) v[j][0] = src[0], v[j][1] = src[1];
                     }
-                    const uint4 top = RowVec<DT, 16>::pack(f);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (!real[j]) continue;
+                        f[j][0] += v[j][0].x, f[j][1] += v[j][0].y, f[j][2] += v[j][0].z, f[j][3] += v[j][0].w;
+                        f[j][4] += v[j][1].x, f[j][5] += v[j][1].y, f[j][6] += v[j][1].z, f[j][7] += v[j][1].w;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (row[j] >= x.rows) continue;
+                    const uint4 top = RowVec<DT, 16>::pack(f[j]);
                     float g[8];
                     RowVec<DT, 16>::unpack(top, g);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) g[k] = f[k] - g[k];
+                    for (int k = 0; k < 8; ++k) g[k] = f[j][k] - g[k];
                     const uint4 rest = RowVec<DT, 16>::pack(g);
-                    const int at = c / 8 * 16384 + (((c % 8) ^ (row & 7)) << 4);
+                    const int at = row[j] * 128 + piece[j] / 8 * 16384 + (((piece[j] % 8) ^ (row[j] & 7)) << 4);
                     *reinterpret_cast<uint4*>(hi + at) = top;
                     *reinterpret_cast<uint4*>(hi + RB * 16384 + at) = rest;
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive_count(u_full0 + 8 * ub, 1);
             ++nu;
@@ -524,7 +540,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     if (warp == 1) {
         tc_fence_after();
         // The last commits' arrivals, and after a timeout the MMAs in flight, end before the block gives up its TMEM.
-        if (lane == 0) {
+        if (elect_one()) {
             umma_commit(drain);
             const unsigned long long t0 = global_ns();
             while (!mbar_try_wait(drain, 0) && global_ns() - t0 < kWaitNs) {
@@ -558,8 +574,9 @@ int expand(const ExpandArgs& e0, int64_t mtiles, cudaStream_t s, DeviceState* st
     const int rb = a.rank <= 64 ? 1 : (a.rank <= 128 ? 2 : 4);
     const int tn = rb == 4 ? 64 : 128;
     e.ntiles = (a.N + tn - 1) / tn;
-    // Column tiles of a unit: u is made once for all of them, but every SM should have two units.
-    e.per_unit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, mtiles * e.ntiles / (2 * st->sm_count))));
+    // Column tiles of a unit: u is made once for all of them, but units of one-row requests are cheap and the others
+    // should spread evenly, so every SM gets six.
+    e.per_unit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, mtiles * e.ntiles / (6 * st->sm_count))));
     e.chunks = (e.ntiles + e.per_unit - 1) / e.per_unit;
     const int64_t units = mtiles * e.chunks;
     if (units > INT32_MAX) return SPMM_ERR_TOO_LARGE;
@@ -589,9 +606,9 @@ Shape shape_of(int32_t requests, int32_t rows, int32_t K) {
     Shape h{};
     h.rows = rows <= 4 * static_cast<int64_t>(requests);
     h.mtiles = rows / kTileM + std::min(requests, rows);
-    // Ranges of the sum over K until about two tiles an SM (of 148) are there, each at least 8 steps of 64 long.
+    // Ranges of the sum over K until about six tiles an SM (of 148) are there, each at least 8 steps of 64 long.
     const int steps = (K + 63) / 64;
-    const int64_t want = h.rows ? 1 : std::max<int64_t>(1, std::min<int64_t>({8, 296 / std::max<int64_t>(1, h.mtiles), steps / 8}));
+    const int64_t want = h.rows ? 1 : std::max<int64_t>(1, std::min<int64_t>({8, 888 / std::max<int64_t>(1, h.mtiles), steps / 8}));
     h.steps_per_split = static_cast<int>((steps + want - 1) / want);
     h.splits = h.steps_per_split ? (steps + h.steps_per_split - 1) / h.steps_per_split : 1;
     return h;

@@ -25,6 +25,19 @@ __device__ __forceinline__ unsigned long long global_ns() {
     return t;
 }
 
+// True in one lane of a converged warp, always the same one. The compiler knows that a branch on it has a single thread:
+// tcgen05 and TMA instructions behind `lane == 0` instead are issued from a loop over the warp's possible lanes (116
+// cycles an MMA against 20, measured by clock64 around four of them).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
