@@ -235,6 +235,23 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, int t
     return r;
 }
 
+// The MMAs of one stage, 16 of k each; the first overwrites the accumulator unless `add`.
+template <int FORM, int TN>
+__device__ __forceinline__ void mma_step(uint32_t acc, uint32_t stage, uint32_t idesc, int slices, bool add) {
+    // From one slice to the next: 32 bytes along a K-major row, two 8-row atoms down an MN-major column (units of 16).
+    constexpr uint64_t kNextA = FORM == kDw ? 128 : 2, kNextB = FORM == kForward ? 2 : 128;
+    const uint64_t da = FORM == kDw ? smem_desc(stage, 8192, 1024, kSwizzle128) : smem_desc(stage, 16, 1024, kSwizzle128);
+    const uint32_t sb = stage + TcLayout<TN>::kA;
+    const uint64_t db = FORM == kForward ? smem_desc(sb, 16, 1024, kSwizzle128) : smem_desc(sb, 8192, 1024, kSwizzle128);
+    if (slices == 4) {
+        umma_f16(acc, da, db, idesc, add ? 1u : 0u);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) umma_f16(acc, da + j * kNextA, db + j * kNextB, idesc, 1u);
+    } else {
+        for (int j = 0; j < slices; ++j) umma_f16(acc, da + j * kNextA, db + j * kNextB, idesc, add || j > 0 ? 1u : 0u);
+    }
+}
+
 template <int FORM, int TN>
 __global__ void __launch_bounds__(kTcThreads, 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_small,
@@ -288,7 +305,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (warp == 0) {
         // ---------------- producer
         if (elect_one()) {
-            int it = 0;
+            int it = 0, s = 0;
+            uint32_t phase = 1;
             bool ok = true;
             for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
                 const Tile r = tile_of<FORM, TN>(a, start, t);
@@ -298,13 +316,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int na = min(2, (a.ms - r.m0 + 63) / 64);  // dw
                 const uint32_t bytes = (FORM == kDw ? na * 8192 : (small ? kSmallRows * 128 : L::kA)) + (FORM == kForward ? L::kB : nb * 8192);
                 for (int ks = 0; ks < r.steps; ++ks, ++it) {
-                    const int s = it % kStages;
                     const uint32_t bar = full0 + 8 * s, sa = sbase + s * L::kStage, sb = sa + L::kA;
-                    if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag)) {
+                    if (!mbar_wait(empty0 + 8 * s, phase, abort_flag)) {
                         ok = false;
                         break;
                     }
                     mbar_arrive_expect_tx(bar, bytes);
+                    if (++s == kStages) s = 0, phase ^= 1u;
                     const int k0 = (r.first + ks) * kStepK;
                     if constexpr (FORM == kDw) {
                         for (int j = 0; j < na; ++j) tma_load_2d(sa + j * 8192, &map_a, bar, r.m0 + 64 * j, r.begin + k0);
@@ -332,53 +350,53 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
     } else if (warp == 1) {
-        // ---------------- MMA issuer (one lane; the whole warp clears rows past a group's end in dw)
+        // ---------------- MMA issuer: one lane; in dw the whole warp clears the rows past a group's end
         const uint32_t idesc = instr_desc_f16(a.dtype, TN, FORM == kDw, FORM != kForward);
         int it = 0, n = 0;
         bool ok = true;
         for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++n) {
             const Tile r = tile_of<FORM, TN>(a, start, t);
             const int buf = n & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag))) {
-                ok = false;
-                break;
-            }
-            tc_fence_after();
             const uint32_t acc = tmem + buf * TN;
             const int sum = FORM == kDw ? r.end - r.begin : a.sum;
-            for (int ks = 0; ks < r.steps; ++ks, ++it) {
-                const int s = it % kStages;
-                if (!__all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag))) {
-                    ok = false;
-                    break;
-                }
-                const int left = min(kStepK, sum - (r.first + ks) * kStepK), slices = (left + 15) / 16;
-                if constexpr (FORM == kDw) {
-                    if (left % 16) {
-                        const int nb = min(TN / 64, (a.outs - r.n0 + 63) / 64), na = min(2, (a.ms - r.m0 + 63) / 64);
-                        const int pieces = (slices * 16 - left) * 8;  // 16-byte pieces of a box's rows to clear
-                        uint8_t* st = base + s * L::kStage;
-                        for (int b = 0; b < na + nb; ++b) {
-                            uint4* rows = reinterpret_cast<uint4*>(st + (b < na ? b * 8192 : L::kA + (b - na) * 8192) + left * 128);
-                            for (int i = lane; i < pieces; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                    }
-                }
+            const int left = min(kStepK, sum - (r.first + r.steps - 1) * kStepK);  // of the last step
+            const int clear = FORM == kDw && left % 16 != 0;
+            if (elect_one()) {
+                ok = mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag);
                 tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t sa = sbase + s * L::kStage, sb = sa + L::kA;
-                    for (int j = 0; j < slices; ++j) {
-                        const uint64_t da = FORM == kDw ? smem_desc(sa + 2048 * j, 8192, 1024, kSwizzle128)
-                                                        : smem_desc(sa + 32 * j, 16, 1024, kSwizzle128);
-                        const uint64_t db = FORM == kForward ? smem_desc(sb + 32 * j, 16, 1024, kSwizzle128)
-                                                             : smem_desc(sb + 2048 * j, 8192, 1024, kSwizzle128);
-                        umma_f16(acc, da, db, idesc, ks + j > 0 ? 1u : 0u);
-                    }
+                int s = it % kStages;
+                uint32_t phase = (it / kStages) & 1u;
+                for (int ks = 0; ok && ks < r.steps - clear; ++ks) {
+                    ok = mbar_wait(full0 + 8 * s, phase, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    mma_step<FORM, TN>(acc, sbase + s * L::kStage, idesc, ks == r.steps - 1 ? (left + 15) / 16 : 4, ks > 0);
                     umma_commit(empty0 + 8 * s);
+                    if (++s == kStages) s = 0, phase ^= 1u;
                 }
-                __syncwarp();
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            it += r.steps;
+            if (FORM == kDw && clear && ok) {
+                const int s = (it - 1) % kStages, slices = (left + 15) / 16;
+                ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, ((it - 1) / kStages) & 1u, abort_flag));
+                if (ok) {
+                    const int nb = min(TN / 64, (a.outs - r.n0 + 63) / 64), na = min(2, (a.ms - r.m0 + 63) / 64);
+                    const int pieces = (slices * 16 - left) * 8;  // 16-byte pieces of a box's rows to clear
+                    uint8_t* st = base + s * L::kStage;
+                    for (int b = 0; b < na + nb; ++b) {
+                        uint4* rows = reinterpret_cast<uint4*>(st + (b < na ? b * 8192 : L::kA + (b - na) * 8192) + left * 128);
+                        for (int i = lane; i < pieces; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    tc_fence_after();
+                    if (elect_one()) {
+                        mma_step<FORM, TN>(acc, sbase + s * L::kStage, idesc, slices, r.steps > 1);
+                        umma_commit(empty0 + 8 * s);
+                    }
+                    __syncwarp();
+                }
             }
             if (elect_one()) umma_commit(acc_full0 + 8 * buf);
             __syncwarp();
