@@ -141,7 +141,8 @@ int any_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st)
 //
 // A persistent block takes 128 x TN tiles of D, 64 of k a step: one warp issues TMA copies into a ring of stages, one
 // issues the MMAs (M = 128, N = TN, FP32 accumulators in TMEM, two of them so that the next tile's MMAs run under this
-// one's epilogue), four move TMEM -> registers -> shared memory -> 16-byte stores of whole 128-byte row pieces.
+// one's epilogue), eight move TMEM -> registers -> memory: a lane holds a row's consecutive columns and
+// stores whole 32-byte sectors.
 // x, dy and w are read as they lie: K-major where k is the contiguous index (both operands of the forward product,
 // dx's A), MN-major where it is not (dx's B, both of dw's), so nothing is transposed in memory.
 // Ragged groups: a row tile may reach past its group. Rows of D past it are computed and not stored (rows do not mix
@@ -151,7 +152,7 @@ int any_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st)
 constexpr int kTileM = 128;
 constexpr int kStepK = 64;
 constexpr int kBand = 8;          // row tiles that run together down a band (their A and the band's B stay in L2)
-constexpr int kTcThreads = 192;   // warp 0 TMA, warp 1 MMA, warps 2..5 epilogue
+constexpr int kTcThreads = 320;   // warp 0 TMA, warp 1 MMA, warps 2..9 epilogue
 constexpr int kSmallRows = 32;    // groups with no more rows left load a box of this many
 
 template <int TN>
@@ -159,9 +160,8 @@ struct TcLayout {
     static constexpr int kA = kTileM * kStepK * 2;
     static constexpr int kB = TN * kStepK * 2;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = TN == 256 ? 4 : (TN == 128 ? 6 : 8);
-    static constexpr int kOut = kStages * kStage;    // 4 warps x 32 rows x 128 bytes
-    static constexpr int kBars = kOut + 4 * 4096;    // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
+    static constexpr int kStages = TN == 256 ? 4 : (TN == 128 ? 6 : 8);  // 192 KB
+    static constexpr int kBars = kStages * kStage;    // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
     static constexpr int kTable = kBars + 8 * (2 * kStages + 5) + 16;
     static constexpr int kFixed = kTable + 1024;     // room to align the base to 1 KB; then int[groups + 1]
 };
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(acc_full0 + 8 * s, 1);
-            mbar_init(acc_empty0 + 8 * s, 4);
+            mbar_init(acc_empty0 + 8 * s, 8);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -406,10 +406,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             record_device_error(a.err, SPMM_ERR_TIMEOUT, 12);
         }
     } else {
-        // ---------------- epilogue
-        const int q = warp & 3;  // TMEM lane quarter this warp may access
-        uint8_t* stage = base + L::kOut + q * 4096;
-        const int size = a.out_f32 ? 4 : 2, per = 128 / size;  // columns of a 128-byte row piece
+        // ---------------- epilogue: two warps a lane quarter, alternate 32-column pieces
+        const int q = warp & 3, half = (warp - 2) >> 2;  // warps q and q + 4 may access TMEM lanes 32 q ..
+        const int size = a.out_f32 ? 4 : 2;
+        const bool sectors = (reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) % 32 == 0;
         int n = 0;
         bool ok = true;
         for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
@@ -421,53 +421,46 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             tc_fence_after();
             const uint32_t acc = tmem + buf * TN + (static_cast<uint32_t>(q * 32) << 16);
-            const int rows = min(32, (FORM == kDw ? a.ms : r.end - r.begin) - r.m0 - q * 32);
-            const long long first = FORM == kDw ? static_cast<long long>(r.g) * a.ms + r.m0 + q * 32 : r.begin + r.m0 + q * 32;
-            char* out = static_cast<char*>(a.out) + (first * a.ldo + r.n0 + r.split * a.split_stride) * size;
-            const int cols = min(TN, a.outs - r.n0);
-            if (rows > 0) {
-                for (int c0 = 0; c0 < cols; c0 += per) {
+            const int row = r.m0 + q * 32 + lane, rows = FORM == kDw ? a.ms : r.end - r.begin;
+            const long long at = FORM == kDw ? static_cast<long long>(r.g) * a.ms + row : r.begin + row;
+            char* out = static_cast<char*>(a.out) + (at * a.ldo + r.n0 + r.split * a.split_stride) * size;
+            const int cols = min(TN, a.outs - r.n0);  // a multiple of 8
+            if (r.m0 + q * 32 < rows) {
+                for (int c0 = half * 32; c0 < cols; c0 += 64) {
+                    uint32_t v[32];
+                    tmem_ld32(acc + c0, v);
+                    if (FORM == kDw && r.steps == 0) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (a.out_f32 && h) continue;
-                        uint32_t v[32];
-                        if (FORM == kDw && r.steps == 0) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = 0u;
-                        } else {
-                            tmem_ld32(acc + c0 + 32 * h, v);
-                        }
-                        if (a.out_f32) {
-#pragma unroll
-                            for (int c = 0; c < 8; ++c)
-                                *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) =
-                                    make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const float lo = __uint_as_float(v[8 * c + 2 * i]), hi = __uint_as_float(v[8 * c + 2 * i + 1]);
-                                    w[i] = a.dtype == SPMM_DTYPE_BF16 ? pack_half2<SPMM_DTYPE_BF16>(lo, hi) : pack_half2<SPMM_DTYPE_F16>(lo, hi);
-                                }
-                                *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * h + c) ^ (lane & 7)) << 4)) =
-                                    make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                        }
+                        for (int i = 0; i < 32; ++i) v[i] = 0u;
                     }
-                    __syncwarp();
-                    const int c = lane & 7, col = c0 + c * (16 / size);
+                    if (row >= rows) {
+                        // nothing to store
+                    } else if (a.out_f32) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int row = 4 * i + (lane >> 3);
-                        if (row < rows && col < cols)
-                            *reinterpret_cast<uint4*>(out + (row * a.ldo + col) * size) =
-                                *reinterpret_cast<const uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) w[i] = v[8 * c + i];
+                            if (c0 + 8 * c < cols) store_32(out + (c0 + 8 * c) * 4, w, sectors);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float lo = __uint_as_float(v[16 * c + 2 * i]), hi = __uint_as_float(v[16 * c + 2 * i + 1]);
+                                w[i] = a.dtype == SPMM_DTYPE_BF16 ? pack_half2<SPMM_DTYPE_BF16>(lo, hi) : pack_half2<SPMM_DTYPE_F16>(lo, hi);
+                            }
+                            const int col = c0 + 16 * c;
+                            if (col + 16 <= cols) store_32(out + col * 2, w, sectors);
+                            else if (col < cols) *reinterpret_cast<uint4*>(out + col * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
                     }
                     __syncwarp();
                 }
             }
+            __syncwarp();
             tc_fence_before();
             if (lane == 0) mbar_arrive_count(acc_empty0 + 8 * buf, 1);
         }
@@ -514,7 +507,7 @@ int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap
 
 bool fits16(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
 
-// Whether TMA and 16-byte stores can address the operands.
+// Whether TMA and stores of 16 bytes can address the operands.
 template <int FORM>
 bool tc_fits(const GroupedArgs& a, DeviceState* st) {
     if (st->cc_major != 10 || a.N % 8 || a.K % 8 || a.rows == 0 || a.N == 0 || a.K == 0) return false;

@@ -225,13 +225,13 @@ __global__ void __launch_bounds__(256) lora_expand_rows_kernel(LoraArgs a, int c
 // little: a persistent block holds u of a 128-row tile in shared memory and streams b and base past it.
 //   warp 0      TMA: b (TN features x rank) and the base tile (128 x TN) into a ring of stages
 //   warp 1      MMA: D = u b^T in TMEM, two accumulators
-//   warps 2..5  D * scale + base -> the base's place in the stage -> 16-byte stores of 128-byte row pieces
-//   warps 6..9  the next tile's u: the parts' sum as two 16-bit terms, hi + lo, K-major under the 128-byte swizzle
+//   warps 2..9  D * scale + base (from the stage) -> 32-byte stores
+//   warps 10..13  the next tile's u: the parts' sum as two 16-bit terms, hi + lo, K-major under the 128-byte swizzle
 // The MMA needs 16-bit u; one term would cost half a step of 16 bits in every product (2^-8 in bf16), two leave 2^-16
 // for twice the MMAs, which still run under the copies.
 
 constexpr int kTileM = 128;
-constexpr int kExpandThreads = 320;
+constexpr int kExpandThreads = 448;
 constexpr int kSmallRows = 8;  // requests with no more rows load a base box of this many
 
 template <int RB>  // rank in blocks of 64
@@ -297,13 +297,13 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         *abort_flag = 0;
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, 4);
+            mbar_init(empty0 + 8 * s, 8);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(u_full0 + 8 * s, 4);
             mbar_init(u_empty0 + 8 * s, 1);
             mbar_init(acc_full0 + 8 * s, 1);
-            mbar_init(acc_empty0 + 8 * s, 4);
+            mbar_init(acc_empty0 + 8 * s, 8);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -400,15 +400,15 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp < 6) {
-        // ---------------- epilogue
-        const int q = warp & 3;
+    } else if (warp < 10) {
+        // ---------------- epilogue: two warps a lane quarter, alternate 32-column pieces
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const bool sectors = (reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldout * 2)) % 32 == 0;
         int it = 0, n = 0;
         bool ok = true;
         for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
             const Unit x = unit_of(e, start, u);
             const float scale = x.i >= 0 && a.scale ? __ldg(a.scale + x.i) : 1.f;
-            const int rows = min(32, x.rows - q * 32);
             for (int nt = x.nt0; nt < x.nt1; ++nt, ++it) {
                 const int s = it % kStages, buf = n & 1;
                 bool got = mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag);
@@ -419,41 +419,37 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                 }
                 tc_fence_after();
                 const int cols = min(kTn, a.N - nt * kTn);
-                if (rows > 0) {
-                    for (int c0 = 0; c0 < cols; c0 += 64) {
-                        uint8_t* block = base + L::kStage0 + s * L::kStage + L::kB + c0 / 64 * 16384 + q * 4096;
+                // A block of 64 columns is 16 KB of the stage; a warp takes half of each, 32 columns.
+                for (int c0 = 32 * half; q * 32 < x.rows && c0 < cols; c0 += 64) {
+                    uint8_t* block = base + L::kStage0 + s * L::kStage + L::kB + c0 / 64 * 16384 + q * 4096;
+                    uint4 b8[4];
+                    if (a.base) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t v[32];
-                            if (x.i >= 0) {
-                                tmem_ld32(tmem + buf * kTn + c0 + 32 * h + (static_cast<uint32_t>(q * 32) << 16), v);
-                            } else {
-#pragma unroll
-                                for (int k = 0; k < 32; ++k) v[k] = 0u;
-                            }
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                uint4* at = reinterpret_cast<uint4*>(block + lane * 128 + (((4 * h + c) ^ (lane & 7)) << 4));
-                                float f[8] = {};
-                                if (a.base) RowVec<DT, 16>::unpack(*at, f);
-                                if (x.i >= 0) {
-#pragma unroll
-                                    for (int k = 0; k < 8; ++k) f[k] = fmaf(__uint_as_float(v[8 * c + k]), scale, f[k]);
-                                }
-                                *at = RowVec<DT, 16>::pack(f);
-                            }
-                        }
-                        __syncwarp();
-                        const int c = lane & 7, col = c0 + 8 * c;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int row = 4 * k + (lane >> 3);
-                            if (row < rows && col < cols)
-                                *reinterpret_cast<uint4*>(a.out + (x.row + q * 32 + row) * a.ldout + nt * kTn + col) =
-                                    *reinterpret_cast<const uint4*>(block + row * 128 + ((c ^ (row & 7)) << 4));
-                        }
+                        for (int c = 0; c < 4; ++c) b8[c] = *swizzled_piece(block, lane, 4 * half + c);
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before TMA writes the stage again
+                    uint32_t v[32];
+                    if (x.i >= 0) tmem_ld32(tmem + buf * kTn + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
+                    uint16_t* out = a.out + (x.row + q * 32 + lane) * a.ldout + nt * kTn + c0;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float f[8] = {};
+                            if (a.base) RowVec<DT, 16>::unpack(b8[2 * h + c], f);
+                            if (x.i >= 0) {
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) f[k] = fmaf(__uint_as_float(v[16 * h + 8 * c + k]), scale, f[k]);
+                            }
+                            const uint4 o = RowVec<DT, 16>::pack(f);
+                            w[4 * c] = o.x, w[4 * c + 1] = o.y, w[4 * c + 2] = o.z, w[4 * c + 3] = o.w;
+                        }
+                        const int col = c0 + 16 * h;
+                        if (q * 32 + lane >= x.rows || col >= cols) continue;
+                        if (col + 16 <= cols) store_32(out + 16 * h, w, sectors);
+                        else *reinterpret_cast<uint4*>(out + 16 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    __syncwarp();
                 }
                 __syncwarp();
                 tc_fence_before();
@@ -486,7 +482,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             uint8_t* hi = base + ub * L::kU;
             const float* parts = a.u + static_cast<long long>(x.row) * a.rank;
             const long long stride = static_cast<long long>(a.rows) * a.rank;
-            for (int first = (warp - 6) * 32 + lane; first < x.rows * pieces; first += 4 * 128) {
+            for (int first = (warp - 10) * 32 + lane; first < x.rows * pieces; first += 4 * 128) {
                 float f[4][8] = {};
                 int row[4], piece[4];
                 bool real[4];

@@ -149,6 +149,23 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// A 16-byte piece of a row of 128 bytes in shared memory, as TMA's 128-byte swizzle places it.
+__device__ __forceinline__ uint4* swizzled_piece(uint8_t* block, int row, int piece) {
+    return reinterpret_cast<uint4*>(block + row * 128 + ((piece ^ (row & 7)) << 4));
+}
+
+// 32 bytes of a row from one thread: a whole sector in one store where the address allows, else two halves.
+__device__ __forceinline__ void store_32(void* at, const uint32_t (&w)[8], bool aligned) {
+    if (aligned) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                     "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(at)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(at)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+}
+
 // Shared-memory matrix descriptor (tcgen05 "version 1" format): start address, leading and
 // stride byte offsets (16-byte units), swizzle mode in bits 61..63.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, uint64_t swizzle) {
