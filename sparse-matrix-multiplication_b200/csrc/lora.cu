@@ -223,15 +223,18 @@ __global__ void __launch_bounds__(256) lora_expand_rows_kernel(LoraArgs a, int c
 // Shrink is the grouped product's kernel on 128-row tiles of the requests, its sum over K cut so that few tiles still
 // fill the GPU (partial_products; FP32 parts in the workspace). Expand moves base and out (2 x rows x N) and computes
 // little: a persistent block holds u of a 128-row tile in shared memory and streams b and base past it.
-//   warp 0      TMA: b (TN features x rank) and the base tile (128 x TN) into a ring of stages
-//   warp 1      MMA: D = u b^T in TMEM, two accumulators
-//   warps 2..9  D * scale + base (from the stage) -> 32-byte stores
-//   warps 10..13  the next tile's u: the parts' sum as two 16-bit terms, hi + lo, K-major under the 128-byte swizzle
+//   warp 0        TMA: b (TN features x rank) and the base tile (128 x TN) into a ring of stages, with what they are
+//   warp 1        MMA: D = u b^T in TMEM, two accumulators
+//   warps 2..17   D * scale + base (from the stage) -> 32-byte stores; a warp has 32 rows x 32 columns, which is mostly
+//                 latency: with 8 warps and twice the columns a tile took 2600 cycles, more than its bytes need (2800
+//                 at 1.9 GHz less the start of every unit)
+//   warps 18..21  the next tile's u: the parts' sum as two 16-bit terms, hi + lo, K-major under the 128-byte swizzle
 // The MMA needs 16-bit u; one term would cost half a step of 16 bits in every product (2^-8 in bf16), two leave 2^-16
 // for twice the MMAs, which still run under the copies.
 
 constexpr int kTileM = 128;
-constexpr int kExpandThreads = 448;
+constexpr int kEpilogueWarps = 16;
+constexpr int kExpandThreads = (2 + kEpilogueWarps + 4) * 32;
 constexpr int kSmallRows = 8;  // requests with no more rows load a base box of this many
 
 template <int RB>  // rank in blocks of 64
@@ -245,7 +248,8 @@ struct ExpandLayout {
     static constexpr int kStages = RB == 1 ? 3 : (RB == 2 ? 2 : 1);
     static constexpr int kStage0 = kUs * kU;
     static constexpr int kBars = kStage0 + kStages * kStage;  // full[], empty[], u_full[2], u_empty[2], acc_full[2], acc_empty[2], drain
-    static constexpr int kSlot = kBars + 8 * (2 * kStages + 9);
+    static constexpr int kInfo = kBars + 8 * (2 * kStages + 9);  // StageInfo[kStages]
+    static constexpr int kSlot = kInfo + 32 * kStages;
     static constexpr int kTable = kSlot + 8;
     static constexpr int kFixed = kTable + 1024;
 };
@@ -260,6 +264,16 @@ struct Unit {
     int i;             // adapter, -1 none
     int row, rows;     // first row, rows of the tile
     int nt0, nt1;      // column tiles
+};
+
+// What a stage holds, from the producer, which runs ahead: finding a unit is a search and three loads that depend on
+// one another, 1400 cycles that the other roles do not wait for.
+struct StageInfo {
+    int rows;          // 0: no more stages
+    int row, i, nt;
+    float scale;
+    int first, last;   // tile of its unit
+    int pad;
 };
 
 __device__ __forceinline__ Unit unit_of(const ExpandArgs& e, const int* start, int u) {
@@ -290,6 +304,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                    acc_full0 = u_empty0 + 16, acc_empty0 = acc_full0 + 16, drain = acc_empty0 + 16;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kSlot);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    StageInfo* infos = reinterpret_cast<StageInfo*>(base + L::kInfo);
     int* start = reinterpret_cast<int*>(base + L::kTable);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -297,13 +312,13 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         *abort_flag = 0;
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, 8);
+            mbar_init(empty0 + 8 * s, kEpilogueWarps);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(u_full0 + 8 * s, 4);
             mbar_init(u_empty0 + 8 * s, 1);
             mbar_init(acc_full0 + 8 * s, 1);
-            mbar_init(acc_empty0 + 8 * s, 8);
+            mbar_init(acc_empty0 + 8 * s, kEpilogueWarps);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -326,25 +341,42 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         if (elect_one()) {
             int it = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                const Unit x = unit_of(e, start, u);
+            for (int u = blockIdx.x;; u += gridDim.x) {
+                Unit x{};
+                StageInfo info{};
+                const bool end = u >= units;
+                if (!end) {
+                    x = unit_of(e, start, u);
+                    info.rows = x.rows;
+                    info.row = x.row;
+                    info.i = x.i;
+                    info.scale = x.i >= 0 && a.scale ? __ldg(a.scale + x.i) : 1.f;
+                }
                 const bool small = x.rows <= kSmallRows;
-                for (int nt = x.nt0; nt < x.nt1; ++nt, ++it) {
+                for (int nt = x.nt0; end ? nt == x.nt0 : nt < x.nt1; ++nt, ++it) {
                     const int s = it % kStages;
                     const uint32_t bar = full0 + 8 * s, sb = sbase + L::kStage0 + s * L::kStage, sbs = sb + L::kB;
                     if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag)) {
                         ok = false;
                         break;
                     }
+                    info.nt = nt;
+                    info.first = nt == x.nt0;
+                    info.last = nt == x.nt1 - 1;
+                    infos[s] = info;
                     const int n0 = nt * kTn, blocks = min(kTn / 64, (a.N - n0 + 63) / 64);
-                    const uint32_t bytes = (x.i >= 0 ? L::kB : 0) + (a.base ? blocks * (small ? kSmallRows * 128 : 16384) : 0);
-                    mbar_arrive_expect_tx(bar, bytes);
+                    if (end) {
+                        mbar_arrive_count(bar, 1);
+                        continue;
+                    }
+                    mbar_arrive_expect_tx(bar, (x.i >= 0 ? L::kB : 0) + (a.base ? blocks * (small ? kSmallRows * 128 : 16384) : 0));
                     if (x.i >= 0)
                         for (int k = 0; k < RB; ++k) tma_load_3d(sb + k * kTn * 128, &map_b, bar, 64 * k, n0, x.i);
                     if (a.base)
                         for (int k = 0; k < blocks; ++k)
                             tma_load_2d(sbs + k * 16384, small ? &map_base_small : &map_base, bar, n0 + 64 * k, x.row);
                 }
+                if (end || !ok) break;
             }
             if (!ok) {
                 *abort_flag = 1;
@@ -361,38 +393,31 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         if (elect_one()) {
             const uint32_t idesc = instr_desc_f16(DT, kTn, false, false);
             const int slices = (a.rank + 15) / 16;
-            int it = 0, nu = 0, n = 0;
+            int nu = 0, n = 0;
             bool ok = true;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                const Unit x = unit_of(e, start, u);
-                if (x.i < 0) {
-                    it += x.nt1 - x.nt0;
-                    continue;
-                }
-                const int ub = nu % kUs;
-                if (!mbar_wait(u_full0 + 8 * ub, (nu / kUs) & 1u, abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                for (int nt = x.nt0; nt < x.nt1; ++nt, ++it, ++n) {
-                    const int s = it % kStages, buf = n & 1;
-                    if (!mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag) ||
-                        !mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag)) {
-                        ok = false;
-                        break;
+            for (int it = 0;; ++it) {
+                const int s = it % kStages, buf = n & 1, ub = nu % kUs;
+                ok = mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag);
+                if (!ok || infos[s].rows == 0) break;
+                if (infos[s].i < 0) continue;
+                ok = mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag) &&
+                     (!infos[s].first || mbar_wait(u_full0 + 8 * ub, (nu / kUs) & 1u, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t su = sbase + ub * L::kU, sb = sbase + L::kStage0 + s * L::kStage;
+                const uint32_t acc = tmem + buf * kTn;
+                for (int t = 0; t < 2; ++t)
+                    for (int k = 0; k < slices; ++k) {
+                        const uint64_t da = smem_desc(su + (t * RB + k / 4) * 16384 + 32 * (k % 4), 16, 1024, kSwizzle128);
+                        const uint64_t db = smem_desc(sb + k / 4 * kTn * 128 + 32 * (k % 4), 16, 1024, kSwizzle128);
+                        umma_f16(acc, da, db, idesc, t + k > 0 ? 1u : 0u);
                     }
-                    tc_fence_after();
-                    const uint32_t su = sbase + ub * L::kU, sb = sbase + L::kStage0 + s * L::kStage;
-                    for (int t = 0; t < 2; ++t)
-                        for (int k = 0; k < slices; ++k) {
-                            const uint64_t da = smem_desc(su + (t * RB + k / 4) * 16384 + 32 * (k % 4), 16, 1024, kSwizzle128);
-                            const uint64_t db = smem_desc(sb + k / 4 * kTn * 128 + 32 * (k % 4), 16, 1024, kSwizzle128);
-                            umma_f16(tmem + buf * kTn, da, db, idesc, t + k > 0 ? 1u : 0u);
-                        }
-                    umma_commit(acc_full0 + 8 * buf);
+                umma_commit(acc_full0 + 8 * buf);
+                ++n;
+                if (infos[s].last) {
+                    umma_commit(u_empty0 + 8 * ub);
+                    ++nu;
                 }
-                umma_commit(u_empty0 + 8 * ub);
-                ++nu;
             }
             if (!ok) {
                 *abort_flag = 1;
@@ -400,65 +425,64 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp < 10) {
-        // ---------------- epilogue: two warps a lane quarter, alternate 32-column pieces
-        const int q = warp & 3, half = (warp - 2) >> 2;
+    } else if (warp < 2 + kEpilogueWarps) {
+        // ---------------- epilogue: four warps a lane quarter, 32 columns each
+        const int q = warp & 3, c0 = (warp - 2) / 4 * 32;
         const bool sectors = (reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldout * 2)) % 32 == 0;
-        int it = 0, n = 0;
+        int n = 0;
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-            const Unit x = unit_of(e, start, u);
-            const float scale = x.i >= 0 && a.scale ? __ldg(a.scale + x.i) : 1.f;
-            for (int nt = x.nt0; nt < x.nt1; ++nt, ++it) {
-                const int s = it % kStages, buf = n & 1;
-                bool got = mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag);
-                if (x.i >= 0) got = got && mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag);
-                if (!__all_sync(0xffffffffu, got)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const int cols = min(kTn, a.N - nt * kTn);
-                // A block of 64 columns is 16 KB of the stage; a warp takes half of each, 32 columns.
-                for (int c0 = 32 * half; q * 32 < x.rows && c0 < cols; c0 += 64) {
-                    uint8_t* block = base + L::kStage0 + s * L::kStage + L::kB + c0 / 64 * 16384 + q * 4096;
-                    uint4 b8[4];
-                    if (a.base) {
+        for (int it = 0;; ++it) {
+            const int s = it % kStages, buf = n & 1;
+            ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag));
+            if (!ok) break;
+            const StageInfo x = infos[s];
+            if (x.rows == 0) break;
+            const int cols = min(kTn, a.N - x.nt * kTn);
+            const bool some = q * 32 < x.rows && c0 < cols, has = x.i >= 0;
+            // A block of 64 columns is 16 KB of the stage.
+            uint8_t* block = base + L::kStage0 + s * L::kStage + L::kB + c0 / 64 * 16384 + q * 4096;
+            uint4 b8[4];
+            if (a.base && some) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) b8[c] = *swizzled_piece(block, lane, 4 * half + c);
-                    }
-                    uint32_t v[32];
-                    if (x.i >= 0) tmem_ld32(tmem + buf * kTn + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
-                    uint16_t* out = a.out + (x.row + q * 32 + lane) * a.ldout + nt * kTn + c0;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float f[8] = {};
-                            if (a.base) RowVec<DT, 16>::unpack(b8[2 * h + c], f);
-                            if (x.i >= 0) {
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) f[k] = fmaf(__uint_as_float(v[16 * h + 8 * c + k]), scale, f[k]);
-                            }
-                            const uint4 o = RowVec<DT, 16>::pack(f);
-                            w[4 * c] = o.x, w[4 * c + 1] = o.y, w[4 * c + 2] = o.z, w[4 * c + 3] = o.w;
-                        }
-                        const int col = c0 + 16 * h;
-                        if (q * 32 + lane >= x.rows || col >= cols) continue;
-                        if (col + 16 <= cols) store_32(out + 16 * h, w, sectors);
-                        else *reinterpret_cast<uint4*>(out + 16 * h) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    __syncwarp();
-                }
-                __syncwarp();
-                tc_fence_before();
-                if (lane == 0) {
-                    mbar_arrive_count(empty0 + 8 * s, 1);
-                    if (x.i >= 0) mbar_arrive_count(acc_empty0 + 8 * buf, 1);
-                }
-                if (x.i >= 0) ++n;
+                for (int c = 0; c < 4; ++c) b8[c] = *swizzled_piece(block, lane, c0 % 64 / 8 + c);
             }
+            uint32_t v[32];
+            if (has) {
+                ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                if (some) tmem_ld32(tmem + buf * kTn + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
+                tc_fence_before();
+            }
+            // The stage and the accumulator are in registers: the next tile's copies and MMAs may begin.
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive_count(empty0 + 8 * s, 1);
+                if (has) mbar_arrive_count(acc_empty0 + 8 * buf, 1);
+            }
+            if (has) ++n;
+            if (some && q * 32 + lane < x.rows) {
+                uint16_t* out = a.out + (x.row + q * 32 + lane) * a.ldout + x.nt * kTn + c0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float f[8] = {};
+                        if (a.base) RowVec<DT, 16>::unpack(b8[2 * h + c], f);
+                        if (has) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) f[k] = fmaf(__uint_as_float(v[16 * h + 8 * c + k]), x.scale, f[k]);
+                        }
+                        const uint4 o = RowVec<DT, 16>::pack(f);
+                        w[4 * c] = o.x, w[4 * c + 1] = o.y, w[4 * c + 2] = o.z, w[4 * c + 3] = o.w;
+                    }
+                    const int col = c0 + 16 * h;
+                    if (col + 16 <= cols) store_32(out + 16 * h, w, sectors);
+                    else if (col < cols) *reinterpret_cast<uint4*>(out + 16 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            __syncwarp();
         }
         if (!ok && lane == 0) {
             *abort_flag = 1;
@@ -478,36 +502,37 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                 ok = false;
                 break;
             }
-            // Pieces of 8 ranks, taken by consecutive threads; four at a time so that their loads overlap.
+            // Pieces of 8 ranks, taken by consecutive threads; kAhead at a time so that their loads overlap.
             uint8_t* hi = base + ub * L::kU;
             const float* parts = a.u + static_cast<long long>(x.row) * a.rank;
             const long long stride = static_cast<long long>(a.rows) * a.rank;
-            for (int first = (warp - 10) * 32 + lane; first < x.rows * pieces; first += 4 * 128) {
-                float f[4][8] = {};
-                int row[4], piece[4];
-                bool real[4];
+            constexpr int kAhead = 2;
+            for (int first = (warp - 2 - kEpilogueWarps) * 32 + lane; first < x.rows * pieces; first += kAhead * 128) {
+                float f[kAhead][8] = {};
+                int row[kAhead], piece[kAhead];
+                bool real[kAhead];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < kAhead; ++j) {
                     row[j] = (first + 128 * j) / pieces;
                     piece[j] = first + 128 * j - row[j] * pieces;
                     real[j] = row[j] < x.rows && 8 * piece[j] < a.rank;
                 }
                 for (int k = 0; k < e.splits; ++k) {
-                    float4 v[4][2];
+                    float4 v[kAhead][2];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < kAhead; ++j) {
                         const float4* src = reinterpret_cast<const float4*>(parts + k * stride + static_cast<long long>(row[j]) * a.rank + 8 * piece[j]);
                         if (real[j]) v[j][0] = src[0], v[j][1] = src[1];
                     }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < kAhead; ++j) {
                         if (!real[j]) continue;
                         f[j][0] += v[j][0].x, f[j][1] += v[j][0].y, f[j][2] += v[j][0].z, f[j][3] += v[j][0].w;
                         f[j][4] += v[j][1].x, f[j][5] += v[j][1].y, f[j][6] += v[j][1].z, f[j][7] += v[j][1].w;
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < kAhead; ++j) {
                     if (row[j] >= x.rows) continue;
                     const uint4 top = RowVec<DT, 16>::pack(f[j]);
                     float g[8];
