@@ -153,6 +153,7 @@ constexpr int kTileM = 128;
 constexpr int kStepK = 64;
 constexpr int kBand = 8;          // row tiles that run together down a band (their A and the band's B stay in L2)
 constexpr int kTcThreads = 320;   // warp 0 TMA, warp 1 MMA, warps 2..9 epilogue
+constexpr int kSingleThreads = 256;  // 8 warps more for the groups of one row
 constexpr int kSmallRows = 32;    // groups with no more rows left load a box of this many
 
 template <int TN>
@@ -183,6 +184,11 @@ struct TcArgs {
     long long split_stride;
     const int* __restrict__ which;
     int matrices;
+    // SINGLES only: the operands themselves.
+    const uint16_t* __restrict__ x;
+    const uint16_t* __restrict__ b;
+    long long ldx;
+    int* singles;      // their number and the groups, for the caller
     DeviceErrorRecord* err;
 };
 
@@ -252,8 +258,34 @@ __device__ __forceinline__ void mma_step(uint32_t acc, uint32_t stage, uint32_t 
     }
 }
 
-template <int FORM, int TN>
-__global__ void __launch_bounds__(kTcThreads, 1)
+// Four results (b's rows q .. q + 3) for the row of a group of one, by one warp.
+template <int DT>
+__device__ __forceinline__ void single_products(const TcArgs& a, int g, int q) {
+    const int lane = threadIdx.x & 31;
+    const long long row = group_range(a.offsets, g, a.rows, nullptr).begin;
+    const int i = group_matrix(a.which, g, a.matrices, nullptr);
+    if (i < 0) return;
+    const int nvec = a.sum / 8;
+    const uint4* x = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+    const uint4* b = reinterpret_cast<const uint4*>(a.b + (static_cast<long long>(i) * a.outs + q) * a.sum);  // outs is a multiple of 8
+    float s[4] = {};
+#pragma unroll 4
+    for (int c = lane; c < nvec; c += 32) {
+        const uint4 v = __ldg(x + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = dot8<DT>(v, __ldg(b + static_cast<long long>(j) * nvec + c), s[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) s[j] += __shfl_xor_sync(0xffffffffu, s[j], d);
+    }
+    if (lane == 0) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * a.ldo + q) = make_float4(s[0], s[1], s[2], s[3]);
+}
+
+// SINGLES (forward, FP32 out): groups of one row are left to eight warps more.
+template <int FORM, int TN, bool SINGLES>
+__global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_small,
                       const __grid_constant__ CUtensorMap map_b, TcArgs a) {
     using L = TcLayout<TN>;
@@ -268,6 +300,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* start = reinterpret_cast<int*>(base + L::kTable);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ int singles;
+    __shared__ uint16_t single[SINGLES ? SPMM_MAX_GROUPS : 1];
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -293,8 +327,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int g = threadIdx.x; g < a.groups; g += kTcThreads) group_range(a.offsets, g, a.rows, a.err);  // records bad ones
         tiles = a.groups * a.mtiles * a.ntiles;
     } else {
-        build_tile_table(start, a.offsets, a.groups, a.rows, kTileM, blockIdx.x == 0 ? a.err : nullptr,
-                         FORM == kForward ? a.which : nullptr, a.matrices);
+        DeviceErrorRecord* err = blockIdx.x == 0 ? a.err : nullptr;
+        if constexpr (SINGLES) {
+            build_table(start, a.groups, [&](int g) {
+                const GroupRange r = group_range(a.offsets, g, a.rows, err);
+                const int rows = r.end - r.begin;
+                single[g] = is_single(r) ? 1 : 0;
+                if (group_matrix(a.which, g, a.matrices, err) < 0 || is_single(r)) return 0;
+                return (rows + kTileM - 1) / kTileM;
+            });
+            if (warp == 2) {
+                // The flags in place to a list in the order of the groups, so that every block has the same.
+                int n = 0;
+                for (int g0 = 0; g0 < a.groups; g0 += 32) {
+                    const unsigned mask = __ballot_sync(0xffffffffu, g0 + lane < a.groups && single[min(g0 + lane, a.groups - 1)]);
+                    if ((mask >> lane) & 1u) single[n + __popc(mask & ((1u << lane) - 1u))] = static_cast<uint16_t>(g0 + lane);
+                    n += __popc(mask);
+                    __syncwarp();
+                }
+                if (lane == 0) singles = n;
+            }
+        } else {
+            build_tile_table(start, a.offsets, a.groups, a.rows, kTileM, err);
+        }
         tiles = start[a.groups] * a.ntiles * (FORM == kForward ? a.splits : 1);
     }
     tc_fence_before();
@@ -405,6 +460,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             *abort_flag = 1;
             record_device_error(a.err, SPMM_ERR_TIMEOUT, 12);
         }
+    } else if (SINGLES && warp >= kTcThreads / 32) {
+        // ---------------- groups of one row, while the tiles stream
+        const int n = singles, quads = a.outs / 4, warps = kSingleThreads / 32;
+        if (blockIdx.x == 0) {
+            const int first = threadIdx.x - kTcThreads;
+            if (first == 0) a.singles[0] = n;
+            for (int k = first; k < n; k += kSingleThreads) a.singles[1 + k] = single[k];
+        }
+        const long long items = static_cast<long long>(n) * quads;
+        for (long long k = static_cast<long long>(blockIdx.x) * warps + warp - kTcThreads / 32; k < items; k += static_cast<long long>(gridDim.x) * warps) {
+            const int m = static_cast<int>(k / quads), q = 4 * static_cast<int>(k - static_cast<long long>(m) * quads), g = single[m];
+            if (a.dtype == SPMM_DTYPE_BF16) single_products<SPMM_DTYPE_BF16>(a, g, q);
+            else single_products<SPMM_DTYPE_F16>(a, g, q);
+        }
     } else {
         // ---------------- epilogue: two warps a lane quarter, alternate 32-column pieces
         const int q = warp & 3, half = (warp - 2) >> 2;  // warps q and q + 4 may access TMEM lanes 32 q ..
@@ -488,7 +557,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
-template <int FORM, int TN>
+template <int FORM, int TN, bool SINGLES = false>
 int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap& mb, const TcArgs& a, long long tiles, cudaStream_t s,
               DeviceState* st) {
     using L = TcLayout<TN>;
@@ -496,13 +565,13 @@ int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap
     static std::atomic<unsigned long long> attr_set{0};
     const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
     if (!bit || !(attr_set.load(std::memory_order_acquire) & bit)) {
-        SPMM_CUDA_TRY(cudaFuncSetAttribute(grouped_tc_kernel<FORM, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        SPMM_CUDA_TRY(cudaFuncSetAttribute(grouped_tc_kernel<FORM, TN, SINGLES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            L::kFixed + 4 * (SPMM_MAX_GROUPS + 1)));
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     const size_t smem = L::kFixed + (FORM == kDw ? 0 : 4 * (static_cast<size_t>(a.groups) + 1));
-    const unsigned grid = static_cast<unsigned>(std::min<long long>(tiles, st->sm_count));
-    return launch_dependent(grouped_tc_kernel<FORM, TN>, dim3(grid), dim3(kTcThreads), smem, s, ma, small, mb, a);
+    const unsigned grid = static_cast<unsigned>(SINGLES ? st->sm_count : std::min<long long>(tiles, st->sm_count));
+    return launch_dependent(grouped_tc_kernel<FORM, TN, SINGLES>, dim3(grid), dim3(kTcThreads + (SINGLES ? kSingleThreads : 0)), smem, s, ma, small, mb, a);
 }
 
 bool fits16(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
@@ -592,6 +661,10 @@ int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st) 
     t.split_stride = static_cast<long long>(p.rows) * p.rank;
     t.which = p.which;
     t.matrices = p.matrices;
+    t.x = static_cast<const uint16_t*>(p.x);
+    t.b = static_cast<const uint16_t*>(p.a);
+    t.ldx = p.ldx;
+    t.singles = p.singles;
     t.err = st->err;
     const int tn = p.rank <= 64 ? 64 : (p.rank <= 128 ? 128 : 256);
     const int64_t tiles = (p.rows / kTileM + std::min<int64_t>(p.groups, p.rows)) * p.splits;
@@ -602,9 +675,9 @@ int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st) 
     SPMM_TRY(encode_2d(&small, p.x, K, rows, p.ldx * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
     SPMM_TRY(encode_3d(&mb, p.a, {K, rank, static_cast<uint64_t>(p.matrices)}, {K * 2, rank * K * 2}, {64, static_cast<uint32_t>(tn), 1},
                        CU_TENSOR_MAP_SWIZZLE_128B));
-    if (tn == 256) return tc_launch<kForward, 256>(ma, small, mb, t, tiles, s, st);
-    if (tn == 128) return tc_launch<kForward, 128>(ma, small, mb, t, tiles, s, st);
-    return tc_launch<kForward, 64>(ma, small, mb, t, tiles, s, st);
+    if (tn == 256) return tc_launch<kForward, 256, true>(ma, small, mb, t, tiles, s, st);
+    if (tn == 128) return tc_launch<kForward, 128, true>(ma, small, mb, t, tiles, s, st);
+    return tc_launch<kForward, 64, true>(ma, small, mb, t, tiles, s, st);
 }
 
 }  // namespace spmm_b200

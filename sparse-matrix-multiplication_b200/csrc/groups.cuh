@@ -26,14 +26,11 @@ __device__ __forceinline__ int group_matrix(const int* __restrict__ which, int g
     return i < 0 || i >= matrices ? -1 : i;
 }
 
-// start[g] = number of row tiles (tile rows each) of the groups before g, start[groups] = all of them. Groups that
-// `which` gives no matrix have none. Called by every thread of the block; ends with a barrier.
-__device__ __forceinline__ void build_tile_table(int* start, const int* __restrict__ offsets, int groups, int rows, int tile,
-                                                 DeviceErrorRecord* err, const int* __restrict__ which = nullptr, int matrices = 0) {
-    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-        const GroupRange r = group_range(offsets, g, rows, err);
-        start[g + 1] = group_matrix(which, g, matrices, err) < 0 ? 0 : (r.end - r.begin + tile - 1) / tile;
-    }
+// start[g] = sum of count(0) .. count(g - 1), start[groups] = all of them. Called by every thread of the block; ends with
+// a barrier.
+template <class Count>
+__device__ __forceinline__ void build_table(int* start, int groups, Count count) {
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) start[g + 1] = count(g);
     if (threadIdx.x == 0) start[0] = 0;
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -53,7 +50,16 @@ __device__ __forceinline__ void build_tile_table(int* start, const int* __restri
     __syncthreads();
 }
 
-// The group of row tile m, 0 <= m < start[groups].
+// The table of row tiles (tile rows each).
+__device__ __forceinline__ void build_tile_table(int* start, const int* __restrict__ offsets, int groups, int rows, int tile,
+                                                 DeviceErrorRecord* err) {
+    build_table(start, groups, [&](int g) {
+        const GroupRange r = group_range(offsets, g, rows, err);
+        return (r.end - r.begin + tile - 1) / tile;
+    });
+}
+
+// The group of entry m, 0 <= m < start[groups].
 __device__ __forceinline__ int tile_group(const int* start, int groups, int m) {
     int lo = 0, hi = groups;  // start[lo] <= m < start[hi]
     while (hi - lo > 1) {
@@ -64,9 +70,14 @@ __device__ __forceinline__ int tile_group(const int* start, int groups, int m) {
     return lo;
 }
 
-// Partial sums of x[p] a[which[g]]^T on the tensor cores (grouped_mm.cu), for lora.cu: parts[s][p][0 .. rank) for each of
-// `splits` ranges of steps_per_split * 64 of K. Rows of groups without a matrix are not written. Operands on 16-byte
-// boundaries, rank and K multiples of 8.
+// Adapter requests of one row are multiplied on CUDA cores, also in a batch with longer ones: a tensor-core tile of one row
+// costs as much as one of 128.
+__device__ __forceinline__ bool is_single(const GroupRange& r) { return r.end - r.begin == 1; }
+
+// Partial sums of x[p] a[which[g]]^T (grouped_mm.cu), for lora.cu: parts[s][p][0 .. rank) for each of `splits` ranges of
+// steps_per_split * 64 of K, on the tensor cores; groups of one row have their whole sum in parts[0] and
+// are listed in `singles`. Rows of
+// groups without a matrix are not written. Operands on 16-byte boundaries, rank and K multiples of 8.
 struct PartialProducts {
     const int* offsets;
     const int* which;
@@ -75,6 +86,7 @@ struct PartialProducts {
     long long ldx;
     const void* a;
     float* parts;
+    int* singles;  // their number, then the groups of one row in any order
     int splits, steps_per_split;
 };
 int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st);

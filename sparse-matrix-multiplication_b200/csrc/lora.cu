@@ -118,17 +118,6 @@ __global__ void __launch_bounds__(256) lora_expand_any_kernel(LoraArgs a) {
 
 constexpr int kRanksPerBlock = 4;
 
-// Dot product of eight 16-bit pairs, added to s.
-template <int DT>
-__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
-    float x[8], y[8];
-    RowVec<DT, 16>::unpack(a, x);
-    RowVec<DT, 16>::unpack(b, y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
-    return s;
-}
-
 template <int DT>
 __global__ void __launch_bounds__(256) lora_shrink_rows_kernel(LoraArgs a, int rank_blocks) {
     __shared__ float sums[8][kRanksPerBlock];
@@ -225,17 +214,19 @@ __global__ void __launch_bounds__(256) lora_expand_rows_kernel(LoraArgs a, int c
 // little: a persistent block holds u of a 128-row tile in shared memory and streams b and base past it.
 //   warp 0        TMA: b (TN features x rank) and the base tile (128 x TN) into a ring of stages, with what they are
 //   warp 1        MMA: D = u b^T in TMEM, two accumulators
-//   warps 2..17   D * scale + base (from the stage) -> 32-byte stores; a warp has 32 rows x 32 columns, which is mostly
-//                 latency: with 8 warps and twice the columns a tile took 2600 cycles, more than its bytes need (2800
-//                 at 1.9 GHz less the start of every unit)
-//   warps 18..21  the next tile's u: the parts' sum as two 16-bit terms, hi + lo, K-major under the 128-byte swizzle
+//   warps 2..17   D * scale + base (from the stage) -> 32-byte stores, two sets of eight on alternate stages
+//   warps 18..21  the next row tile's u: the parts' sum as two 16-bit terms, hi + lo, K-major under the 128-byte swizzle
+// Requests of one row come behind the tiles through the same ring: a stage is then as many of b's column tiles as it
+// holds, and the epilogue warps take the dot products with u from it on CUDA cores (lanes loading b themselves took 17 us
+// where the 100 single rows of a mixed batch now take 4).
 // The MMA needs 16-bit u; one term would cost half a step of 16 bits in every product (2^-8 in bf16), two leave 2^-16
 // for twice the MMAs, which still run under the copies.
 
 constexpr int kTileM = 128;
-constexpr int kEpilogueWarps = 16;
+constexpr int kSetWarps = 8;
+constexpr int kEpilogueWarps = 2 * kSetWarps;
 constexpr int kExpandThreads = (2 + kEpilogueWarps + 4) * 32;
-constexpr int kSmallRows = 8;  // requests with no more rows load a base box of this many
+constexpr int kSmallRows = 32;  // tiles with no more rows load a base box of this many
 
 template <int RB>  // rank in blocks of 64
 struct ExpandLayout {
@@ -245,10 +236,13 @@ struct ExpandLayout {
     static constexpr int kB = RB * kTn * 128;
     static constexpr int kBase = kTn / 64 * 16384;            // 64-column blocks of 128 rows
     static constexpr int kStage = kB + kBase;
+    // A single row's stage: column tiles of b, then the row's base, then (1 KB on) u in FP32.
+    static constexpr int kSingle = RB == 1 ? 2 : 1;
+    static constexpr int kSingleBase = kSingle * kB;
     static constexpr int kStages = RB == 1 ? 3 : (RB == 2 ? 2 : 1);
     static constexpr int kStage0 = kUs * kU;
-    static constexpr int kBars = kStage0 + kStages * kStage;  // full[], empty[], u_full[2], u_empty[2], acc_full[2], acc_empty[2], drain
-    static constexpr int kInfo = kBars + 8 * (2 * kStages + 9);  // StageInfo[kStages]
+    static constexpr int kBars = kStage0 + kStages * kStage;  // full[], empty[], u_full[2], u_empty[2], acc_full[2], acc_empty[2], drain, u_first
+    static constexpr int kInfo = kBars + 8 * (2 * kStages + 10);  // StageInfo[kStages]
     static constexpr int kSlot = kInfo + 32 * kStages;
     static constexpr int kTable = kSlot + 8;
     static constexpr int kFixed = kTable + 1024;
@@ -256,10 +250,13 @@ struct ExpandLayout {
 
 struct ExpandArgs {
     LoraArgs l;
+    const int* singles;  // the requests of one row, from the shrink
     int splits;
-    int ntiles, per_unit, chunks;  // column tiles, of which a unit takes per_unit, units along a row
+    int ntiles;        // column tiles
 };
 
+// A run of column tiles of one row tile. A block takes an equal, contiguous range of all (row tile, column tile) pairs,
+// row tiles outermost: at most one column tile more than any other, and u made once for each row tile that it meets.
 struct Unit {
     int i;             // adapter, -1 none
     int row, rows;     // first row, rows of the tile
@@ -272,21 +269,104 @@ struct StageInfo {
     int rows;          // 0: no more stages
     int row, i, nt;
     float scale;
-    int first, last;   // tile of its unit
-    int pad;
+    int16_t first, last;  // tile of its unit
+    int tile;          // 1: a tile for the tensor cores
+    int singles;       // column tiles from nt on of a request of one row, else 0
 };
 
-__device__ __forceinline__ Unit unit_of(const ExpandArgs& e, const int* start, int u) {
-    const int m = u / e.chunks, c = u - m * e.chunks;
+// The unit that begins at pair t of the block's range, which ends before pair `end`.
+__device__ __forceinline__ Unit unit_of(const ExpandArgs& e, const int* start, int t, int end) {
+    const int m = t / e.ntiles;
     const int r = tile_group(start, e.l.requests, m);
     const GroupRange g = group_range(e.l.offsets, r, e.l.rows, nullptr);
     Unit x;
     x.row = g.begin + (m - start[r]) * kTileM;
     x.rows = min(kTileM, g.end - x.row);
     x.i = adapter_of(e.l, r, nullptr);
-    x.nt0 = c * e.per_unit;
-    x.nt1 = min(e.ntiles, x.nt0 + e.per_unit);
+    x.nt0 = t - m * e.ntiles;
+    x.nt1 = min(e.ntiles, end - m * e.ntiles);
     return x;
+}
+
+// u of one unit into shared memory, by `warps` warps of which this is the `w`-th: the parts' sum, hi and lo. Pieces of 8
+// ranks to consecutive threads; the parts' loads of a piece are in flight together.
+template <int DT, int RB>
+__device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8_t* hi, int w, int warps) {
+    const LoraArgs& a = e.l;
+    const int pieces = (a.rank + 15) / 16 * 2;  // the last may lie past the rank and is zero
+    const float* parts = a.u + static_cast<long long>(x.row) * a.rank;
+    const long long stride = static_cast<long long>(a.rows) * a.rank;
+    for (int k = w * 32 + (threadIdx.x & 31); k < x.rows * pieces; k += warps * 32) {
+        const int row = k / pieces, piece = k - row * pieces;
+        float f[8] = {};
+        if (8 * piece < a.rank) {
+            const float* src = parts + static_cast<long long>(row) * a.rank + 8 * piece;
+#pragma unroll 4
+            for (int s = 0; s < e.splits; ++s) {
+                const float4 lo = *reinterpret_cast<const float4*>(src + s * stride), hi4 = *reinterpret_cast<const float4*>(src + s * stride + 4);
+                f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
+                f[4] += hi4.x, f[5] += hi4.y, f[6] += hi4.z, f[7] += hi4.w;
+            }
+        }
+        const uint4 top = RowVec<DT, 16>::pack(f);
+        float g[8];
+        RowVec<DT, 16>::unpack(top, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = f[j] - g[j];
+        const int at = row * 128 + piece / 8 * 16384 + (((piece % 8) ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4*>(hi + at) = top;
+        *reinterpret_cast<uint4*>(hi + RB * 16384 + at) = RowVec<DT, 16>::pack(g);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+
+// One row's outputs from a stage of b's column tiles, by one of a set's warps: 8 lanes to a feature, 4 features a step.
+// Gives the stage back once it is in registers.
+template <int DT, int RB>
+__device__ __forceinline__ void single_dots(const LoraArgs& a, const StageInfo& x, uint8_t* stage, int w, uint32_t empty,
+                                            uint32_t acc_empty) {
+    using L = ExpandLayout<RB>;
+    constexpr int kSteps = L::kTn / kSetWarps / 4, kSums = L::kSingle * kSteps;  // of a column tile, of the stage
+    static_assert(kSums <= 8, "a lane of the eight keeps each sum");
+    const int lane = threadIdx.x & 31, piece = lane & 7;
+    // The lane that keeps sum k has the feature of step k % kSteps of column tile k / kSteps.
+    const int local = (piece / kSteps) * L::kTn + (w * kSteps + piece % kSteps) * 4 + lane / 8;
+    float base = 0.f, d[kSums] = {};
+    if (a.base) base = half_bits_to_float<DT>(reinterpret_cast<const uint16_t*>(stage + L::kSingleBase)[local % (L::kSingle * L::kTn)]);
+    if (x.i >= 0) {
+        const float* u = reinterpret_cast<const float*>(stage + L::kSingleBase + 1024);
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            const int q = 64 * b + 8 * piece;
+            float4 lo = {}, hi = {};
+            if (q < a.rank) lo = *reinterpret_cast<const float4*>(u + q), hi = *reinterpret_cast<const float4*>(u + q + 4);
+#pragma unroll
+            for (int k = 0; k < kSums; ++k) {  // of a tile that the stage does not have, too: those sums are not stored
+                float f[8];
+                RowVec<DT, 16>::unpack(*swizzled_piece(stage + k / kSteps * L::kB + b * L::kTn * 128, (w * kSteps + k % kSteps) * 4 + lane / 8, piece), f);
+                d[k] = fmaf(f[0], lo.x, fmaf(f[1], lo.y, fmaf(f[2], lo.z, fmaf(f[3], lo.w, d[k]))));
+                d[k] = fmaf(f[4], hi.x, fmaf(f[5], hi.y, fmaf(f[6], hi.z, fmaf(f[7], hi.w, d[k]))));
+            }
+        }
+    }
+    __syncwarp();
+    if (lane == 0) {
+        mbar_arrive_count(empty, 1);
+        mbar_arrive_count(acc_empty, 1);
+    }
+    float mine = 0.f;
+#pragma unroll
+    for (int o = 4; o > 0; o /= 2) {
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) d[k] += __shfl_xor_sync(0xffffffffu, d[k], o);
+    }
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) mine = piece == k ? d[k] : mine;
+    const int n = x.nt * L::kTn + local;
+    if (piece < kSums && piece / kSteps < x.singles && n < a.N)
+        a.out[x.row * a.ldout + n] = float_to_half_bits<DT>(x.i >= 0 ? fmaf(mine, x.scale, base) : base);
+    __syncwarp();
 }
 
 template <int DT, int RB>
@@ -301,7 +381,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);
     const uint32_t sbase = smem_addr(base);
     const uint32_t full0 = sbase + L::kBars, empty0 = full0 + 8 * kStages, u_full0 = empty0 + 8 * kStages, u_empty0 = u_full0 + 16,
-                   acc_full0 = u_empty0 + 16, acc_empty0 = acc_full0 + 16, drain = acc_empty0 + 16;
+                   acc_full0 = u_empty0 + 16, acc_empty0 = acc_full0 + 16, drain = acc_empty0 + 16, u_first = drain + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kSlot);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     StageInfo* infos = reinterpret_cast<StageInfo*>(base + L::kInfo);
@@ -312,15 +392,16 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         *abort_flag = 0;
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full0 + 8 * s, 1);
-            mbar_init(empty0 + 8 * s, kEpilogueWarps);
+            mbar_init(empty0 + 8 * s, kSetWarps);
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(u_full0 + 8 * s, 4);
             mbar_init(u_empty0 + 8 * s, 1);
             mbar_init(acc_full0 + 8 * s, 1);
-            mbar_init(acc_empty0 + 8 * s, kEpilogueWarps);
+            mbar_init(acc_empty0 + 8 * s, kSetWarps);
         }
         mbar_init(drain, 1);
+        mbar_init(u_first, kExpandThreads / 32 - 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_tensormap(&map_b);
         if (a.base) prefetch_tensormap(&map_base);
@@ -329,54 +410,96 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     // Only the warps that read the shrink's parts wait for it (every block has them, so none ends before it): the shrink
     // itself waited for everything before it, and writes nothing else.
     allow_dependent_launch();
-    build_tile_table(start, a.offsets, a.requests, a.rows, kTileM, blockIdx.x == 0 ? a.err : nullptr);
-    const int units = start[a.requests] * e.chunks;
+    build_table(start, a.requests, [&](int r) {
+        const GroupRange g = group_range(a.offsets, r, a.rows, blockIdx.x == 0 ? a.err : nullptr);
+        return is_single(g) ? 0 : (g.end - g.begin + kTileM - 1) / kTileM;
+    });
+    const long long pairs = static_cast<long long>(start[a.requests]) * e.ntiles;
+    const int begin = static_cast<int>(pairs * blockIdx.x / gridDim.x), end = static_cast<int>(pairs * (blockIdx.x + 1) / gridDim.x);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+
+    // The first unit with an adapter has its u made by every warp but the first two: nothing else can begin without it.
+    if (warp >= 2) {
+        grid_dependency_wait();
+        for (int t = begin; t < end;) {
+            const Unit x = unit_of(e, start, t, end);
+            t += x.nt1 - x.nt0;
+            if (x.i < 0) continue;
+            make_u<DT, RB>(e, x, base, warp - 2, kExpandThreads / 32 - 2);
+            if (lane == 0) mbar_arrive_count(u_first, 1);
+            break;
+        }
+    }
 
     if (warp == 0) {
         // ---------------- producer
         if (elect_one()) {
             int it = 0;
             bool ok = true;
-            for (int u = blockIdx.x;; u += gridDim.x) {
-                Unit x{};
-                StageInfo info{};
-                const bool end = u >= units;
-                if (!end) {
-                    x = unit_of(e, start, u);
-                    info.rows = x.rows;
-                    info.row = x.row;
-                    info.i = x.i;
-                    info.scale = x.i >= 0 && a.scale ? __ldg(a.scale + x.i) : 1.f;
-                }
-                const bool small = x.rows <= kSmallRows;
-                for (int nt = x.nt0; end ? nt == x.nt0 : nt < x.nt1; ++nt, ++it) {
-                    const int s = it % kStages;
-                    const uint32_t bar = full0 + 8 * s, sb = sbase + L::kStage0 + s * L::kStage, sbs = sb + L::kB;
-                    if (!mbar_wait(empty0 + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    info.nt = nt;
-                    info.first = nt == x.nt0;
-                    info.last = nt == x.nt1 - 1;
+            // The next stage, once it is free, with its description; its copies follow.
+            const auto claim = [&](const StageInfo& info) {
+                const int s = it % kStages;
+                ok = mbar_wait(empty0 + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
+                if (ok) {
                     infos[s] = info;
+                    ++it;
+                }
+                return s;
+            };
+            for (int t = begin; ok && t < end;) {
+                const Unit x = unit_of(e, start, t, end);
+                t += x.nt1 - x.nt0;
+                const bool small = x.rows <= kSmallRows;
+                const float scale = x.i >= 0 && a.scale ? __ldg(a.scale + x.i) : 1.f;
+                for (int nt = x.nt0; nt < x.nt1; ++nt) {
+                    const int s = claim({x.rows, x.row, x.i, nt, scale, nt == x.nt0, nt == x.nt1 - 1, x.i >= 0, 0});
+                    if (!ok) break;
+                    const uint32_t bar = full0 + 8 * s, sb = sbase + L::kStage0 + s * L::kStage, sbs = sb + L::kB;
                     const int n0 = nt * kTn, blocks = min(kTn / 64, (a.N - n0 + 63) / 64);
-                    if (end) {
-                        mbar_arrive_count(bar, 1);
-                        continue;
-                    }
-                    mbar_arrive_expect_tx(bar, (x.i >= 0 ? L::kB : 0) + (a.base ? blocks * (small ? kSmallRows * 128 : 16384) : 0));
+                    mbar_arrive_expect_tx(bar, static_cast<uint32_t>(x.i >= 0 ? L::kB : 0) + (a.base ? blocks * (small ? kSmallRows * 128 : 16384) : 0));
                     if (x.i >= 0)
                         for (int k = 0; k < RB; ++k) tma_load_3d(sb + k * kTn * 128, &map_b, bar, 64 * k, n0, x.i);
                     if (a.base)
                         for (int k = 0; k < blocks; ++k)
                             tma_load_2d(sbs + k * 16384, small ? &map_base_small : &map_base, bar, n0 + 64 * k, x.row);
                 }
-                if (end || !ok) break;
+            }
+            grid_dependency_wait();  // the list is the shrink's
+            const int pieces = (e.ntiles + L::kSingle - 1) / L::kSingle;
+            const long long items = static_cast<long long>(e.singles[0]) * pieces;
+            const long long last = items * (blockIdx.x + 1) / gridDim.x;
+            int m = -1;
+            StageInfo info{};
+            for (long long k = items * blockIdx.x / gridDim.x; ok && k < last; ++k) {
+                if (k / pieces != m) {
+                    m = static_cast<int>(k / pieces);
+                    const int r = e.singles[1 + m];
+                    info.rows = 1;
+                    info.row = group_range(a.offsets, r, a.rows, nullptr).begin;
+                    info.i = adapter_of(a, r, nullptr);
+                    info.scale = info.i >= 0 && a.scale ? __ldg(a.scale + info.i) : 1.f;
+                }
+                info.nt = static_cast<int>(k - static_cast<long long>(m) * pieces) * L::kSingle;
+                info.singles = min(L::kSingle, e.ntiles - info.nt);
+                const int s = claim(info);
+                if (!ok) break;
+                const uint32_t bar = full0 + 8 * s, sb = sbase + L::kStage0 + s * L::kStage;
+                const uint32_t bytes = a.base ? 2 * min(info.singles * kTn, a.N - info.nt * kTn) : 0;
+                mbar_arrive_expect_tx(bar, bytes + (info.i >= 0 ? info.singles * L::kB + 4 * a.rank : 0));
+                if (a.base) bulk_load(sb + L::kSingleBase, a.base + info.row * a.ldbase + info.nt * kTn, bytes, bar);
+                if (info.i >= 0) {
+                    bulk_load(sb + L::kSingleBase + 1024, a.u + static_cast<long long>(info.row) * a.rank, 4 * a.rank, bar);
+                    for (int j = 0; j < info.singles; ++j)
+                        for (int b = 0; b < RB; ++b)
+                            tma_load_3d(sb + j * L::kB + b * kTn * 128, &map_b, bar, 64 * b, (info.nt + j) * kTn, info.i);
+                }
+            }
+            for (int k = 0; ok && k < 2; ++k) {  // the end, for either set of epilogue warps
+                const int s = claim({});
+                if (ok) mbar_arrive_count(full0 + 8 * s, 1);
             }
             if (!ok) {
                 *abort_flag = 1;
@@ -393,15 +516,22 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         if (elect_one()) {
             const uint32_t idesc = instr_desc_f16(DT, kTn, false, false);
             const int slices = (a.rank + 15) / 16;
-            int nu = 0, n = 0;
+            int nu = 0;
             bool ok = true;
-            for (int it = 0;; ++it) {
-                const int s = it % kStages, buf = n & 1, ub = nu % kUs;
-                ok = mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag);
-                if (!ok || infos[s].rows == 0) break;
-                if (infos[s].i < 0) continue;
-                ok = mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag) &&
-                     (!infos[s].first || mbar_wait(u_full0 + 8 * ub, (nu / kUs) & 1u, abort_flag));
+            // Stage `it` goes to epilogue set it & 1 with accumulator it & 1, whether or not it is a tile: so a set sees every
+            // phase of its barriers, in order.
+            for (int it = 0, ends = 0; ends < 2; ++it) {
+                const int s = it % kStages, ub = nu % kUs, buf = it & 1;
+                ok = mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag) &&
+                     mbar_wait(acc_empty0 + 8 * buf, ((it >> 1) & 1u) ^ 1u, abort_flag);
+                if (!ok) break;
+                const StageInfo x = infos[s];
+                if (!x.tile) {
+                    ends += x.rows == 0;
+                    mbar_arrive_count(acc_full0 + 8 * buf, 1);
+                    continue;
+                }
+                ok = !x.first || (nu == 0 ? mbar_wait(u_first, 0, abort_flag) : mbar_wait(u_full0 + 8 * ub, ((nu - (ub == 0)) / kUs) & 1u, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t su = sbase + ub * L::kU, sb = sbase + L::kStage0 + s * L::kStage;
@@ -413,8 +543,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                         umma_f16(acc, da, db, idesc, t + k > 0 ? 1u : 0u);
                     }
                 umma_commit(acc_full0 + 8 * buf);
-                ++n;
-                if (infos[s].last) {
+                if (x.last) {
                     umma_commit(u_empty0 + 8 * ub);
                     ++nu;
                 }
@@ -426,128 +555,86 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         }
         __syncwarp();
     } else if (warp < 2 + kEpilogueWarps) {
-        // ---------------- epilogue: four warps a lane quarter, 32 columns each
-        const int q = warp & 3, c0 = (warp - 2) / 4 * 32;
+        // ---------------- epilogue: two sets of eight warps take alternate stages; in a set two warps a lane quarter
+        const int set = (warp - 2) / kSetWarps, w = (warp - 2) % kSetWarps, q = warp & 3, half = w / 4;
         const bool sectors = (reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldout * 2)) % 32 == 0;
-        int n = 0;
         bool ok = true;
-        for (int it = 0;; ++it) {
-            const int s = it % kStages, buf = n & 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag));
+        for (int it = set;; it += 2) {
+            const int s = it % kStages;
+            uint8_t* stage = base + L::kStage0 + s * L::kStage;
+            // The stage's own barrier too, for the copies' writes; its phase cannot pass before this set gives the stage back.
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * set, (it >> 1) & 1u, abort_flag) &&
+                                             mbar_wait(full0 + 8 * s, (it / kStages) & 1u, abort_flag));
             if (!ok) break;
+            tc_fence_after();
             const StageInfo x = infos[s];
-            if (x.rows == 0) break;
-            const int cols = min(kTn, a.N - x.nt * kTn);
-            const bool some = q * 32 < x.rows && c0 < cols, has = x.i >= 0;
-            // A block of 64 columns is 16 KB of the stage.
-            uint8_t* block = base + L::kStage0 + s * L::kStage + L::kB + c0 / 64 * 16384 + q * 4096;
-            uint4 b8[4];
-            if (a.base && some) {
+            if (x.singles) {
+                single_dots<DT, RB>(a, x, stage, w, empty0 + 8 * s, acc_empty0 + 8 * set);
+                continue;
+            }
+            const int cols = min(kTn, a.N - x.nt * kTn), row = q * 32 + lane;
+            uint16_t* out = a.out + (x.row + row) * a.ldout + x.nt * kTn;
+            if (q * 32 < x.rows) {
+                // 32 columns at a time, half of a 64-column block (16 KB of the stage).
+                for (int c0 = half * 32; c0 < cols; c0 += 64) {
+                    uint4 o[4] = {};
+                    if (a.base) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) b8[c] = *swizzled_piece(block, lane, c0 % 64 / 8 + c);
+                        for (int c = 0; c < 4; ++c) o[c] = *swizzled_piece(stage + L::kB + c0 / 64 * 16384, row, 4 * half + c);
+                    }
+                    if (x.tile) {
+                        uint32_t v[32];
+                        tmem_ld32(tmem + set * kTn + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float f[8];
+                            RowVec<DT, 16>::unpack(o[c], f);
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) f[k] = fmaf(__uint_as_float(v[8 * c + k]), x.scale, f[k]);
+                            o[c] = RowVec<DT, 16>::pack(f);
+                        }
+                    }
+                    if (row < x.rows) {
+                        uint4* at = reinterpret_cast<uint4*>(out + c0);
+                        if (sectors && c0 + 32 <= cols) {
+                            store_32(at, o[0], o[1]);
+                            store_32(at + 2, o[2], o[3]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                if (c0 + 8 * c < cols) at[c] = o[c];
+                        }
+                    }
+                    __syncwarp();
+                }
             }
-            uint32_t v[32];
-            if (has) {
-                ok = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag));
-                if (!ok) break;
-                tc_fence_after();
-                if (some) tmem_ld32(tmem + buf * kTn + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
-                tc_fence_before();
-            }
-            // The stage and the accumulator are in registers: the next tile's copies and MMAs may begin.
+            tc_fence_before();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive_count(empty0 + 8 * s, 1);
-                if (has) mbar_arrive_count(acc_empty0 + 8 * buf, 1);
+                mbar_arrive_count(acc_empty0 + 8 * set, 1);
             }
-            if (has) ++n;
-            if (some && q * 32 + lane < x.rows) {
-                uint16_t* out = a.out + (x.row + q * 32 + lane) * a.ldout + x.nt * kTn + c0;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t w[8];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        float f[8] = {};
-                        if (a.base) RowVec<DT, 16>::unpack(b8[2 * h + c], f);
-                        if (has) {
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) f[k] = fmaf(__uint_as_float(v[16 * h + 8 * c + k]), x.scale, f[k]);
-                        }
-                        const uint4 o = RowVec<DT, 16>::pack(f);
-                        w[4 * c] = o.x, w[4 * c + 1] = o.y, w[4 * c + 2] = o.z, w[4 * c + 3] = o.w;
-                    }
-                    const int col = c0 + 16 * h;
-                    if (col + 16 <= cols) store_32(out + 16 * h, w, sectors);
-                    else if (col < cols) *reinterpret_cast<uint4*>(out + 16 * h) = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-            }
-            __syncwarp();
+            if (x.rows == 0) break;
         }
         if (!ok && lane == 0) {
             *abort_flag = 1;
             record_device_error(a.err, SPMM_ERR_TIMEOUT, 23);
         }
     } else {
-        // ---------------- u: sum of the parts -> hi + lo
-        grid_dependency_wait();
-        const int pieces = (a.rank + 15) / 16 * 2;  // 8 ranks each; the last may lie past the rank and is zero
+        // ---------------- u of the units behind the first
         int nu = 0;
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-            const Unit x = unit_of(e, start, u);
+        for (int t = begin; ok && t < end;) {
+            const Unit x = unit_of(e, start, t, end);
+            t += x.nt1 - x.nt0;
             if (x.i < 0) continue;
             const int ub = nu % kUs;
-            if (!__all_sync(0xffffffffu, mbar_wait(u_empty0 + 8 * ub, ((nu / kUs) & 1u) ^ 1u, abort_flag))) {
-                ok = false;
-                break;
+            if (nu > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(u_empty0 + 8 * ub, ((nu / kUs) & 1u) ^ 1u, abort_flag));
+                if (!ok) break;
+                make_u<DT, RB>(e, x, base + ub * L::kU, warp - 2 - kEpilogueWarps, 4);
+                if (lane == 0) mbar_arrive_count(u_full0 + 8 * ub, 1);
             }
-            // Pieces of 8 ranks, taken by consecutive threads; kAhead at a time so that their loads overlap.
-            uint8_t* hi = base + ub * L::kU;
-            const float* parts = a.u + static_cast<long long>(x.row) * a.rank;
-            const long long stride = static_cast<long long>(a.rows) * a.rank;
-            constexpr int kAhead = 2;
-            for (int first = (warp - 2 - kEpilogueWarps) * 32 + lane; first < x.rows * pieces; first += kAhead * 128) {
-                float f[kAhead][8] = {};
-                int row[kAhead], piece[kAhead];
-                bool real[kAhead];
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    row[j] = (first + 128 * j) / pieces;
-                    piece[j] = first + 128 * j - row[j] * pieces;
-                    real[j] = row[j] < x.rows && 8 * piece[j] < a.rank;
-                }
-                for (int k = 0; k < e.splits; ++k) {
-                    float4 v[kAhead][2];
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j) {
-                        const float4* src = reinterpret_cast<const float4*>(parts + k * stride + static_cast<long long>(row[j]) * a.rank + 8 * piece[j]);
-                        if (real[j]) v[j][0] = src[0], v[j][1] = src[1];
-                    }
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j) {
-                        if (!real[j]) continue;
-                        f[j][0] += v[j][0].x, f[j][1] += v[j][0].y, f[j][2] += v[j][0].z, f[j][3] += v[j][0].w;
-                        f[j][4] += v[j][1].x, f[j][5] += v[j][1].y, f[j][6] += v[j][1].z, f[j][7] += v[j][1].w;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    if (row[j] >= x.rows) continue;
-                    const uint4 top = RowVec<DT, 16>::pack(f[j]);
-                    float g[8];
-                    RowVec<DT, 16>::unpack(top, g);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) g[k] = f[j][k] - g[k];
-                    const uint4 rest = RowVec<DT, 16>::pack(g);
-                    const int at = row[j] * 128 + piece[j] / 8 * 16384 + (((piece[j] % 8) ^ (row[j] & 7)) << 4);
-                    *reinterpret_cast<uint4*>(hi + at) = top;
-                    *reinterpret_cast<uint4*>(hi + RB * 16384 + at) = rest;
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive_count(u_full0 + 8 * ub, 1);
             ++nu;
         }
         if (!ok && lane == 0) {
@@ -573,8 +660,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
 }
 
 template <int DT, int RB>
-int expand_launch(const CUtensorMap& mb, const CUtensorMap& ms, const CUtensorMap& small, const ExpandArgs& e, long long units,
-                  cudaStream_t s, DeviceState* st) {
+int expand_launch(const CUtensorMap& mb, const CUtensorMap& ms, const CUtensorMap& small, const ExpandArgs& e, cudaStream_t s,
+                  DeviceState* st) {
     using L = ExpandLayout<RB>;
     static std::atomic<unsigned long long> attr_set{0};
     const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
@@ -584,8 +671,7 @@ int expand_launch(const CUtensorMap& mb, const CUtensorMap& ms, const CUtensorMa
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     const size_t smem = L::kFixed + 4 * (static_cast<size_t>(e.l.requests) + 1);
-    const unsigned grid = static_cast<unsigned>(std::min<long long>(units, st->sm_count));
-    return launch_dependent(lora_expand_tc_kernel<DT, RB>, dim3(grid), dim3(kExpandThreads), smem, s, mb, ms, small, e);
+    return launch_dependent(lora_expand_tc_kernel<DT, RB>, dim3(st->sm_count), dim3(kExpandThreads), smem, s, mb, ms, small, e);
 }
 
 template <int DT>
@@ -595,12 +681,7 @@ int expand(const ExpandArgs& e0, int64_t mtiles, cudaStream_t s, DeviceState* st
     const int rb = a.rank <= 64 ? 1 : (a.rank <= 128 ? 2 : 4);
     const int tn = rb == 4 ? 64 : 128;
     e.ntiles = (a.N + tn - 1) / tn;
-    // Column tiles of a unit: u is made once for all of them, but units of one-row requests are cheap and the others
-    // should spread evenly, so every SM gets six.
-    e.per_unit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(8, mtiles * e.ntiles / (6 * st->sm_count))));
-    e.chunks = (e.ntiles + e.per_unit - 1) / e.per_unit;
-    const int64_t units = mtiles * e.chunks;
-    if (units > INT32_MAX) return SPMM_ERR_TOO_LARGE;
+    if (mtiles * e.ntiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
     CUtensorMap mb, ms{}, small{};
     const uint64_t N = a.N, rank = a.rank, rows = a.rows;
     SPMM_TRY(encode_3d(&mb, a.b, {rank, N, static_cast<uint64_t>(a.adapters)}, {rank * 2, N * rank * 2}, {64, static_cast<uint32_t>(tn), 1},
@@ -609,9 +690,9 @@ int expand(const ExpandArgs& e0, int64_t mtiles, cudaStream_t s, DeviceState* st
         SPMM_TRY(encode_2d(&ms, a.base, N, rows, a.ldbase * 2, 64, kTileM, CU_TENSOR_MAP_SWIZZLE_128B));
         SPMM_TRY(encode_2d(&small, a.base, N, rows, a.ldbase * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
     }
-    if (rb == 1) return expand_launch<DT, 1>(mb, ms, small, e, units, s, st);
-    if (rb == 2) return expand_launch<DT, 2>(mb, ms, small, e, units, s, st);
-    return expand_launch<DT, 4>(mb, ms, small, e, units, s, st);
+    if (rb == 1) return expand_launch<DT, 1>(mb, ms, small, e, s, st);
+    if (rb == 2) return expand_launch<DT, 2>(mb, ms, small, e, s, st);
+    return expand_launch<DT, 4>(mb, ms, small, e, s, st);
 }
 
 // ------------------------------------------------------------------ host
@@ -627,9 +708,9 @@ Shape shape_of(int32_t requests, int32_t rows, int32_t K) {
     Shape h{};
     h.rows = rows <= 4 * static_cast<int64_t>(requests);
     h.mtiles = rows / kTileM + std::min(requests, rows);
-    // Ranges of the sum over K until about six tiles an SM (of 148) are there, each at least 8 steps of 64 long.
+    // Ranges of the sum over K until about eight tiles an SM (of 148) are there, each at least 8 steps of 64 long.
     const int steps = (K + 63) / 64;
-    const int64_t want = h.rows ? 1 : std::max<int64_t>(1, std::min<int64_t>({8, 888 / std::max<int64_t>(1, h.mtiles), steps / 8}));
+    const int64_t want = h.rows ? 1 : std::max<int64_t>(1, std::min<int64_t>({8, 1184 / std::max<int64_t>(1, h.mtiles), steps / 8}));
     h.steps_per_split = static_cast<int>((steps + want - 1) / want);
     h.splits = h.steps_per_split ? (steps + h.steps_per_split - 1) / h.steps_per_split : 1;
     return h;
@@ -660,7 +741,8 @@ extern "C" {
 int spmm_lora_workspace_size(const spmm_lora_view* l, int32_t requests, int32_t rows, size_t* bytes) {
     SPMM_TRY(check_view(l, requests, rows));
     if (!bytes) return SPMM_ERR_INVALID_ARG;
-    *bytes = sizeof(float) * static_cast<size_t>(rows) * l->rank * shape_of(requests, rows, l->K).splits;
+    const Shape h = shape_of(requests, rows, l->K);
+    *bytes = sizeof(float) * static_cast<size_t>(rows) * l->rank * h.splits + (h.rows ? 0 : sizeof(int) * (1 + static_cast<size_t>(requests)));
     return SPMM_OK;
 }
 
@@ -725,10 +807,12 @@ int spmm_lora(const spmm_lora_view* l, const int32_t* offsets, const int32_t* ad
                                 dim3(static_cast<unsigned>(rows) * col_blocks), dim3(256), 0, s, a, col_blocks);
     }
     if (fits) {
-        PartialProducts p{offsets, adapter, requests, rows, l->adapters, l->rank, l->K, l->dtype, x, ldx, l->a, a.u, h.splits, h.steps_per_split};
+        PartialProducts p{offsets, adapter, requests, rows, l->adapters, l->rank, l->K, l->dtype, x, ldx, l->a, a.u, nullptr, h.splits, h.steps_per_split};
+        p.singles = reinterpret_cast<int*>(a.u + static_cast<size_t>(rows) * l->rank * h.splits);
         SPMM_TRY(partial_products(p, s, st));
         ExpandArgs e{};
         e.l = a;
+        e.singles = p.singles;
         e.splits = h.splits;
         return bf16 ? expand<SPMM_DTYPE_BF16>(e, h.mtiles, s, st) : expand<SPMM_DTYPE_F16>(e, h.mtiles, s, st);
     }

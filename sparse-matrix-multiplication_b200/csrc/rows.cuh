@@ -96,6 +96,17 @@ struct RowVec {
     }
 };
 
+// Dot product of eight 16-bit pairs, added to s.
+template <int DT>
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& b, float s) {
+    float x[8], y[8];
+    RowVec<DT, 16>::unpack(a, x);
+    RowVec<DT, 16>::unpack(b, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
+    return s;
+}
+
 // Launch as a programmatic dependent of the previous kernel in the stream: the kernel calls
 // grid_dependency_wait() before it touches global memory.
 template <typename... P, typename... A>
