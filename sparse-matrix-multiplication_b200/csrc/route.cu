@@ -9,10 +9,12 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstdint>
 
 #include "rows.cuh"
+#include "tcgen05.cuh"
 
 namespace spmm_b200 {
 namespace {
@@ -25,9 +27,10 @@ constexpr unsigned kFull = 0xffffffffu;
 // launch; with more, a first launch leaves each block's histogram in the workspace and every block of the second
 // adds up what it needs (blocks x groups ints from L2), so there is no wait between blocks.
 
-constexpr int kSortThreads = 1024;
-constexpr int kPairsPerBlock = 4096;
-constexpr int kMaxSortBlocks = 128;  // blocks grow beyond kPairsPerBlock instead
+constexpr int kMaxSortThreads = 1024;
+constexpr int kOneBlock = 4096;       // pairs that one block takes alone: a second launch costs more than they do
+constexpr int kPairsPerBlock = 2048;
+constexpr int kMaxSortBlocks = 128;   // blocks grow beyond kPairsPerBlock instead
 
 struct SortShape {
     int warps;      // warps with a histogram of their own
@@ -38,10 +41,12 @@ struct SortShape {
 
 SortShape sort_shape(int pairs, int groups) {
     SortShape s{};
-    // Per-warp histograms (ints) within 128 KiB, totals and block prefixes behind them.
-    s.warps = groups <= 1024 ? 32 : (groups <= 2048 ? 16 : 8);
+    // 128 pairs a warp (four steps) in blocks of the usual size; per-warp histograms (ints) within 128 KiB, totals and block
+    // prefixes behind them.
+    const int usual = pairs <= kOneBlock ? kOneBlock : kPairsPerBlock;
+    s.warps = std::min(groups <= 1024 ? 32 : (groups <= 2048 ? 16 : 8), std::max(4, (std::min(pairs, usual) + 127) / 128));
     const int unit = 32 * s.warps;
-    const long long want = std::max<long long>(kPairsPerBlock, (static_cast<long long>(pairs) + kMaxSortBlocks - 1) / kMaxSortBlocks);
+    const long long want = std::max<long long>(std::max(1, std::min(pairs, usual)), (static_cast<long long>(pairs) + kMaxSortBlocks - 1) / kMaxSortBlocks);
     s.per_block = static_cast<int>((want + unit - 1) / unit * unit);
     s.blocks = std::max(1, static_cast<int>((static_cast<long long>(pairs) + s.per_block - 1) / s.per_block));
     s.smem = sizeof(int) * (static_cast<size_t>(s.warps) * groups + 2 * static_cast<size_t>(groups) + 1 + 32);
@@ -55,7 +60,7 @@ __device__ __forceinline__ int group_of(const int* __restrict__ ids, int i, int 
     return id < 0 || id >= groups ? -1 : id;
 }
 
-__global__ void __launch_bounds__(kSortThreads) route_count_kernel(const int* __restrict__ ids, int pairs, int groups,
+__global__ void __launch_bounds__(kMaxSortThreads) route_count_kernel(const int* __restrict__ ids, int pairs, int groups,
                                                                    int per_block, int* __restrict__ counts,
                                                                    DeviceErrorRecord* err) {
     extern __shared__ int sm[];
@@ -72,7 +77,7 @@ __global__ void __launch_bounds__(kSortThreads) route_count_kernel(const int* __
     for (int g = threadIdx.x; g < groups; g += blockDim.x) counts[static_cast<size_t>(blockIdx.x) * groups + g] = sm[g];
 }
 
-__global__ void __launch_bounds__(kSortThreads)
+__global__ void __launch_bounds__(kMaxSortThreads)
     route_place_kernel(const int* __restrict__ ids, int pairs, int groups, int warps, int per_block,
                        const int* __restrict__ counts, int* __restrict__ offsets, int* __restrict__ order,
                        int* __restrict__ pos, DeviceErrorRecord* err) {
@@ -95,6 +100,7 @@ __global__ void __launch_bounds__(kSortThreads)
                                            static_cast<long long>(blockIdx.x) * per_block + static_cast<long long>(warp) * per_warp));
     const int end = warp < warps ? begin + min(per_warp, pairs - begin) : begin;
     int* mine = hist + warp * groups;
+#pragma unroll 4
     for (int i = begin + lane; i < end; i += 32) {
         const int g = group_of(ids, i, groups, alone ? err : nullptr);
         if (g >= 0) atomicAdd(mine + g, 1);
@@ -104,7 +110,7 @@ __global__ void __launch_bounds__(kSortThreads)
         for (int u = threadIdx.x; u < parts * groups; u += blockDim.x) {
             const int g = u % groups;
             int all = 0, prev = 0;
-#pragma unroll 8
+#pragma unroll 16
             for (int b = u / groups; b < static_cast<int>(gridDim.x); b += parts) {
                 const int c = __ldg(counts + static_cast<size_t>(b) * groups + g);
                 all += c;
@@ -166,9 +172,10 @@ __global__ void __launch_bounds__(kSortThreads)
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) offsets[groups] = rows;
     __syncthreads();
+    int ahead = begin + lane < end ? group_of(ids, begin + lane, groups, nullptr) : -1;
     for (int base = begin; base < end; base += 32) {
-        const int i = base + lane;
-        const int g = i < end ? group_of(ids, i, groups, nullptr) : -1;
+        const int i = base + lane, g = ahead;
+        ahead = base + 32 < end && i + 32 < end ? group_of(ids, i + 32, groups, nullptr) : -1;
         const unsigned peers = __match_any_sync(kFull, g);
         const int first = g >= 0 ? mine[g] : 0;
         __syncwarp();
@@ -239,9 +246,9 @@ __global__ void __launch_bounds__(128) route_gather_kernel(RouteArgs a, const ch
     }
 }
 
-// y[t] = sum_j w[t, j] ys[pos[t, j]]: a thread sums one vector over the pairs, J loads in flight. FP32 FMA in the
+// y[t] = sum_j w[t, j] ys[pos[t, j]]: a thread sums U vectors over the pairs, J x U = 8 loads in flight. FP32 FMA in the
 // order of j, as spmm_csr_f32 sums a row's nonzeros; one rounding at the end.
-template <int DT, int VB, int J>
+template <int DT, int VB, int J, int U>
 __global__ void __launch_bounds__(128) route_combine_kernel(RouteArgs a, const char* __restrict__ ys, long long ldys,
                                                             const float* __restrict__ w, char* __restrict__ y, long long ldy) {
     using R = RowVec<DT, VB>;
@@ -250,13 +257,11 @@ __global__ void __launch_bounds__(128) route_combine_kernel(RouteArgs a, const c
     allow_dependent_launch();
     const int chunk = blockIdx.x % a.chunks;
     const long long t = static_cast<long long>(blockIdx.x / a.chunks) * blockDim.y + threadIdx.y;
-    const int c = chunk * blockDim.x + threadIdx.x;
-    if (t >= a.tokens || c >= a.nvec) return;
-    float acc[R::N];
-#pragma unroll
-    for (int i = 0; i < R::N; ++i) acc[i] = 0.f;
+    const int c0 = chunk * blockDim.x * U + threadIdx.x;
+    if (t >= a.tokens || c0 >= a.nvec) return;
+    float acc[U][R::N] = {};
     for (int j0 = 0; j0 < a.topk; j0 += J) {
-        V v[J];
+        V v[J][U];
         float wj[J];
         int p[J];
 #pragma unroll
@@ -268,18 +273,28 @@ __global__ void __launch_bounds__(128) route_combine_kernel(RouteArgs a, const c
             wj[j] = w ? __ldg(w + pair) : 1.f;
         }
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (p[j] >= 0) v[j] = __ldg(reinterpret_cast<const V*>(ys + p[j] * ldys) + c);
+        for (int j = 0; j < J; ++j) {
+            if (p[j] < 0) continue;
+            const V* row = reinterpret_cast<const V*>(ys + p[j] * ldys);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (U == 1 || c0 + u * static_cast<int>(blockDim.x) < a.nvec) v[j][u] = __ldg(row + c0 + u * blockDim.x);
+        }
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             if (p[j] < 0) continue;
-            float f[R::N];
-            R::unpack(v[j], f);
 #pragma unroll
-            for (int i = 0; i < R::N; ++i) acc[i] = fmaf(wj[j], f[i], acc[i]);
+            for (int u = 0; u < U; ++u) {
+                float f[R::N];
+                R::unpack(v[j][u], f);
+#pragma unroll
+                for (int i = 0; i < R::N; ++i) acc[u][i] = fmaf(wj[j], f[i], acc[u][i]);
+            }
         }
     }
-    reinterpret_cast<V*>(y + t * ldy)[c] = R::pack(acc);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (U == 1 || c0 + u * static_cast<int>(blockDim.x) < a.nvec) reinterpret_cast<V*>(y + t * ldy)[c0 + u * blockDim.x] = R::pack(acc[u]);
 }
 
 // dys[pos[t, j]] = w[t, j] dy[t], dw[t, j] = <dy[t], ys[pos[t, j]]>: one block row (blockDim.x threads) takes a whole
@@ -366,6 +381,189 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// ------------------------------------------------------------------ combine_grad, streamed
+//
+// For batches that fill the GPU for a while. A persistent block keeps a ring of row pieces in shared memory that bulk
+// copies fill: 190 KB of reads are under way on every SM whatever the warps do, where the kernel above loads a token's rows,
+// sums and writes before it looks up the next token's. Lane j of the producer warp issues pair j's copies, its position read
+// a token ahead; the consumer warps share every stage (a warp that took only some of them could not tell one phase of a
+// stage's barrier from the one two later). 16384 tokens x 8
+// rows of 4 KB: 279 us by the kernel above (4.1 TB/s), 206 us streamed; the other two operators gain nothing by it
+// (gather 198 -> 215 us, combine 212 -> 207 us at 8 KB rows).
+
+constexpr int kRing = 196608;          // bytes of the ring
+constexpr int kConsumers = 8;          // warps that take pieces out of it
+constexpr int kMaxPairs = 8;           // pairs of a token that a stage holds
+constexpr int kPiece = kConsumers * 512;  // bytes of a row that a stage holds at most: 16 to a thread
+constexpr int kMaxStages = 32;
+
+struct StreamArgs {
+    RouteArgs r;
+    const char* __restrict__ dy;
+    long long lddy;
+    const char* __restrict__ ys;
+    long long ldys;
+    const float* __restrict__ w;
+    char* dys;
+    long long lddys;
+    float* dw;
+    int row_bytes, piece, pieces;      // a row, a stage's piece of it, pieces of a row
+    int stage_bytes, stages;
+};
+
+// Weights and positions of a stage's pairs, from the producer.
+struct PairInfo {
+    float w[kMaxPairs];
+    int p[kMaxPairs];
+};
+
+struct RingState {
+    unsigned long long full[kMaxStages], empty[kMaxStages];
+    PairInfo pairs[kMaxStages];
+    float sums[2][kConsumers][kMaxPairs];  // of alternate tokens
+    int abort_flag;
+};
+constexpr int kRingSmem = kRing + static_cast<int>(sizeof(RingState)) + 128;
+
+template <int DT, int J>  // J pairs at most
+__global__ void __launch_bounds__(kConsumers * 32 + 32, 1) route_combine_grad_stream_kernel(StreamArgs a) {
+    using R = RowVec<DT, 16>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* ring = raw + ((128 - (smem_addr(raw) & 127)) & 127);
+    RingState* b = reinterpret_cast<RingState*>(ring + kRing);
+    volatile int* abort_flag = &b->abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < a.stages; ++s) {
+            mbar_init(smem_addr(&b->full[s]), 1);
+            mbar_init(smem_addr(&b->empty[s]), kConsumers);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    grid_dependency_wait();
+    allow_dependent_launch();
+
+    if (warp == kConsumers) {
+        // ---------------- producer
+        int it = 0, next = -1;
+        float next_w = 1.f;
+        bool ok = true;
+        const auto fetch = [&](long long t) {  // lane j's position and weight
+            next = -1;
+            if (t >= a.r.tokens || lane >= a.r.topk) return;
+            const long long pair = t * a.r.topk + lane;
+            next = __ldg(a.r.pos + pair);
+            next_w = a.w ? __ldg(a.w + pair) : 1.f;
+        };
+        fetch(blockIdx.x);
+        for (long long t = blockIdx.x; ok && t < a.r.tokens; t += gridDim.x) {
+            int p = next;
+            const float w = next_w;
+            fetch(t + gridDim.x);
+            if (p < -1 || p >= a.r.rows) {
+                record_device_error(a.r.err, SPMM_ERR_BAD_INDEX, t * a.r.topk + lane);
+                p = -1;
+            }
+            const int rows = 1 + (a.dw ? __popc(__ballot_sync(kFull, p >= 0)) : 0);  // dy's, and the pairs'
+            for (int c = 0; c < a.pieces; ++c, ++it) {
+                const int s = it % a.stages, at = c * a.piece, bytes = min(a.piece, a.row_bytes - at);
+                const uint32_t full = smem_addr(&b->full[s]), dst = smem_addr(ring + s * a.stage_bytes);
+                if (lane == 0) ok = mbar_wait(smem_addr(&b->empty[s]), ((it / a.stages) & 1u) ^ 1u, abort_flag);
+                ok = __shfl_sync(kFull, ok ? 1 : 0, 0) != 0;
+                if (!ok) break;
+                if (lane < kMaxPairs) {
+                    b->pairs[s].p[lane] = p;
+                    b->pairs[s].w[lane] = w;
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(full, bytes * rows);
+                    bulk_load(dst, a.dy + t * a.lddy + at, bytes, full);
+                }
+                __syncwarp();
+                if (a.dw && p >= 0) bulk_load(dst + (lane + 1) * a.piece, a.ys + p * a.ldys + at, bytes, full);
+            }
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_device_error(a.r.err, SPMM_ERR_TIMEOUT, 31);
+        }
+        // Every copy lands before the block ends.
+        if (lane == 0)
+            for (int i = max(0, it - a.stages); i < it; ++i) {
+                const unsigned long long t0 = global_ns();
+                while (!mbar_try_wait(smem_addr(&b->full[i % a.stages]), (i / a.stages) & 1u) && global_ns() - t0 < kWaitNs) {
+                }
+            }
+        return;
+    }
+    // ---------------- consumers
+    int it = 0, buf = 0;
+    bool ok = true;
+    for (long long t = blockIdx.x; t < a.r.tokens; t += gridDim.x, buf ^= 1) {
+        float dot[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) dot[j] = 0.f;
+        for (int c = 0; c < a.pieces; ++c, ++it) {
+            const int s = it % a.stages, v = threadIdx.x * 16;
+            // A timeout ends the waits and the work, not the warps' barriers below.
+            ok = __all_sync(kFull, ok && mbar_wait(smem_addr(&b->full[s]), (it / a.stages) & 1u, abort_flag));
+            if (!ok) continue;
+            const uint8_t* stage = ring + s * a.stage_bytes;
+            const PairInfo& info = b->pairs[s];
+            if (v < min(a.piece, a.row_bytes - c * a.piece)) {
+                float g[R::N];
+                R::unpack(*reinterpret_cast<const uint4*>(stage + v), g);
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    if (j >= a.r.topk) continue;
+                    const int p = info.p[j];
+                    if (p < 0) continue;
+                    if (a.dys) {
+                        const float w = info.w[j];
+                        float o[R::N];
+#pragma unroll
+                        for (int i = 0; i < R::N; ++i) o[i] = w * g[i];
+                        *reinterpret_cast<uint4*>(a.dys + p * a.lddys + c * a.piece + v) = R::pack(o);
+                    }
+                    if (a.dw) {
+                        float f[R::N];
+                        R::unpack(*reinterpret_cast<const uint4*>(stage + (j + 1) * a.piece + v), f);
+#pragma unroll
+                        for (int i = 0; i < R::N; ++i) dot[j] = fmaf(g[i], f[i], dot[j]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_count(smem_addr(&b->empty[s]), 1);
+        }
+        if (!a.dw) continue;
+        // One tree of a fixed shape over the threads.
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) dot[j] += __shfl_xor_sync(kFull, dot[j], d);
+        }
+        if (lane == 0) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) b->sums[buf][warp][j] = dot[j];
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+        if (ok && static_cast<int>(threadIdx.x) < a.r.topk) {
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < kConsumers; ++k) sum += b->sums[buf][k][threadIdx.x];
+            a.dw[t * a.r.topk + threadIdx.x] = sum;
+        }
+    }
+    if (!ok && lane == 0) {
+        *abort_flag = 1;
+        record_device_error(a.r.err, SPMM_ERR_TIMEOUT, 32);
+    }
+}
+
 int route_args(const spmm_route_view* r, int32_t H, int32_t dtype) {
     if (!r || r->tokens < 0 || r->topk < 1 || r->rows < 0 || H < 0) return SPMM_ERR_INVALID_ARG;
     if (dtype != SPMM_DTYPE_F16 && dtype != SPMM_DTYPE_BF16 && dtype != SPMM_DTYPE_F32) return SPMM_ERR_INVALID_ARG;
@@ -411,14 +609,23 @@ int gather_launch(RouteArgs a, const void* x, int64_t ldx, void* xs, int64_t ldx
                             static_cast<long long>(ldx), static_cast<char*>(xs), static_cast<long long>(ldxs));
 }
 
-template <int DT, int VB>
-int combine_launch(RouteArgs a, const void* ys, int64_t ldys, const float* w, void* y, int64_t ldy, cudaStream_t s) {
-    const dim3 block = row_block(a.nvec, 128);
-    a.chunks = (a.nvec + block.x - 1) / block.x;
+template <int DT, int VB, int J, int U>
+int combine_launch_ju(RouteArgs a, const void* ys, int64_t ldys, const float* w, void* y, int64_t ldy, cudaStream_t s) {
+    const dim3 block = row_block((a.nvec + U - 1) / U, 128);
+    a.chunks = (a.nvec + block.x * U - 1) / (block.x * U);
     unsigned grid = 0;
     SPMM_TRY(row_grid(a, block, &grid));
-    return launch_dependent(route_combine_kernel<DT, VB, 8>, dim3(grid), block, 0, s, a, static_cast<const char*>(ys),
+    return launch_dependent(route_combine_kernel<DT, VB, J, U>, dim3(grid), block, 0, s, a, static_cast<const char*>(ys),
                             static_cast<long long>(ldys), w, static_cast<char*>(y), static_cast<long long>(ldy));
+}
+
+template <int DT, int VB>
+int combine_launch(const RouteArgs& a, const void* ys, int64_t ldys, const float* w, void* y, int64_t ldy, cudaStream_t s) {
+    // Few pairs leave loads for more vectors; only where there are blocks enough without splitting a row so finely.
+    const bool many = static_cast<int64_t>(a.tokens) * a.nvec >= 512 * 1024;
+    if (many && a.topk <= 2) return combine_launch_ju<DT, VB, 2, 4>(a, ys, ldys, w, y, ldy, s);
+    if (many && a.topk <= 4) return combine_launch_ju<DT, VB, 4, 2>(a, ys, ldys, w, y, ldy, s);
+    return combine_launch_ju<DT, VB, 8, 1>(a, ys, ldys, w, y, ldy, s);
 }
 
 template <int DT, int VB>
@@ -431,6 +638,28 @@ int combine_grad_launch(RouteArgs a, const void* dy, int64_t lddy, const void* y
     return launch_dependent(route_combine_grad_kernel<DT, VB, 8>, dim3(grid), block, 0, s, a, static_cast<const char*>(dy),
                             static_cast<long long>(lddy), static_cast<const char*>(ys), static_cast<long long>(ldys), w,
                             static_cast<char*>(dys), static_cast<long long>(lddys), dw);
+}
+
+template <int DT>
+int combine_grad_stream_launch(const RouteArgs& r, const void* dy, int64_t lddy, const void* ys, int64_t ldys, const float* w, void* dys,
+                               int64_t lddys, float* dw, cudaStream_t s, DeviceState* st) {
+    void (*kernel)(StreamArgs) = r.topk <= 2 ? route_combine_grad_stream_kernel<DT, 2>
+                                 : r.topk <= 4 ? route_combine_grad_stream_kernel<DT, 4> : route_combine_grad_stream_kernel<DT, kMaxPairs>;
+    static std::atomic<unsigned long long> attr_set[3];
+    const int slot = r.topk <= 2 ? 0 : (r.topk <= 4 ? 1 : 2);
+    const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
+    if (!bit || !(attr_set[slot].load(std::memory_order_acquire) & bit)) {
+        SPMM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+        attr_set[slot].fetch_or(bit, std::memory_order_acq_rel);
+    }
+    StreamArgs a{r, static_cast<const char*>(dy), lddy, static_cast<const char*>(ys), ldys, w, static_cast<char*>(dys), lddys, dw, 0, 0, 0, 0, 0};
+    a.row_bytes = r.nvec * 16;
+    a.piece = std::min(a.row_bytes, kPiece);
+    a.pieces = (a.row_bytes + a.piece - 1) / a.piece;
+    a.stage_bytes = a.piece * (r.topk + 1);
+    a.stages = std::min(kMaxStages, kRing / a.stage_bytes);
+    const unsigned grid = static_cast<unsigned>(std::min(st->sm_count, r.tokens));
+    return launch_dependent(kernel, dim3(grid), dim3(kConsumers * 32 + 32), kRingSmem, s, a);
 }
 
 #define SPMM_ROUTE_DISPATCH(fn, ...)                                                     \
@@ -475,10 +704,12 @@ int spmm_route_build(const int32_t* ids, int32_t tokens, int32_t topk, int32_t g
     if (h.smem > 48 * 1024)
         SPMM_CUDA_TRY(cudaFuncSetAttribute(route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(h.smem)));
     int* counts = static_cast<int*>(ws);
+    // More threads than the warps with histograms only where there are groups for them.
+    const int threads = std::max(h.warps * 32, std::min(kMaxSortThreads, (groups + 31) / 32 * 32));
     if (h.blocks > 1)
-        SPMM_TRY(launch_dependent(route_count_kernel, dim3(h.blocks), dim3(kSortThreads), sizeof(int) * groups, s, ids, pairs, groups,
+        SPMM_TRY(launch_dependent(route_count_kernel, dim3(h.blocks), dim3(threads), sizeof(int) * groups, s, ids, pairs, groups,
                                   h.per_block, counts, st->err));
-    return launch_dependent(route_place_kernel, dim3(h.blocks), dim3(kSortThreads), h.smem, s, ids, pairs, groups, h.warps, h.per_block,
+    return launch_dependent(route_place_kernel, dim3(h.blocks), dim3(threads), h.smem, s, ids, pairs, groups, h.warps, h.per_block,
                             counts, offsets, order, pos, st->err);
 }
 
@@ -540,6 +771,14 @@ int spmm_route_combine_grad(const spmm_route_view* r, const void* dy, int64_t ld
     al.add(nullptr, static_cast<int64_t>(H) * e);
     const int vb = al.vector_bytes();
     const RouteArgs a = make_args(r, H, dtype, vb, st);
+    // Streamed: whole vectors, a stage's pairs, rows of a piece at least, and enough bytes that filling the ring pays.
+    // (32 MB of 4 KB rows: 19.1 us above, 16.8 us streamed, of 8 KB rows 14.6 and 16.8; 128 MB: 75 and 56, two pairs 140 and 77.)
+    constexpr int64_t kLeast = INT64_C(64) << 20;
+    if (vb == 16 && r->topk <= kMaxPairs && static_cast<int64_t>(H) * e >= 1024 && static_cast<int64_t>(r->tokens) * r->topk * H * e >= kLeast) {
+        if (dtype == SPMM_DTYPE_BF16) return combine_grad_stream_launch<SPMM_DTYPE_BF16>(a, dy, lddy * e, ys, ldys * e, w, dys, lddys * e, dw, as_stream(stream), st);
+        if (dtype == SPMM_DTYPE_F16) return combine_grad_stream_launch<SPMM_DTYPE_F16>(a, dy, lddy * e, ys, ldys * e, w, dys, lddys * e, dw, as_stream(stream), st);
+        return combine_grad_stream_launch<SPMM_DTYPE_F32>(a, dy, lddy * e, ys, ldys * e, w, dys, lddys * e, dw, as_stream(stream), st);
+    }
     SPMM_ROUTE_DISPATCH(combine_grad_launch, a, dy, lddy * e, ys, ldys * e, w, dys, lddys * e, dw, as_stream(stream))
 }
 

@@ -7,7 +7,9 @@ shared library is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
+import struct
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -186,14 +188,14 @@ def lib() -> C.CDLL:
         "spmm_rank_plan_destroy": (None, [vp]),
         "spmm_route_workspace_size": (C.c_int, [i32, i32, i32, C.POINTER(C.c_size_t)]),
         "spmm_route_build": (C.c_int, [vp, i32, i32, i32, vp, vp, vp, vp, C.c_size_t, vp]),
-        "spmm_route_gather": (C.c_int, [C.POINTER(RouteView), vp, i64, vp, i64, i32, i32, vp]),
-        "spmm_route_combine": (C.c_int, [C.POINTER(RouteView), vp, i64, vp, vp, i64, i32, i32, vp]),
-        "spmm_route_combine_grad": (C.c_int, [C.POINTER(RouteView), vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, vp]),
+        "spmm_route_gather": (C.c_int, [vp, vp, i64, vp, i64, i32, i32, vp]),
+        "spmm_route_combine": (C.c_int, [vp, vp, i64, vp, vp, i64, i32, i32, vp]),
+        "spmm_route_combine_grad": (C.c_int, [vp, vp, i64, vp, i64, vp, vp, i64, vp, i32, i32, vp]),
         "spmm_grouped_mm": (C.c_int, [vp, i32, i32, vp, i64, vp, vp, i64, i32, i32, i32, i32, vp]),
         "spmm_grouped_mm_dx": (C.c_int, [vp, i32, i32, vp, i64, vp, vp, i64, i32, i32, i32, i32, vp]),
         "spmm_grouped_mm_dw": (C.c_int, [vp, i32, i32, vp, i64, vp, i64, vp, i32, i32, i32, i32, vp]),
         "spmm_lora_workspace_size": (C.c_int, [C.POINTER(LoraView), i32, i32, C.POINTER(C.c_size_t)]),
-        "spmm_lora": (C.c_int, [C.POINTER(LoraView), vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp, C.c_size_t, vp]),
+        "spmm_lora": (C.c_int, [vp, vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp, C.c_size_t, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -741,6 +743,7 @@ def _workspace(ws, need: int, stream: int, dev: int):
     return ws, ws.data_ptr(), ws.numel() * ws.element_size()
 
 
+@functools.lru_cache(maxsize=1024)
 def route_workspace_size(tokens: int, topk: int, groups: int) -> int:
     n = C.c_size_t()
     check(lib().spmm_route_workspace_size(tokens, topk, groups, C.byref(n)), "spmm_route_workspace_size")
@@ -760,17 +763,21 @@ def route_build(ids, groups: int, offsets, order, pos, ws=None, stream=None) -> 
           "spmm_route_build")
 
 
-def _route_view(pos, rows: int, dev: int) -> RouteView:
-    tokens, topk = pos.shape
-    return RouteView(tokens, topk, rows, _flat(pos, "pos", (tokens, topk), _torch.int32, dev))
+_pack_route = struct.Struct("@iiiP").pack  # the bytes of a RouteView, in a third of its constructor's time
+_pack_lora = struct.Struct("@iiiiiPPP").pack
+
+
+def _route_view(pos, tokens: int, topk: int, rows: int, dev: int) -> bytes:
+    return _pack_route(tokens, topk, rows, _flat(pos, "pos", (tokens, topk), _torch.int32, dev))
 
 
 def route_gather(pos, x, xs, stream=None) -> None:
     """xs[pos[t, j]] = x[t] (rows of xs without a pair stay as they are)."""
     dev = _device(pos)
+    tokens, topk = pos.shape
     shape = rows, H = xs.shape
-    v = _route_view(pos, rows, dev)
-    check(lib().spmm_route_gather(v, x.data_ptr(), _rows(x, "x", (v.tokens, H), x.dtype, dev), xs.data_ptr(),
+    v = _route_view(pos, tokens, topk, rows, dev)
+    check(lib().spmm_route_gather(v, x.data_ptr(), _rows(x, "x", (tokens, H), x.dtype, dev), xs.data_ptr(),
                                   _rows(xs, "xs", shape, x.dtype, dev), H, _value_dtype(x, "x", True), stream_ptr(stream)),
           "spmm_route_gather")
 
@@ -778,11 +785,12 @@ def route_gather(pos, x, xs, stream=None) -> None:
 def route_combine(pos, ys, y, w=None, stream=None) -> None:
     """y[t] = sum_j w[t, j] ys[pos[t, j]] (w None: all 1, the gradient of route_gather)."""
     dev = _device(pos)
+    tokens, topk = pos.shape
     shape = rows, H = ys.shape
-    v = _route_view(pos, rows, dev)
+    v = _route_view(pos, tokens, topk, rows, dev)
     check(lib().spmm_route_combine(v, ys.data_ptr(), _rows(ys, "ys", shape, ys.dtype, dev),
                                    _flat(w, "w", pos.shape, _torch.float32, dev), y.data_ptr(),
-                                   _rows(y, "y", (v.tokens, H), ys.dtype, dev), H, _value_dtype(ys, "ys", True), stream_ptr(stream)),
+                                   _rows(y, "y", (tokens, H), ys.dtype, dev), H, _value_dtype(ys, "ys", True), stream_ptr(stream)),
           "spmm_route_combine")
 
 
@@ -797,10 +805,11 @@ def route_combine_grad(pos, dy, ys=None, w=None, dys=None, dw=None, stream=None)
     H = dy.shape[1]
     ys = ys if dw is not None else None
     shape = ((dys if dys is not None else ys).shape[0], H)
-    v = _route_view(pos, shape[0], dev)
+    tokens, topk = pos.shape
+    v = _route_view(pos, tokens, topk, shape[0], dev)
     f32 = _torch.float32
     check(lib().spmm_route_combine_grad(
-        v, dy.data_ptr(), _rows(dy, "dy", (v.tokens, H), dy.dtype, dev), ptr(ys),
+        v, dy.data_ptr(), _rows(dy, "dy", (tokens, H), dy.dtype, dev), ptr(ys),
         _rows(ys, "ys", shape, dy.dtype, dev) if ys is not None else 0, _flat(w, "w", pos.shape, f32, dev), ptr(dys),
         _rows(dys, "dys", shape, dy.dtype, dev) if dys is not None else 0, _flat(dw, "dw", pos.shape, f32, dev), H,
         _value_dtype(dy, "dy", True), stream_ptr(stream)), "spmm_route_combine_grad")
@@ -839,31 +848,30 @@ def grouped_mm_dw(offsets, dy, x, dw, stream=None) -> None:
                                    stream_ptr(stream)), "spmm_grouped_mm_dw")
 
 
-def _lora_view(a, b, scale, dev: int) -> LoraView:
-    adapters, rank, K = a.shape
-    N = b.shape[1]
-    return LoraView(adapters, rank, N, K, _value_dtype(a, "a"), _flat(a, "a", a.shape, a.dtype, dev),
-                    _flat(b, "b", (adapters, N, rank), a.dtype, dev), _flat(scale, "scale", (adapters,), _torch.float32, dev))
+@functools.lru_cache(maxsize=1024)
+def _lora_workspace(adapters: int, rank: int, N: int, K: int, dtype: int, requests: int, rows: int) -> int:
+    v = LoraView(adapters, rank, N, K, dtype, 0, 0, 0)
+    n = C.c_size_t()
+    check(lib().spmm_lora_workspace_size(C.byref(v), requests, rows, C.byref(n)), "spmm_lora_workspace_size")
+    return int(n.value)
 
 
 def lora_workspace_size(a, b, requests: int, rows: int) -> int:
-    v = _lora_view(a, b, None, _device(a))
-    n = C.c_size_t()
-    check(lib().spmm_lora_workspace_size(v, requests, rows, C.byref(n)), "spmm_lora_workspace_size")
-    return n.value
+    _device(a)
+    return _lora_workspace(a.shape[0], a.shape[1], b.shape[1], a.shape[2], _value_dtype(a, "a"), requests, rows)
 
 
 def lora(offsets, adapter, x, a, b, out, base=None, scale=None, ws=None, stream=None) -> None:
     """out[p] = base[p] + scale * b (a x[p]) with the matrices of adapter[r], offsets[r] <= p < offsets[r + 1] (offsets None: every
     row a request of its own); x (rows, K), a (adapters, rank, K), b (adapters, N, rank), base and out (rows, N)."""
     dev = _device(adapter)
-    v = _lora_view(a, b, scale, dev)
-    rows, requests = x.shape[0], adapter.shape[0]
-    n = C.c_size_t()
-    check(lib().spmm_lora_workspace_size(v, requests, rows, C.byref(n)), "spmm_lora_workspace_size")
-    sp, wide = stream_ptr(stream), (rows, v.N)
-    _ws, wp, wn = _workspace(ws, n.value, sp, dev)
+    shape = adapters, rank, K = a.shape
+    N, rows, requests, dt = b.shape[1], x.shape[0], adapter.shape[0], _value_dtype(a, "a")
+    v = _pack_lora(adapters, rank, N, K, dt, _flat(a, "a", shape, a.dtype, dev), _flat(b, "b", (adapters, N, rank), a.dtype, dev),
+                   _flat(scale, "scale", (adapters,), _torch.float32, dev))
+    sp, wide = stream_ptr(stream), (rows, N)
+    _ws, wp, wn = _workspace(ws, _lora_workspace(adapters, rank, N, K, dt, requests, rows), sp, dev)
     check(lib().spmm_lora(v, _flat(offsets, "offsets", (requests + 1,), _torch.int32, dev),
                           _flat(adapter, "adapter", (requests,), _torch.int32, dev), requests, rows, x.data_ptr(),
-                          _rows(x, "x", (rows, v.K), a.dtype, dev), ptr(base), _rows(base, "base", wide, a.dtype, dev) if base is not None else 0,
+                          _rows(x, "x", (rows, K), a.dtype, dev), ptr(base), _rows(base, "base", wide, a.dtype, dev) if base is not None else 0,
                           out.data_ptr(), _rows(out, "out", wide, a.dtype, dev), wp, wn, sp), "spmm_lora")
