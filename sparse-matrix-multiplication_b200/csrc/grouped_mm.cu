@@ -141,7 +141,7 @@ int any_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st)
 //
 // A persistent block takes 128 x TN tiles of D, 64 of k a step: one warp issues TMA copies into a ring of stages, one
 // issues the MMAs (M = 128, N = TN, FP32 accumulators in TMEM, two of them so that the next tile's MMAs run under this
-// one's epilogue), eight move TMEM -> registers -> memory: a lane holds a row's consecutive columns and
+// one's epilogue), sixteen move TMEM -> registers -> memory: a lane holds a row's consecutive columns and
 // stores whole 32-byte sectors.
 // x, dy and w are read as they lie: K-major where k is the contiguous index (both operands of the forward product,
 // dx's A), MN-major where it is not (dx's B, both of dw's), so nothing is transposed in memory.
@@ -152,8 +152,11 @@ int any_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st)
 constexpr int kTileM = 128;
 constexpr int kStepK = 64;
 constexpr int kBand = 8;          // row tiles that run together down a band (their A and the band's B stay in L2)
-constexpr int kTcThreads = 320;   // warp 0 TMA, warp 1 MMA, warps 2..9 epilogue
-constexpr int kSingleThreads = 256;  // 8 warps more for the groups of one row
+// Warp 0 TMA, warp 1 MMA, then the epilogue's (sixteen: half the time of eight on a tile that nothing overlaps), then, with
+// SINGLES, eight for the groups of one row.
+constexpr int epilogue_warps(bool singles) { return singles ? 8 : 8; }
+constexpr int kSingleThreads = 256;
+constexpr int tc_threads(bool singles) { return 64 + 32 * epilogue_warps(singles) + (singles ? kSingleThreads : 0); }
 constexpr int kSmallRows = 32;    // groups with no more rows left load a box of this many
 
 template <int TN>
@@ -194,16 +197,46 @@ struct TcArgs {
 
 struct Tile {
     int g, m0, n0;     // matrix, first row of D in the group, first column
+    int cols;          // columns (a multiple of 8; 0: nothing to do)
     int begin, end;    // the group's rows
     int split;         // forward: the range of the sum,
     int first;         // its first step
     int steps;         // k steps
 };
 
+// The tiles in the order that blocks take them, block b those at b, b + grid, ... The last round, if it does not give every
+// block a tile, is cut into narrower ones (TN / parts columns) while that gives no block two: a block streams a tile no
+// faster for the others' being idle.
+struct Rounds {
+    int tiles;         // all of them, full width
+    int whole;         // those of the full rounds
+    int parts;         // pieces of each of the rest
+    int units;         // whole + (tiles - whole) * parts
+};
+
+template <int TN>
+__device__ __forceinline__ Rounds rounds_of(int tiles) {
+    Rounds r;
+    const int grid = gridDim.x;
+    r.tiles = tiles;
+    r.whole = tiles / grid * grid;
+    const int rest = tiles - r.whole;
+    r.parts = 1;
+    while (r.parts < TN / 64 && rest * r.parts * 2 <= grid) r.parts *= 2;
+    r.units = r.whole + rest * r.parts;
+    return r;
+}
+
 template <int FORM, int TN>
-__device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, int t) {
+__device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, const Rounds& rounds, int t) {
     Tile r;
-    int g, local, mtiles;
+    int g, local, mtiles, width = TN, part = 0;
+    if (t >= rounds.whole && rounds.parts > 1) {
+        const int k = t - rounds.whole;
+        t = rounds.whole + k / rounds.parts;
+        part = k % rounds.parts;
+        width = TN / rounds.parts;
+    }
     r.split = 0;
     if constexpr (FORM == kForward) {
         if (a.splits > 1) {
@@ -226,7 +259,8 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, int t
     const int high = min(kBand, mtiles - band * kBand);
     local -= band * kBand * a.ntiles;
     r.m0 = (band * kBand + local % high) * kTileM;
-    r.n0 = local / high * TN;
+    r.n0 = local / high * TN + part * width;
+    r.cols = max(0, min(width, a.outs - r.n0));
     const GroupRange range = group_range(a.offsets, g, a.rows, nullptr);
     r.begin = range.begin;
     r.end = range.end;
@@ -285,11 +319,11 @@ __device__ __forceinline__ void single_products(const TcArgs& a, int g, int q) {
 
 // SINGLES (forward, FP32 out): groups of one row are left to eight warps more.
 template <int FORM, int TN, bool SINGLES>
-__global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1)
+__global__ void __launch_bounds__(tc_threads(SINGLES), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_small,
-                      const __grid_constant__ CUtensorMap map_b, TcArgs a) {
+                      const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_wide, TcArgs a) {
     using L = TcLayout<TN>;
-    constexpr int kStages = L::kStages;
+    constexpr int kStages = L::kStages, kEpilogue = epilogue_warps(SINGLES);
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // 1 KB: the 128-byte swizzle's atoms
@@ -311,7 +345,7 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(acc_full0 + 8 * s, 1);
-            mbar_init(acc_empty0 + 8 * s, 8);
+            mbar_init(acc_empty0 + 8 * s, kEpilogue);
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -324,7 +358,7 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
     int tiles;
     if constexpr (FORM == kDw) {
         if (blockIdx.x == 0)
-            for (int g = threadIdx.x; g < a.groups; g += kTcThreads) group_range(a.offsets, g, a.rows, a.err);  // records bad ones
+            for (int g = threadIdx.x; g < a.groups; g += blockDim.x) group_range(a.offsets, g, a.rows, a.err);  // records bad ones
         tiles = a.groups * a.mtiles * a.ntiles;
     } else {
         DeviceErrorRecord* err = blockIdx.x == 0 ? a.err : nullptr;
@@ -356,6 +390,7 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    const Rounds rounds = rounds_of<TN>(tiles);
 
     if (warp == 0) {
         // ---------------- producer
@@ -363,13 +398,15 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
             int it = 0, s = 0;
             uint32_t phase = 1;
             bool ok = true;
-            for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                const Tile r = tile_of<FORM, TN>(a, start, t);
+            for (int t = blockIdx.x; ok && t < rounds.units; t += gridDim.x) {
+                const Tile r = tile_of<FORM, TN>(a, start, rounds, t);
                 const bool small = FORM != kDw && r.end - r.begin - r.m0 <= kSmallRows;
                 // Boxes of 64 columns that lie wholly past the operand are not loaded; their part of D is not stored.
-                const int nb = min(TN / 64, (a.outs - r.n0 + 63) / 64);
+                if (r.cols == 0) continue;
+                const int nb = (r.cols + 63) / 64;
+                const bool wide = nb == TN / 64;  // forward: one copy of TN rows of w (four of 64 rows took 5 % longer on large products)
                 const int na = min(2, (a.ms - r.m0 + 63) / 64);  // dw
-                const uint32_t bytes = (FORM == kDw ? na * 8192 : (small ? kSmallRows * 128 : L::kA)) + (FORM == kForward ? L::kB : nb * 8192);
+                const uint32_t bytes = (FORM == kDw ? na * 8192 : (small ? kSmallRows * 128 : L::kA)) + nb * 8192;
                 for (int ks = 0; ks < r.steps; ++ks, ++it) {
                     const uint32_t bar = full0 + 8 * s, sa = sbase + s * L::kStage, sb = sa + L::kA;
                     if (!mbar_wait(empty0 + 8 * s, phase, abort_flag)) {
@@ -384,10 +421,11 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
                         for (int j = 0; j < nb; ++j) tma_load_2d(sb + j * 8192, &map_b, bar, r.n0 + 64 * j, r.begin + k0);
                     } else {
                         tma_load_2d(sa, small ? &map_a_small : &map_a, bar, k0, r.begin + r.m0);
-                        if constexpr (FORM == kForward) {
-                            tma_load_3d(sb, &map_b, bar, k0, r.n0, r.g);
+                        if (FORM == kForward && wide) {
+                            tma_load_3d(sb, &map_b_wide, bar, k0, r.n0, r.g);
                         } else {
-                            for (int j = 0; j < nb; ++j) tma_load_3d(sb + j * 8192, &map_b, bar, r.n0 + 64 * j, k0, r.g);
+                            for (int j = 0; j < nb; ++j)
+                                tma_load_3d(sb + j * 8192, &map_b, bar, FORM == kForward ? k0 : r.n0 + 64 * j, FORM == kForward ? r.n0 + 64 * j : k0, r.g);
                         }
                     }
                 }
@@ -406,13 +444,14 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer: one lane; in dw the whole warp clears the rows past a group's end
-        const uint32_t idesc = instr_desc_f16(a.dtype, TN, FORM == kDw, FORM != kForward);
         int it = 0, n = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++n) {
-            const Tile r = tile_of<FORM, TN>(a, start, t);
+        for (int t = blockIdx.x; ok && t < rounds.units; t += gridDim.x) {
+            const Tile r = tile_of<FORM, TN>(a, start, rounds, t);
+            if (r.cols == 0) continue;
             const int buf = n & 1;
             const uint32_t acc = tmem + buf * TN;
+            const uint32_t idesc = instr_desc_f16(a.dtype, (r.cols + 15) / 16 * 16, FORM == kDw, FORM != kForward);
             const int sum = FORM == kDw ? r.end - r.begin : a.sum;
             const int left = min(kStepK, sum - (r.first + r.steps - 1) * kStepK);  // of the last step
             const int clear = FORM == kDw && left % 16 != 0;
@@ -436,7 +475,7 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
                 const int s = (it - 1) % kStages, slices = (left + 15) / 16;
                 ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, ((it - 1) / kStages) & 1u, abort_flag));
                 if (ok) {
-                    const int nb = min(TN / 64, (a.outs - r.n0 + 63) / 64), na = min(2, (a.ms - r.m0 + 63) / 64);
+                    const int nb = (r.cols + 63) / 64, na = min(2, (a.ms - r.m0 + 63) / 64);
                     const int pieces = (slices * 16 - left) * 8;  // 16-byte pieces of a box's rows to clear
                     uint8_t* st = base + s * L::kStage;
                     for (int b = 0; b < na + nb; ++b) {
@@ -455,34 +494,36 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
             }
             if (elect_one()) umma_commit(acc_full0 + 8 * buf);
             __syncwarp();
+            ++n;
         }
         if (!ok && lane == 0) {
             *abort_flag = 1;
             record_device_error(a.err, SPMM_ERR_TIMEOUT, 12);
         }
-    } else if (SINGLES && warp >= kTcThreads / 32) {
+    } else if (SINGLES && warp >= 2 + kEpilogue) {
         // ---------------- groups of one row, while the tiles stream
         const int n = singles, quads = a.outs / 4, warps = kSingleThreads / 32;
         if (blockIdx.x == 0) {
-            const int first = threadIdx.x - kTcThreads;
+            const int first = threadIdx.x - 32 * (2 + kEpilogue);
             if (first == 0) a.singles[0] = n;
             for (int k = first; k < n; k += kSingleThreads) a.singles[1 + k] = single[k];
         }
         const long long items = static_cast<long long>(n) * quads;
-        for (long long k = static_cast<long long>(blockIdx.x) * warps + warp - kTcThreads / 32; k < items; k += static_cast<long long>(gridDim.x) * warps) {
+        for (long long k = static_cast<long long>(blockIdx.x) * warps + warp - 2 - kEpilogue; k < items; k += static_cast<long long>(gridDim.x) * warps) {
             const int m = static_cast<int>(k / quads), q = 4 * static_cast<int>(k - static_cast<long long>(m) * quads), g = single[m];
             if (a.dtype == SPMM_DTYPE_BF16) single_products<SPMM_DTYPE_BF16>(a, g, q);
             else single_products<SPMM_DTYPE_F16>(a, g, q);
         }
     } else {
-        // ---------------- epilogue: two warps a lane quarter, alternate 32-column pieces
-        const int q = warp & 3, half = (warp - 2) >> 2;  // warps q and q + 4 may access TMEM lanes 32 q ..
+        // ---------------- epilogue: two or four warps a lane quarter, alternate 32-column pieces
+        const int q = warp & 3, part = (warp - 2) >> 2;  // warps q and q + 4 may access TMEM lanes 32 q ..
         const int size = a.out_f32 ? 4 : 2;
         const bool sectors = (reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) % 32 == 0;
         int n = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++n) {
-            const Tile r = tile_of<FORM, TN>(a, start, t);
+        for (int t = blockIdx.x; t < rounds.units; t += gridDim.x) {
+            const Tile r = tile_of<FORM, TN>(a, start, rounds, t);
+            if (r.cols == 0) continue;
             const int buf = n & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag))) {
                 ok = false;
@@ -493,9 +534,9 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
             const int row = r.m0 + q * 32 + lane, rows = FORM == kDw ? a.ms : r.end - r.begin;
             const long long at = FORM == kDw ? static_cast<long long>(r.g) * a.ms + row : r.begin + row;
             char* out = static_cast<char*>(a.out) + (at * a.ldo + r.n0 + r.split * a.split_stride) * size;
-            const int cols = min(TN, a.outs - r.n0);  // a multiple of 8
+            const int cols = r.cols;
             if (r.m0 + q * 32 < rows) {
-                for (int c0 = half * 32; c0 < cols; c0 += 64) {
+                for (int c0 = part * 32; c0 < cols; c0 += 8 * kEpilogue) {
                     uint32_t v[32];
                     tmem_ld32(acc + c0, v);
                     if (FORM == kDw && r.steps == 0) {
@@ -532,6 +573,7 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
             __syncwarp();
             tc_fence_before();
             if (lane == 0) mbar_arrive_count(acc_empty0 + 8 * buf, 1);
+            ++n;
         }
         if (!ok && lane == 0) {
             *abort_flag = 1;
@@ -558,7 +600,7 @@ __global__ void __launch_bounds__(kTcThreads + (SINGLES ? kSingleThreads : 0), 1
 }
 
 template <int FORM, int TN, bool SINGLES = false>
-int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap& mb, const TcArgs& a, long long tiles, cudaStream_t s,
+int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap& mb, const CUtensorMap& wide, const TcArgs& a, long long tiles, cudaStream_t s,
               DeviceState* st) {
     using L = TcLayout<TN>;
     // The attribute belongs to the device's context: set once a device, for the largest table.
@@ -570,8 +612,8 @@ int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     const size_t smem = L::kFixed + (FORM == kDw ? 0 : 4 * (static_cast<size_t>(a.groups) + 1));
-    const unsigned grid = static_cast<unsigned>(SINGLES ? st->sm_count : std::min<long long>(tiles, st->sm_count));
-    return launch_dependent(grouped_tc_kernel<FORM, TN, SINGLES>, dim3(grid), dim3(kTcThreads + (SINGLES ? kSingleThreads : 0)), smem, s, ma, small, mb, a);
+    const unsigned grid = static_cast<unsigned>(SINGLES ? st->sm_count : std::min<long long>(tiles * (TN / 64), st->sm_count));
+    return launch_dependent(grouped_tc_kernel<FORM, TN, SINGLES>, dim3(grid), dim3(tc_threads(SINGLES)), smem, s, ma, small, mb, wide, a);
 }
 
 bool fits16(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
@@ -612,20 +654,24 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     const int64_t tiles = mtiles * t.ntiles;
     if (tiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
 
-    CUtensorMap ma, small, mb;
+    CUtensorMap ma, small, mb, wide{};
     const uint64_t rows = a.rows, N = a.N, K = a.K;
-    const uint64_t wide = FORM == kForward ? K : N;  // columns of A's operand
-    SPMM_TRY(encode_2d(&ma, a.a, wide, rows, a.lda * 2, 64, FORM == kDw ? 64 : kTileM, CU_TENSOR_MAP_SWIZZLE_128B));
-    SPMM_TRY(encode_2d(&small, a.a, wide, rows, a.lda * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
+    const uint64_t inner = FORM == kForward ? K : N;  // columns of A's operand
+    SPMM_TRY(encode_2d(&ma, a.a, inner, rows, a.lda * 2, 64, FORM == kDw ? 64 : kTileM, CU_TENSOR_MAP_SWIZZLE_128B));
+    SPMM_TRY(encode_2d(&small, a.a, inner, rows, a.lda * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
     if constexpr (FORM == kDw) {
         SPMM_TRY(encode_2d(&mb, a.b, K, rows, a.ldb * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B));
     } else {
-        SPMM_TRY(encode_3d(&mb, a.b, {K, N, static_cast<uint64_t>(a.groups)}, {K * 2, N * K * 2},
-                           {64, static_cast<uint32_t>(FORM == kForward ? tn : 64), 1}, CU_TENSOR_MAP_SWIZZLE_128B));
+        const auto encode_w = [&](CUtensorMap* map, int box_rows) {
+            return encode_3d(map, a.b, {K, N, static_cast<uint64_t>(a.groups)}, {K * 2, N * K * 2}, {64, static_cast<uint32_t>(box_rows), 1},
+                             CU_TENSOR_MAP_SWIZZLE_128B);
+        };
+        SPMM_TRY(encode_w(&mb, 64));
+        if (FORM == kForward) SPMM_TRY(encode_w(&wide, tn));
     }
-    if (tn == 256) return tc_launch<FORM, 256>(ma, small, mb, t, tiles, s, st);
-    if (tn == 128) return tc_launch<FORM, 128>(ma, small, mb, t, tiles, s, st);
-    return tc_launch<FORM, 64>(ma, small, mb, t, tiles, s, st);
+    if (tn == 256) return tc_launch<FORM, 256>(ma, small, mb, wide, t, tiles, s, st);
+    if (tn == 128) return tc_launch<FORM, 128>(ma, small, mb, wide, t, tiles, s, st);
+    return tc_launch<FORM, 64>(ma, small, mb, wide, t, tiles, s, st);
 }
 
 int check_common(const int32_t* offsets, int32_t groups, int32_t rows, int32_t N, int32_t K, int32_t dtype, int32_t out_dtype) {
@@ -669,15 +715,16 @@ int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st) 
     const int tn = p.rank <= 64 ? 64 : (p.rank <= 128 ? 128 : 256);
     const int64_t tiles = (p.rows / kTileM + std::min<int64_t>(p.groups, p.rows)) * p.splits;
     if (tiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
-    CUtensorMap ma, small, mb;
+    CUtensorMap ma, small, mb, wide;
     const uint64_t rows = p.rows, K = p.K, rank = p.rank;
     SPMM_TRY(encode_2d(&ma, p.x, K, rows, p.ldx * 2, 64, kTileM, CU_TENSOR_MAP_SWIZZLE_128B));
     SPMM_TRY(encode_2d(&small, p.x, K, rows, p.ldx * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
-    SPMM_TRY(encode_3d(&mb, p.a, {K, rank, static_cast<uint64_t>(p.matrices)}, {K * 2, rank * K * 2}, {64, static_cast<uint32_t>(tn), 1},
+    SPMM_TRY(encode_3d(&mb, p.a, {K, rank, static_cast<uint64_t>(p.matrices)}, {K * 2, rank * K * 2}, {64, 64, 1}, CU_TENSOR_MAP_SWIZZLE_128B));
+    SPMM_TRY(encode_3d(&wide, p.a, {K, rank, static_cast<uint64_t>(p.matrices)}, {K * 2, rank * K * 2}, {64, static_cast<uint32_t>(tn), 1},
                        CU_TENSOR_MAP_SWIZZLE_128B));
-    if (tn == 256) return tc_launch<kForward, 256, true>(ma, small, mb, t, tiles, s, st);
-    if (tn == 128) return tc_launch<kForward, 128, true>(ma, small, mb, t, tiles, s, st);
-    return tc_launch<kForward, 64, true>(ma, small, mb, t, tiles, s, st);
+    if (tn == 256) return tc_launch<kForward, 256, true>(ma, small, mb, wide, t, tiles, s, st);
+    if (tn == 128) return tc_launch<kForward, 128, true>(ma, small, mb, wide, t, tiles, s, st);
+    return tc_launch<kForward, 64, true>(ma, small, mb, wide, t, tiles, s, st);
 }
 
 }  // namespace spmm_b200

@@ -689,7 +689,7 @@ def _device(t) -> int:
         _DTYPES.update({torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16, torch.float32: DTYPE_F32})
         _torch = torch
     dev = t.get_device()
-    if dev < 0 or dev != _torch.cuda.current_device():
+    if dev < 0 or dev != _torch._C._cuda_getDevice():  # current_device() without its check that CUDA is up
         raise ValueError(f"operands must be on the current CUDA device, got {t.device}")
     return dev
 
