@@ -141,7 +141,7 @@ int any_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st)
 //
 // A persistent block takes 128 x TN tiles of D, 64 of k a step: one warp issues TMA copies into a ring of stages, one
 // issues the MMAs (M = 128, N = TN, FP32 accumulators in TMEM, two of them so that the next tile's MMAs run under this
-// one's epilogue), sixteen move TMEM -> registers -> memory: a lane holds a row's consecutive columns and
+// one's epilogue), eight move TMEM -> registers -> memory: a lane holds a row's consecutive columns and
 // stores whole 32-byte sectors.
 // x, dy and w are read as they lie: K-major where k is the contiguous index (both operands of the forward product,
 // dx's A), MN-major where it is not (dx's B, both of dw's), so nothing is transposed in memory.
@@ -152,11 +152,11 @@ int any_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st)
 constexpr int kTileM = 128;
 constexpr int kStepK = 64;
 constexpr int kBand = 8;          // row tiles that run together down a band (their A and the band's B stay in L2)
-// Warp 0 TMA, warp 1 MMA, then the epilogue's (sixteen: half the time of eight on a tile that nothing overlaps), then, with
-// SINGLES, eight for the groups of one row.
-constexpr int epilogue_warps(bool singles) { return singles ? 8 : 8; }
+// Warp 0 TMA, warp 1 MMA, then the epilogue's (sixteen were 2 to 5 % slower on large products), then, with SINGLES, eight
+// for the groups of one row.
+constexpr int kEpilogue = 8;
 constexpr int kSingleThreads = 256;
-constexpr int tc_threads(bool singles) { return 64 + 32 * epilogue_warps(singles) + (singles ? kSingleThreads : 0); }
+constexpr int tc_threads(bool singles) { return 64 + 32 * kEpilogue + (singles ? kSingleThreads : 0); }
 constexpr int kSmallRows = 32;    // groups with no more rows left load a box of this many
 
 template <int TN>
@@ -181,9 +181,9 @@ struct TcArgs {
     void* out;
     long long ldo;     // row stride of out
     int out_f32, dtype;
-    // Forward only: the sum over k cut into `splits` ranges of split_steps steps, each with a result of its own
-    // (split_stride elements apart), and the groups' matrices by index (NULL: group g has matrix g).
-    int splits, split_steps;
+    // SINGLES only: at most this many ranges of the sum over k, each with a result of its own (split_stride elements apart),
+    // and the groups' matrices by index (NULL: group g has matrix g).
+    int most_splits;
     long long split_stride;
     const int* __restrict__ which;
     int matrices;
@@ -212,7 +212,26 @@ struct Rounds {
     int whole;         // those of the full rounds
     int parts;         // pieces of each of the rest
     int units;         // whole + (tiles - whole) * parts
+    int splits;        // SINGLES: ranges of the sum, of split_steps steps; each tile comes once for each
+    int split_steps;
 };
+
+// Into how many ranges the sum of `steps` steps is cut so that the rounds of tiles take the fewest steps, two more a round for
+// its start. The same for every block, and for the reader of the parts.
+__device__ __forceinline__ void choose_splits(Rounds& r, int tiles, int steps, int most) {
+    r.splits = 1;
+    r.split_steps = steps;
+    long long best = LLONG_MAX;
+    for (int s = 1; s <= most; ++s) {
+        const int length = (steps + s - 1) / s, n = (steps + length - 1) / length;
+        const long long cost = (static_cast<long long>(tiles) * n + gridDim.x - 1) / gridDim.x * (length + 2);
+        if (cost < best) {
+            best = cost;
+            r.splits = n;
+            r.split_steps = length;
+        }
+    }
+}
 
 template <int TN>
 __device__ __forceinline__ Rounds rounds_of(int tiles) {
@@ -227,7 +246,7 @@ __device__ __forceinline__ Rounds rounds_of(int tiles) {
     return r;
 }
 
-template <int FORM, int TN>
+template <int FORM, int TN, bool SINGLES>
 __device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, const Rounds& rounds, int t) {
     Tile r;
     int g, local, mtiles, width = TN, part = 0;
@@ -238,12 +257,9 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, const
         width = TN / rounds.parts;
     }
     r.split = 0;
-    if constexpr (FORM == kForward) {
-        if (a.splits > 1) {
-            const int whole = t / a.splits;
-            r.split = t - whole * a.splits;
-            t = whole;
-        }
+    if constexpr (SINGLES) {
+        r.split = t % rounds.splits;
+        t /= rounds.splits;
     }
     if constexpr (FORM == kDw) {
         const int per = a.mtiles * a.ntiles;
@@ -268,9 +284,9 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, const
     const int sum = FORM == kDw ? r.end - r.begin : a.sum;
     r.steps = (sum + kStepK - 1) / kStepK;
     r.first = 0;
-    if constexpr (FORM == kForward) {
-        r.first = r.split * a.split_steps;
-        r.steps = min(a.split_steps, r.steps - r.first);
+    if constexpr (SINGLES) {
+        r.first = r.split * rounds.split_steps;
+        r.steps = min(rounds.split_steps, r.steps - r.first);
     }
     return r;
 }
@@ -323,7 +339,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_small,
                       const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_wide, TcArgs a) {
     using L = TcLayout<TN>;
-    constexpr int kStages = L::kStages, kEpilogue = epilogue_warps(SINGLES);
+    constexpr int kStages = L::kStages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // 1 KB: the 128-byte swizzle's atoms
@@ -384,13 +400,17 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
         } else {
             build_tile_table(start, a.offsets, a.groups, a.rows, kTileM, err);
         }
-        tiles = start[a.groups] * a.ntiles * (FORM == kForward ? a.splits : 1);
+        tiles = start[a.groups] * a.ntiles;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const Rounds rounds = rounds_of<TN>(tiles);
+    Rounds rounds = rounds_of<TN>(tiles);
+    if constexpr (SINGLES) {
+        choose_splits(rounds, tiles, (a.sum + kStepK - 1) / kStepK, a.most_splits);
+        rounds.units = rounds.whole = tiles * rounds.splits;  // cut along the sum, not the columns
+    }
 
     if (warp == 0) {
         // ---------------- producer
@@ -399,7 +419,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
             uint32_t phase = 1;
             bool ok = true;
             for (int t = blockIdx.x; ok && t < rounds.units; t += gridDim.x) {
-                const Tile r = tile_of<FORM, TN>(a, start, rounds, t);
+                const Tile r = tile_of<FORM, TN, SINGLES>(a, start, rounds, t);
                 const bool small = FORM != kDw && r.end - r.begin - r.m0 <= kSmallRows;
                 // Boxes of 64 columns that lie wholly past the operand are not loaded; their part of D is not stored.
                 if (r.cols == 0) continue;
@@ -447,7 +467,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
         int it = 0, n = 0;
         bool ok = true;
         for (int t = blockIdx.x; ok && t < rounds.units; t += gridDim.x) {
-            const Tile r = tile_of<FORM, TN>(a, start, rounds, t);
+            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, rounds, t);
             if (r.cols == 0) continue;
             const int buf = n & 1;
             const uint32_t acc = tmem + buf * TN;
@@ -505,8 +525,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
         const int n = singles, quads = a.outs / 4, warps = kSingleThreads / 32;
         if (blockIdx.x == 0) {
             const int first = threadIdx.x - 32 * (2 + kEpilogue);
-            if (first == 0) a.singles[0] = n;
-            for (int k = first; k < n; k += kSingleThreads) a.singles[1 + k] = single[k];
+            if (first == 0) a.singles[0] = n, a.singles[1] = rounds.splits;
+            for (int k = first; k < n; k += kSingleThreads) a.singles[2 + k] = single[k];
         }
         const long long items = static_cast<long long>(n) * quads;
         for (long long k = static_cast<long long>(blockIdx.x) * warps + warp - 2 - kEpilogue; k < items; k += static_cast<long long>(gridDim.x) * warps) {
@@ -515,14 +535,14 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
             else single_products<SPMM_DTYPE_F16>(a, g, q);
         }
     } else {
-        // ---------------- epilogue: two or four warps a lane quarter, alternate 32-column pieces
+        // ---------------- epilogue: two warps a lane quarter, alternate 32-column pieces
         const int q = warp & 3, part = (warp - 2) >> 2;  // warps q and q + 4 may access TMEM lanes 32 q ..
         const int size = a.out_f32 ? 4 : 2;
         const bool sectors = (reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) % 32 == 0;
         int n = 0;
         bool ok = true;
         for (int t = blockIdx.x; t < rounds.units; t += gridDim.x) {
-            const Tile r = tile_of<FORM, TN>(a, start, rounds, t);
+            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, rounds, t);
             if (r.cols == 0) continue;
             const int buf = n & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag))) {
@@ -642,8 +662,6 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     t.ldo = FORM == kDw ? a.K : a.ldo;
     t.out_f32 = a.out_f32;
     t.dtype = dtype;
-    t.splits = 1;
-    t.split_steps = (t.sum + kStepK - 1) / kStepK;
     t.err = a.err;
     // Row tiles: exact for dw, else as many as the groups can have (how many they do have is on the device).
     const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * t.mtiles : a.rows / kTileM + std::min(a.groups, a.rows);
@@ -702,8 +720,7 @@ int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st) 
     t.ldo = p.rank;
     t.out_f32 = 1;
     t.dtype = p.dtype;
-    t.splits = p.splits;
-    t.split_steps = p.steps_per_split;
+    t.most_splits = p.most_splits;
     t.split_stride = static_cast<long long>(p.rows) * p.rank;
     t.which = p.which;
     t.matrices = p.matrices;
@@ -713,7 +730,7 @@ int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st) 
     t.singles = p.singles;
     t.err = st->err;
     const int tn = p.rank <= 64 ? 64 : (p.rank <= 128 ? 128 : 256);
-    const int64_t tiles = (p.rows / kTileM + std::min<int64_t>(p.groups, p.rows)) * p.splits;
+    const int64_t tiles = (p.rows / kTileM + std::min<int64_t>(p.groups, p.rows)) * p.most_splits;
     if (tiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
     CUtensorMap ma, small, mb, wide;
     const uint64_t rows = p.rows, K = p.K, rank = p.rank;

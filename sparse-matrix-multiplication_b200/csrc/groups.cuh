@@ -74,10 +74,9 @@ __device__ __forceinline__ int tile_group(const int* start, int groups, int m) {
 // costs as much as one of 128.
 __device__ __forceinline__ bool is_single(const GroupRange& r) { return r.end - r.begin == 1; }
 
-// Partial sums of x[p] a[which[g]]^T (grouped_mm.cu), for lora.cu: parts[s][p][0 .. rank) for each of `splits` ranges of
-// steps_per_split * 64 of K, on the tensor cores; groups of one row have their whole sum in parts[0] and
-// are listed in `singles`. Rows of
-// groups without a matrix are not written. Operands on 16-byte boundaries, rank and K multiples of 8.
+// Partial sums of x[p] a[which[g]]^T (grouped_mm.cu), for lora.cu: parts[s][p][0 .. rank) for each of up to most_splits ranges
+// of K, on the tensor cores; groups of one row have their whole sum in parts[0]. Rows of groups without a matrix are not
+// written. Operands on 16-byte boundaries, rank and K multiples of 8.
 struct PartialProducts {
     const int* offsets;
     const int* which;
@@ -86,8 +85,8 @@ struct PartialProducts {
     long long ldx;
     const void* a;
     float* parts;
-    int* singles;  // their number, then the groups of one row in any order
-    int splits, steps_per_split;
+    int* singles;  // the number of groups of one row, the number of ranges, and those groups in order (2 + groups ints)
+    int most_splits;
 };
 int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st);
 

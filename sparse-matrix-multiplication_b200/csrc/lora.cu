@@ -250,8 +250,7 @@ struct ExpandLayout {
 
 struct ExpandArgs {
     LoraArgs l;
-    const int* singles;  // the requests of one row, from the shrink
-    int splits;
+    const int* singles;  // from the shrink: the number of requests of one row, of parts, and those requests
     int ntiles;        // column tiles
 };
 
@@ -294,6 +293,7 @@ template <int DT, int RB>
 __device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8_t* hi, int w, int warps) {
     const LoraArgs& a = e.l;
     const int pieces = (a.rank + 15) / 16 * 2;  // the last may lie past the rank and is zero
+    const int splits = e.singles[1];
     const float* parts = a.u + static_cast<long long>(x.row) * a.rank;
     const long long stride = static_cast<long long>(a.rows) * a.rank;
     for (int k = w * 32 + (threadIdx.x & 31); k < x.rows * pieces; k += warps * 32) {
@@ -302,7 +302,7 @@ __device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8
         if (8 * piece < a.rank) {
             const float* src = parts + static_cast<long long>(row) * a.rank + 8 * piece;
 #pragma unroll 4
-            for (int s = 0; s < e.splits; ++s) {
+            for (int s = 0; s < splits; ++s) {
                 const float4 lo = *reinterpret_cast<const float4*>(src + s * stride), hi4 = *reinterpret_cast<const float4*>(src + s * stride + 4);
                 f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w;
                 f[4] += hi4.x, f[5] += hi4.y, f[6] += hi4.z, f[7] += hi4.w;
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             for (long long k = items * blockIdx.x / gridDim.x; ok && k < last; ++k) {
                 if (k / pieces != m) {
                     m = static_cast<int>(k / pieces);
-                    const int r = e.singles[1 + m];
+                    const int r = e.singles[2 + m];
                     info.rows = 1;
                     info.row = group_range(a.offsets, r, a.rows, nullptr).begin;
                     info.i = adapter_of(a, r, nullptr);
@@ -700,7 +700,7 @@ int expand(const ExpandArgs& e0, int64_t mtiles, cudaStream_t s, DeviceState* st
 // How a call runs, by its sizes alone (the lengths are on the device). `fits`: 16-byte boundaries throughout.
 struct Shape {
     bool rows;         // CUDA cores, a few rows a request
-    int splits, steps_per_split;
+    int most_splits;   // parts of u
     int64_t mtiles;
 };
 
@@ -708,11 +708,8 @@ Shape shape_of(int32_t requests, int32_t rows, int32_t K) {
     Shape h{};
     h.rows = rows <= 4 * static_cast<int64_t>(requests);
     h.mtiles = rows / kTileM + std::min(requests, rows);
-    // Ranges of the sum over K until about eight tiles an SM (of 148) are there, each at least 8 steps of 64 long.
-    const int steps = (K + 63) / 64;
-    const int64_t want = h.rows ? 1 : std::max<int64_t>(1, std::min<int64_t>({8, 1184 / std::max<int64_t>(1, h.mtiles), steps / 8}));
-    h.steps_per_split = static_cast<int>((steps + want - 1) / want);
-    h.splits = h.steps_per_split ? (steps + h.steps_per_split - 1) / h.steps_per_split : 1;
+    // Ranges of the sum over K, from which the shrink chooses: enough that few tiles fill the GPU, each at least 4 steps of 64.
+    h.most_splits = h.rows ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 1184 / std::max<int64_t>(1, h.mtiles), K / 256})));
     return h;
 }
 
@@ -742,7 +739,7 @@ int spmm_lora_workspace_size(const spmm_lora_view* l, int32_t requests, int32_t 
     SPMM_TRY(check_view(l, requests, rows));
     if (!bytes) return SPMM_ERR_INVALID_ARG;
     const Shape h = shape_of(requests, rows, l->K);
-    *bytes = sizeof(float) * static_cast<size_t>(rows) * l->rank * h.splits + (h.rows ? 0 : sizeof(int) * (1 + static_cast<size_t>(requests)));
+    *bytes = sizeof(float) * static_cast<size_t>(rows) * l->rank * h.most_splits + (h.rows ? 0 : sizeof(int) * (2 + static_cast<size_t>(requests)));
     return SPMM_OK;
 }
 
@@ -807,13 +804,12 @@ int spmm_lora(const spmm_lora_view* l, const int32_t* offsets, const int32_t* ad
                                 dim3(static_cast<unsigned>(rows) * col_blocks), dim3(256), 0, s, a, col_blocks);
     }
     if (fits) {
-        PartialProducts p{offsets, adapter, requests, rows, l->adapters, l->rank, l->K, l->dtype, x, ldx, l->a, a.u, nullptr, h.splits, h.steps_per_split};
-        p.singles = reinterpret_cast<int*>(a.u + static_cast<size_t>(rows) * l->rank * h.splits);
+        PartialProducts p{offsets, adapter, requests, rows, l->adapters, l->rank, l->K, l->dtype, x, ldx, l->a, a.u, nullptr, h.most_splits};
+        p.singles = reinterpret_cast<int*>(a.u + static_cast<size_t>(rows) * l->rank * h.most_splits);
         SPMM_TRY(partial_products(p, s, st));
         ExpandArgs e{};
         e.l = a;
         e.singles = p.singles;
-        e.splits = h.splits;
         return bf16 ? expand<SPMM_DTYPE_BF16>(e, h.mtiles, s, st) : expand<SPMM_DTYPE_F16>(e, h.mtiles, s, st);
     }
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(rows, st->sm_count * 8)));
