@@ -364,8 +364,8 @@ int spmm_route_combine_grad(const spmm_route_view* r, const void* dy, int64_t ld
  * blocks). x is rows x K, y rows x N; rows in no group are left as they were. offsets (groups + 1, non-decreasing,
  * within [0, rows]) stays on the device; an offset out of order is clamped to its neighbours and recorded.
  * dtype F16 or BF16 (x, w); out_dtype the same or F32; sums in FP32. 16-byte aligned pointers and rows (N and K
- * multiples of 8, ldx/ldy * size multiples of 16) run on tcgen05; other operands on a slower kernel.
- * groups <= 4096 (SPMM_ERR_TOO_LARGE above). */
+ * multiples of 8, ldx/ldy * size multiples of 16) are loaded by TMA, other operands by the kernel's own warps, at about a
+ * fifth of the rate. groups <= 4096 (SPMM_ERR_TOO_LARGE above). */
 int spmm_grouped_mm(const int32_t* offsets, int32_t groups, int32_t rows, const void* x, int64_t ldx, const void* w,
                     void* y, int64_t ldy, int32_t N, int32_t K, int32_t dtype, int32_t out_dtype, void* stream);
 

@@ -31,112 +31,6 @@ struct GroupedArgs {
     DeviceErrorRecord* err;
 };
 
-// ------------------------------------------------------------------ any strides and alignment
-//
-// 64 x 64 tiles, 16 of k at a time through shared memory as FP32, 4 x 4 results a thread. For operands that TMA
-// cannot address (rows off 16-byte boundaries) and for empty sums.
-
-constexpr int kTile = 64;
-constexpr int kStep = 16;
-
-template <int FORM, int DT>
-__global__ void __launch_bounds__(256) grouped_any_kernel(GroupedArgs a) {
-    extern __shared__ int start[];
-    __shared__ float As[kStep][kTile + 1], Bs[kStep][kTile + 1];
-    grid_dependency_wait();
-    allow_dependent_launch();
-    const int outs = FORM == kDx ? a.K : (FORM == kForward ? a.N : a.K);  // columns of D
-    const int ntiles = (outs + kTile - 1) / kTile;
-    long long tiles;
-    if constexpr (FORM == kDw) {
-        tiles = static_cast<long long>(a.groups) * ((a.N + kTile - 1) / kTile) * ntiles;
-    } else {
-        build_tile_table(start, a.offsets, a.groups, a.rows, kTile, blockIdx.x == 0 ? a.err : nullptr);
-        tiles = static_cast<long long>(start[a.groups]) * ntiles;
-    }
-    const int tm = (threadIdx.x / 16) * 4, tn = (threadIdx.x % 16) * 4;
-    for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const int nt = static_cast<int>(t % ntiles) * kTile;
-        int g, m0, ms, ks;  // group, first row of D in the group, rows of D, length of the sum
-        GroupRange r;
-        if constexpr (FORM == kDw) {
-            const int mtiles = (a.N + kTile - 1) / kTile;
-            const int mt = static_cast<int>((t / ntiles) % mtiles);
-            g = static_cast<int>(t / ntiles / mtiles);
-            r = group_range(a.offsets, g, a.rows, nt == 0 && mt == 0 ? a.err : nullptr);
-            m0 = mt * kTile;
-            ms = a.N;
-            ks = r.end - r.begin;
-        } else {
-            const int mt = static_cast<int>(t / ntiles);
-            g = tile_group(start, a.groups, mt);
-            r = group_range(a.offsets, g, a.rows, nullptr);
-            m0 = (mt - start[g]) * kTile;
-            ms = r.end - r.begin;
-            ks = FORM == kForward ? a.K : a.N;
-        }
-        float acc[4][4] = {};
-        for (int k0 = 0; k0 < ks; k0 += kStep) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-                // Consecutive threads take the index that is contiguous in memory.
-                const int mk_k = FORM == kDw ? i / kTile : i % kStep, mk_m = FORM == kDw ? i % kTile : i / kStep;
-                float v = 0.f;
-                if (m0 + mk_m < ms && k0 + mk_k < ks) {
-                    const long long row = FORM == kDw ? r.begin + k0 + mk_k : r.begin + m0 + mk_m;
-                    const int col = FORM == kDw ? m0 + mk_m : k0 + mk_k;
-                    v = half_bits_to_float<DT>(__ldg(a.a + row * a.lda + col));
-                }
-                As[mk_k][mk_m] = v;
-                const int nk_k = FORM == kForward ? i % kStep : i / kTile, nk_n = FORM == kForward ? i / kStep : i % kTile;
-                v = 0.f;
-                if (nt + nk_n < outs && k0 + nk_k < ks) {
-                    long long at;
-                    if constexpr (FORM == kForward) at = (static_cast<long long>(g) * a.N + nt + nk_n) * a.K + k0 + nk_k;
-                    else if constexpr (FORM == kDx) at = (static_cast<long long>(g) * a.N + k0 + nk_k) * a.K + nt + nk_n;
-                    else at = static_cast<long long>(r.begin + k0 + nk_k) * a.ldb + nt + nk_n;
-                    v = half_bits_to_float<DT>(__ldg(a.b + at));
-                }
-                Bs[nk_k][nk_n] = v;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kStep; ++k) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(As[k][tm + i], Bs[k][tn + j], acc[i][j]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int m = m0 + tm + i;
-            if (m >= ms) continue;
-            const long long row = FORM == kDw ? (static_cast<long long>(g) * a.N + m) * a.K : (r.begin + m) * a.ldo;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = nt + tn + j;
-                if (n >= outs) continue;
-                if (a.out_f32) static_cast<float*>(a.out)[row + n] = acc[i][j];
-                else static_cast<uint16_t*>(a.out)[row + n] = float_to_half_bits<DT>(acc[i][j]);
-            }
-        }
-    }
-}
-
-template <int FORM>
-int any_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st) {
-    const size_t smem = FORM == kDw ? 0 : sizeof(int) * (static_cast<size_t>(a.groups) + 1);
-    const int outs = FORM == kForward ? a.N : a.K;
-    const int64_t ntiles = (outs + kTile - 1) / kTile;
-    const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * ((a.N + kTile - 1) / kTile)
-                                       : a.rows / kTile + std::min<int64_t>(a.groups, a.rows);
-    const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(mtiles * ntiles, st->sm_count * 6)));
-    if (dtype == SPMM_DTYPE_BF16)
-        return launch_dependent(grouped_any_kernel<FORM, SPMM_DTYPE_BF16>, dim3(grid), dim3(256), smem, s, a);
-    return launch_dependent(grouped_any_kernel<FORM, SPMM_DTYPE_F16>, dim3(grid), dim3(256), smem, s, a);
-}
-
 // ------------------------------------------------------------------ tcgen05
 //
 // A persistent block takes 128 x TN tiles of D, 64 of k a step: one warp issues TMA copies into a ring of stages, one
@@ -153,19 +47,23 @@ constexpr int kTileM = 128;
 constexpr int kStepK = 64;
 constexpr int kBand = 8;          // row tiles that run together down a band (their A and the band's B stay in L2)
 // Warp 0 TMA, warp 1 MMA, then the epilogue's (sixteen were 2 to 5 % slower on large products), then, with SINGLES, eight
-// for the groups of one row.
+// for the groups of one row, or with ANY sixteen that load in TMA's place.
 constexpr int kEpilogue = 8;
 constexpr int kSingleThreads = 256;
-constexpr int tc_threads(bool singles) { return 64 + 32 * kEpilogue + (singles ? kSingleThreads : 0); }
+constexpr int kLoaders = 16;
+constexpr int tc_threads(bool singles, bool any) { return 64 + 32 * kEpilogue + (singles ? kSingleThreads : 0) + (any ? 32 * kLoaders : 0); }
 constexpr int kSmallRows = 32;    // groups with no more rows left load a box of this many
 
-template <int TN>
+constexpr int kTransposed = 32 * 33 * 4;  // ANY: an epilogue warp's 32 x 32 results, to be stored by columns of lanes
+
+template <int TN, bool ANY>
 struct TcLayout {
     static constexpr int kA = kTileM * kStepK * 2;
     static constexpr int kB = TN * kStepK * 2;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = TN == 256 ? 4 : (TN == 128 ? 6 : 8);  // 192 KB
-    static constexpr int kBars = kStages * kStage;    // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
+    static constexpr int kStages = ANY ? 4 : (TN == 256 ? 4 : (TN == 128 ? 6 : 8));  // 192 KB, 128 with ANY
+    static constexpr int kOut = kStages * kStage;
+    static constexpr int kBars = kOut + (ANY ? kEpilogue * kTransposed : 0);  // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
     static constexpr int kTable = kBars + 8 * (2 * kStages + 5) + 16;
     static constexpr int kFixed = kTable + 1024;     // room to align the base to 1 KB; then int[groups + 1]
 };
@@ -187,11 +85,11 @@ struct TcArgs {
     long long split_stride;
     const int* __restrict__ which;
     int matrices;
-    // SINGLES only: the operands themselves.
+    int* singles;      // their number and the groups, for the caller
+    // SINGLES and ANY: the operands themselves (A; B, with its stride in dw).
     const uint16_t* __restrict__ x;
     const uint16_t* __restrict__ b;
-    long long ldx;
-    int* singles;      // their number and the groups, for the caller
+    long long ldx, ldb;
     DeviceErrorRecord* err;
 };
 
@@ -292,12 +190,12 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, const
 }
 
 // The MMAs of one stage, 16 of k each; the first overwrites the accumulator unless `add`.
-template <int FORM, int TN>
+template <int FORM>
 __device__ __forceinline__ void mma_step(uint32_t acc, uint32_t stage, uint32_t idesc, int slices, bool add) {
     // From one slice to the next: 32 bytes along a K-major row, two 8-row atoms down an MN-major column (units of 16).
     constexpr uint64_t kNextA = FORM == kDw ? 128 : 2, kNextB = FORM == kForward ? 2 : 128;
     const uint64_t da = FORM == kDw ? smem_desc(stage, 8192, 1024, kSwizzle128) : smem_desc(stage, 16, 1024, kSwizzle128);
-    const uint32_t sb = stage + TcLayout<TN>::kA;
+    const uint32_t sb = stage + kTileM * kStepK * 2;
     const uint64_t db = FORM == kForward ? smem_desc(sb, 16, 1024, kSwizzle128) : smem_desc(sb, 8192, 1024, kSwizzle128);
     if (slices == 4) {
         umma_f16(acc, da, db, idesc, add ? 1u : 0u);
@@ -333,12 +231,87 @@ __device__ __forceinline__ void single_products(const TcArgs& a, int g, int q) {
     if (lane == 0) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * a.ldo + q) = make_float4(s[0], s[1], s[2], s[3]);
 }
 
+// ANY: operands off 16-byte boundaries, which TMA cannot address. Sixteen warps fill the stages instead, in the layout that
+// TMA would have written: a lane reads the two aligned 16-byte vectors that hold its eight elements and shifts them into
+// place, so the reads are as wide as TMA's; elements past the operand are zero. 5003 rows over 60 groups, N = 999,
+// K = 1957: 226 us (a CUDA-core kernel: 1.7 ms); 16384 rows over 8, N = 2047, K = 2049: 200 TFLOP/s, bound by these loads.
+
+// The eight elements from `at` on, of which `count` belong to the row (at most 0: none).
+struct Unaligned {
+    uint4 lo, hi;
+    int shift, count;
+};
+
+__device__ __forceinline__ Unaligned load_unaligned(const uint16_t* at, int count) {
+    Unaligned v;
+    const uintptr_t p = reinterpret_cast<uintptr_t>(at);
+    const uint4* base = reinterpret_cast<const uint4*>(p & ~static_cast<uintptr_t>(15));
+    v.shift = static_cast<int>(p & 15);
+    v.count = min(count, 8);
+    v.lo = v.hi = make_uint4(0, 0, 0, 0);
+    // A vector that holds a byte of the row lies in the row's allocation whole.
+    if (v.count > 0) v.lo = __ldg(base);
+    if (v.shift + 2 * v.count > 16) v.hi = __ldg(base + 1);
+    return v;
+}
+
+__device__ __forceinline__ uint4 shift_unaligned(const Unaligned& v) {
+    const uint32_t w[8] = {v.lo.x, v.lo.y, v.lo.z, v.lo.w, v.hi.x, v.hi.y, v.hi.z, v.hi.w};
+    uint32_t t[6], u[5], o[4];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) t[i] = v.shift & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) u[i] = v.shift & 4 ? t[i + 1] : t[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        o[i] = __funnelshift_r(u[i], u[i + 1], (v.shift & 2) * 8);
+        o[i] = 2 * i >= v.count ? 0u : (2 * i + 1 >= v.count ? o[i] & 0xffffu : o[i]);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Row `line` of a stage's 128-byte rows (A's 128, then B's TN) at step k0: where its 64 elements begin and how many are real.
+template <int FORM>
+__device__ __forceinline__ const uint16_t* stage_line(const TcArgs& a, const Tile& r, int k0, int line, int* count) {
+    const bool in_a = line < kTileM;
+    const int l = in_a ? line : line - kTileM, box = l & ~63, k = k0 + (l & 63);  // MN-major: boxes of 64 columns, rows of k
+    bool real;
+    int col, cols;
+    const uint16_t* row;
+    if (FORM == kDw) {
+        const long long p = r.begin + k;
+        real = p < r.end;
+        col = (in_a ? r.m0 : r.n0) + box;
+        cols = in_a ? a.ms : r.n0 + r.cols;
+        row = in_a ? a.x + p * a.ldx : a.b + p * a.ldb;
+    } else if (in_a) {
+        const long long p = r.begin + r.m0 + l;
+        real = p < r.end;
+        col = k0;
+        cols = a.sum;
+        row = a.x + p * a.ldx;
+    } else if (FORM == kForward) {
+        const int n = r.n0 + l;
+        real = l < r.cols;
+        col = k0;
+        cols = a.sum;
+        row = a.b + (static_cast<long long>(r.g) * a.outs + n) * a.sum;
+    } else {
+        real = k < a.sum;
+        col = r.n0 + box;
+        cols = r.n0 + r.cols;
+        row = a.b + (static_cast<long long>(r.g) * a.sum + k) * a.outs;
+    }
+    *count = real ? cols - col : 0;
+    return row + col;
+}
+
 // SINGLES (forward, FP32 out): groups of one row are left to eight warps more.
-template <int FORM, int TN, bool SINGLES>
-__global__ void __launch_bounds__(tc_threads(SINGLES), 1)
+template <int FORM, int TN, bool SINGLES, bool ANY>
+__global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_small,
                       const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_wide, TcArgs a) {
-    using L = TcLayout<TN>;
+    using L = TcLayout<TN, ANY>;
     constexpr int kStages = L::kStages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
@@ -356,7 +329,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(full0 + 8 * s, 1);
+            mbar_init(full0 + 8 * s, ANY ? kLoaders : 1);
             mbar_init(empty0 + 8 * s, 1);
         }
         for (int s = 0; s < 2; ++s) {
@@ -365,8 +338,10 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
         }
         mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        prefetch_tensormap(&map_a);
-        prefetch_tensormap(&map_b);
+        if constexpr (!ANY) {
+            prefetch_tensormap(&map_a);
+            prefetch_tensormap(&map_b);
+        }
     }
     if (warp == 1) tmem_alloc(smem_addr(tmem_slot), 2 * TN);
     grid_dependency_wait();
@@ -414,7 +389,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
 
     if (warp == 0) {
         // ---------------- producer
-        if (elect_one()) {
+        if (!ANY && elect_one()) {
             int it = 0, s = 0;
             uint32_t phase = 1;
             bool ok = true;
@@ -474,7 +449,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
             const uint32_t idesc = instr_desc_f16(a.dtype, (r.cols + 15) / 16 * 16, FORM == kDw, FORM != kForward);
             const int sum = FORM == kDw ? r.end - r.begin : a.sum;
             const int left = min(kStepK, sum - (r.first + r.steps - 1) * kStepK);  // of the last step
-            const int clear = FORM == kDw && left % 16 != 0;
+            const int clear = FORM == kDw && !ANY && left % 16 != 0;
             if (elect_one()) {
                 ok = mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag);
                 tc_fence_after();
@@ -484,14 +459,14 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
                     ok = mbar_wait(full0 + 8 * s, phase, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    mma_step<FORM, TN>(acc, sbase + s * L::kStage, idesc, ks == r.steps - 1 ? (left + 15) / 16 : 4, ks > 0);
+                    mma_step<FORM>(acc, sbase + s * L::kStage, idesc, ks == r.steps - 1 ? (left + 15) / 16 : 4, ks > 0);
                     umma_commit(empty0 + 8 * s);
                     if (++s == kStages) s = 0, phase ^= 1u;
                 }
             }
             ok = __all_sync(0xffffffffu, ok);
             it += r.steps;
-            if (FORM == kDw && clear && ok) {
+            if (FORM == kDw && !ANY && clear && ok) {
                 const int s = (it - 1) % kStages, slices = (left + 15) / 16;
                 ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, ((it - 1) / kStages) & 1u, abort_flag));
                 if (ok) {
@@ -506,7 +481,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
                     __syncwarp();
                     tc_fence_after();
                     if (elect_one()) {
-                        mma_step<FORM, TN>(acc, sbase + s * L::kStage, idesc, slices, r.steps > 1);
+                        mma_step<FORM>(acc, sbase + s * L::kStage, idesc, slices, r.steps > 1);
                         umma_commit(empty0 + 8 * s);
                     }
                     __syncwarp();
@@ -534,6 +509,44 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
             if (a.dtype == SPMM_DTYPE_BF16) single_products<SPMM_DTYPE_BF16>(a, g, q);
             else single_products<SPMM_DTYPE_F16>(a, g, q);
         }
+    } else if (ANY && warp >= 2 + kEpilogue) {
+        // ---------------- loads in TMA's place: eight lanes to a row of 128 bytes, 64 rows a pass, two passes' reads together
+        const int group = (warp - 2 - kEpilogue) * 4 + lane / 8, piece = lane & 7;
+        int s = 0;
+        uint32_t phase = 1;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < rounds.units; t += gridDim.x) {
+            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, rounds, t);
+            if (r.cols == 0) continue;
+            for (int ks = 0; ks < r.steps; ++ks) {
+                ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, phase, abort_flag));
+                if (!ok) break;
+                uint8_t* stage = base + s * L::kStage;
+                for (int line = group; line < kTileM + TN; line += 128) {
+                    Unaligned v[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        int count;
+                        const uint16_t* at = stage_line<FORM>(a, r, ks * kStepK, line + 64 * j, &count);
+                        v[j] = load_unaligned(at + 8 * piece, count - 8 * piece);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) *swizzled_piece(stage, line + 64 * j, piece) = shift_unaligned(v[j]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_count(full0 + 8 * s, 1);
+                if (++s == kStages) s = 0, phase ^= 1u;
+            }
+        }
+        for (int k = 0; ok && k < kStages; ++k) {  // the MMAs' last arrivals come before the block ends
+            ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, phase, abort_flag));
+            if (++s == kStages) s = 0, phase ^= 1u;
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_device_error(a.err, SPMM_ERR_TIMEOUT, 14);
+        }
     } else {
         // ---------------- epilogue: two warps a lane quarter, alternate 32-column pieces
         const int q = warp & 3, part = (warp - 2) >> 2;  // warps q and q + 4 may access TMEM lanes 32 q ..
@@ -559,11 +572,26 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
                 for (int c0 = part * 32; c0 < cols; c0 += 8 * kEpilogue) {
                     uint32_t v[32];
                     tmem_ld32(acc + c0, v);
-                    if (FORM == kDw && r.steps == 0) {
+                    if ((FORM == kDw || ANY) && r.steps == 0) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = 0u;
                     }
-                    if (row >= rows) {
+                    if constexpr (ANY) {
+                        // Elements one by one, a row's 32 by the warp's lanes.
+                        float* tile = reinterpret_cast<float*>(base + L::kOut + (warp - 2) * kTransposed);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) tile[lane * 33 + i] = __uint_as_float(v[i]);
+                        __syncwarp();
+                        char* corner = static_cast<char*>(a.out) + ((at - lane) * a.ldo + r.n0 + c0 + lane) * size;
+                        const int high = c0 + lane < cols ? min(32, rows - (row - lane)) : 0;
+#pragma unroll 8
+                        for (int i = 0; i < high; ++i) {
+                            const float f = tile[i * 33 + lane];
+                            char* o = corner + i * a.ldo * size;
+                            if (a.out_f32) *reinterpret_cast<float*>(o) = f;
+                            else *reinterpret_cast<uint16_t*>(o) = a.dtype == SPMM_DTYPE_BF16 ? float_to_half_bits<SPMM_DTYPE_BF16>(f) : float_to_half_bits<SPMM_DTYPE_F16>(f);
+                        }
+                    } else if (row >= rows) {
                         // nothing to store
                     } else if (a.out_f32) {
 #pragma unroll
@@ -619,29 +647,29 @@ __global__ void __launch_bounds__(tc_threads(SINGLES), 1)
     }
 }
 
-template <int FORM, int TN, bool SINGLES = false>
+template <int FORM, int TN, bool SINGLES = false, bool ANY = false>
 int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap& mb, const CUtensorMap& wide, const TcArgs& a, long long tiles, cudaStream_t s,
               DeviceState* st) {
-    using L = TcLayout<TN>;
+    using L = TcLayout<TN, ANY>;
     // The attribute belongs to the device's context: set once a device, for the largest table.
     static std::atomic<unsigned long long> attr_set{0};
     const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
     if (!bit || !(attr_set.load(std::memory_order_acquire) & bit)) {
-        SPMM_CUDA_TRY(cudaFuncSetAttribute(grouped_tc_kernel<FORM, TN, SINGLES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        SPMM_CUDA_TRY(cudaFuncSetAttribute(grouped_tc_kernel<FORM, TN, SINGLES, ANY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            L::kFixed + 4 * (SPMM_MAX_GROUPS + 1)));
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     const size_t smem = L::kFixed + (FORM == kDw ? 0 : 4 * (static_cast<size_t>(a.groups) + 1));
     const unsigned grid = static_cast<unsigned>(SINGLES ? st->sm_count : std::min<long long>(tiles * (TN / 64), st->sm_count));
-    return launch_dependent(grouped_tc_kernel<FORM, TN, SINGLES>, dim3(grid), dim3(tc_threads(SINGLES)), smem, s, ma, small, mb, wide, a);
+    return launch_dependent(grouped_tc_kernel<FORM, TN, SINGLES, ANY>, dim3(grid), dim3(tc_threads(SINGLES, ANY)), smem, s, ma, small, mb, wide, a);
 }
 
 bool fits16(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
 
 // Whether TMA and stores of 16 bytes can address the operands.
 template <int FORM>
-bool tc_fits(const GroupedArgs& a, DeviceState* st) {
-    if (st->cc_major != 10 || a.N % 8 || a.K % 8 || a.rows == 0 || a.N == 0 || a.K == 0) return false;
+bool tma_fits(const GroupedArgs& a) {
+    if (a.N % 8 || a.K % 8 || a.rows == 0 || a.N == 0 || a.K == 0) return false;
     const int size = a.out_f32 ? 4 : 2;
     if (!fits16(a.a, a.lda, 2) || !fits16(a.b, FORM == kDw ? a.ldb : 8, 2)) return false;
     return fits16(a.out, FORM == kDw ? 8 : a.ldo, size);
@@ -649,7 +677,8 @@ bool tc_fits(const GroupedArgs& a, DeviceState* st) {
 
 template <int FORM>
 int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState* st) {
-    if (!tc_fits<FORM>(a, st)) return any_launch<FORM>(a, dtype, s, st);
+    if (st->cc_major != 10) return SPMM_ERR_UNSUPPORTED;
+    const bool any = !tma_fits<FORM>(a);  // also empty sums, for which there is nothing to map
     TcArgs t{};
     t.offsets = a.offsets;
     t.groups = a.groups;
@@ -662,17 +691,23 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     t.ldo = FORM == kDw ? a.K : a.ldo;
     t.out_f32 = a.out_f32;
     t.dtype = dtype;
+    t.x = a.a;
+    t.b = a.b;
+    t.ldx = a.lda;
+    t.ldb = a.ldb;
     t.err = a.err;
     // Row tiles: exact for dw, else as many as the groups can have (how many they do have is on the device).
     const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * t.mtiles : a.rows / kTileM + std::min(a.groups, a.rows);
     // The widest tile that still gives every SM one: a wide tile reads A less often, narrow ones spread few rows.
     int tn = 256;
-    while (tn > 64 && (mtiles * ((t.outs + tn - 1) / tn) < st->sm_count || t.outs <= tn / 2)) tn /= 2;
+    if (any) tn = 128;
+    while (!any && tn > 64 && (mtiles * ((t.outs + tn - 1) / tn) < st->sm_count || t.outs <= tn / 2)) tn /= 2;
     t.ntiles = (t.outs + tn - 1) / tn;
     const int64_t tiles = mtiles * t.ntiles;
     if (tiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
 
-    CUtensorMap ma, small, mb, wide{};
+    CUtensorMap ma{}, small{}, mb{}, wide{};
+    if (any) return tc_launch<FORM, 128, false, true>(ma, small, mb, wide, t, tiles, s, st);
     const uint64_t rows = a.rows, N = a.N, K = a.K;
     const uint64_t inner = FORM == kForward ? K : N;  // columns of A's operand
     SPMM_TRY(encode_2d(&ma, a.a, inner, rows, a.lda * 2, 64, FORM == kDw ? 64 : kTileM, CU_TENSOR_MAP_SWIZZLE_128B));

@@ -84,7 +84,7 @@ def test_widths(cuda, N, K):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("N,K,pad,shift", [(1, 1, 0, 0), (7, 13, 0, 0), (65, 130, 0, 0), (9, 300, 0, 0), (64, 64, 1, 0), (64, 64, 0, 1), (72, 40, 3, 5)])
+@pytest.mark.parametrize("N,K,pad,shift", [(1, 1, 0, 0), (7, 13, 0, 0), (65, 130, 0, 0), (9, 300, 0, 0), (64, 64, 1, 0), (64, 64, 0, 1), (72, 40, 3, 5), (515, 1001, 0, 0)])
 def test_operands_off_16_byte_boundaries(cuda, N, K, pad, shift, dtype):
     check_all([3, 70, 0, 1], N, K, dtype, pad=pad, shift=shift, tail=2)
 
