@@ -55,15 +55,16 @@ constexpr int tc_threads(bool singles, bool any) { return 64 + 32 * kEpilogue + 
 constexpr int kSmallRows = 32;    // groups with no more rows left load a box of this many
 
 constexpr int kTransposed = 32 * 33 * 4;  // ANY: an epilogue warp's 32 x 32 results, to be stored by columns of lanes
+constexpr int kStoreBox = 32 * 128;       // dw: an epilogue warp's 32 rows of 128 bytes, for TMA to store
 
-template <int TN, bool ANY>
+template <int FORM, int TN, bool ANY>
 struct TcLayout {
     static constexpr int kA = kTileM * kStepK * 2;
     static constexpr int kB = TN * kStepK * 2;
     static constexpr int kStage = kA + kB;
     static constexpr int kStages = ANY ? 4 : (TN == 256 ? 4 : (TN == 128 ? 6 : 8));  // 192 KB, 128 with ANY
     static constexpr int kOut = kStages * kStage;
-    static constexpr int kBars = kOut + (ANY ? kEpilogue * kTransposed : 0);  // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
+    static constexpr int kBars = kOut + (ANY ? kEpilogue * kTransposed : (FORM == kDw ? kEpilogue * kStoreBox : 0));  // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
     static constexpr int kTable = kBars + 8 * (2 * kStages + 5) + 16;
     static constexpr int kFixed = kTable + 1024;     // room to align the base to 1 KB; then int[groups + 1]
 };
@@ -310,8 +311,8 @@ __device__ __forceinline__ const uint16_t* stage_line(const TcArgs& a, const Til
 template <int FORM, int TN, bool SINGLES, bool ANY>
 __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_a_small,
-                      const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_wide, TcArgs a) {
-    using L = TcLayout<TN, ANY>;
+                      const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b_wide /* dw: the output */, TcArgs a) {
+    using L = TcLayout<FORM, TN, ANY>;
     constexpr int kStages = L::kStages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
@@ -568,11 +569,48 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
             const long long at = FORM == kDw ? static_cast<long long>(r.g) * a.ms + row : r.begin + row;
             char* out = static_cast<char*>(a.out) + (at * a.ldo + r.n0 + r.split * a.split_stride) * size;
             const int cols = r.cols;
-            if (r.m0 + q * 32 < rows) {
+            if (FORM == kDw && !ANY && r.m0 + q * 32 < rows) {
+                // dw's tiles end where the operand does, which TMA knows: whole boxes through shared memory, nothing waits for
+                // them. (Each lane its row's sectors, as below, is one line a lane: 2.2 us for a tile of 128 x 256 in FP32.)
+                uint8_t* box = base + L::kOut + (warp - 2) * kStoreBox;
+                const int per = 128 / size;  // columns of a box
+                for (int c0 = part * per; c0 < cols; c0 += 2 * per) {
+                    if (lane == 0) bulk_store_read_wait();
+                    __syncwarp();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h && a.out_f32) break;
+                        uint32_t v[32];
+                        tmem_ld32(acc + c0 + 32 * h, v);
+                        if (r.steps == 0) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = 0u;
+                        }
+                        if (a.out_f32) {
+#pragma unroll
+                            for (int c = 0; c < 8; ++c) *swizzled_piece(box, lane, c) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float lo = __uint_as_float(v[8 * c + 2 * i]), hi = __uint_as_float(v[8 * c + 2 * i + 1]);
+                                    w[i] = a.dtype == SPMM_DTYPE_BF16 ? pack_half2<SPMM_DTYPE_BF16>(lo, hi) : pack_half2<SPMM_DTYPE_F16>(lo, hi);
+                                }
+                                *swizzled_piece(box, lane, 4 * h + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) tma_store_3d(&map_b_wide, smem_addr(box), r.n0 + c0, r.m0 + q * 32, r.g);
+                }
+            } else if (r.m0 + q * 32 < rows) {
                 for (int c0 = part * 32; c0 < cols; c0 += 8 * kEpilogue) {
                     uint32_t v[32];
                     tmem_ld32(acc + c0, v);
-                    if ((FORM == kDw || ANY) && r.steps == 0) {
+                    if (ANY && r.steps == 0) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = 0u;
                     }
@@ -623,6 +661,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
             if (lane == 0) mbar_arrive_count(acc_empty0 + 8 * buf, 1);
             ++n;
         }
+        if (FORM == kDw && !ANY && lane == 0) bulk_store_wait();
         if (!ok && lane == 0) {
             *abort_flag = 1;
             record_device_error(a.err, SPMM_ERR_TIMEOUT, 13);
@@ -650,13 +689,13 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
 template <int FORM, int TN, bool SINGLES = false, bool ANY = false>
 int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap& mb, const CUtensorMap& wide, const TcArgs& a, long long tiles, cudaStream_t s,
               DeviceState* st) {
-    using L = TcLayout<TN, ANY>;
+    using L = TcLayout<FORM, TN, ANY>;
     // The attribute belongs to the device's context: set once a device, for the largest table.
     static std::atomic<unsigned long long> attr_set{0};
     const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
     if (!bit || !(attr_set.load(std::memory_order_acquire) & bit)) {
         SPMM_CUDA_TRY(cudaFuncSetAttribute(grouped_tc_kernel<FORM, TN, SINGLES, ANY>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           L::kFixed + 4 * (SPMM_MAX_GROUPS + 1)));
+                                           L::kFixed + (FORM == kDw ? 0 : 4 * (SPMM_MAX_GROUPS + 1))));
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     const size_t smem = L::kFixed + (FORM == kDw ? 0 : 4 * (static_cast<size_t>(a.groups) + 1));
@@ -714,6 +753,9 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     SPMM_TRY(encode_2d(&small, a.a, inner, rows, a.lda * 2, 64, kSmallRows, CU_TENSOR_MAP_SWIZZLE_128B));
     if constexpr (FORM == kDw) {
         SPMM_TRY(encode_2d(&mb, a.b, K, rows, a.ldb * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+        const uint64_t size = a.out_f32 ? 4 : 2;  // the output's map
+        SPMM_TRY(encode_3d(&wide, a.out, {K, N, static_cast<uint64_t>(a.groups)}, {K * size, N * K * size}, {static_cast<uint32_t>(128 / size), 32, 1},
+                           CU_TENSOR_MAP_SWIZZLE_128B, a.out_f32));
     } else {
         const auto encode_w = [&](CUtensorMap* map, int box_rows) {
             return encode_3d(map, a.b, {K, N, static_cast<uint64_t>(a.groups)}, {K * 2, N * K * 2}, {64, static_cast<uint32_t>(box_rows), 1},

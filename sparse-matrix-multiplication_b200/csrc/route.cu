@@ -298,8 +298,9 @@ __global__ void __launch_bounds__(128) route_combine_kernel(RouteArgs a, const c
 }
 
 // dys[pos[t, j]] = w[t, j] dy[t], dw[t, j] = <dy[t], ys[pos[t, j]]>: one block row (blockDim.x threads) takes a whole
-// token, J pairs at a time, so that a dot product is one tree in a fixed order and needs no second pass.
-template <int DT, int VB, int J>
+// token, J pairs and U vectors at a time (their loads in flight together), so that a dot product is one tree in a fixed
+// order and needs no second pass.
+template <int DT, int VB, int J, int U>
 __global__ void __launch_bounds__(256)
     route_combine_grad_kernel(RouteArgs a, const char* __restrict__ dy, long long lddy, const char* __restrict__ ys, long long ldys,
                               const float* __restrict__ w, char* __restrict__ dys, long long lddys, float* __restrict__ dw) {
@@ -325,38 +326,48 @@ __global__ void __launch_bounds__(256)
             if (w) wj[j] = __ldg(w + pair);
         }
         if (real) {
-            for (int c = threadIdx.x; c < a.nvec; c += tx) {
-                const V dv = __ldg(reinterpret_cast<const V*>(dy + t * lddy) + c);
-                V v[J];
-                if (dw) {
+            for (int c0 = threadIdx.x; c0 < a.nvec; c0 += tx * U) {
+                V dv[U], v[U][J];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int c = c0 + u * tx;
+                    if (c >= a.nvec) break;
+                    dv[u] = __ldg(reinterpret_cast<const V*>(dy + t * lddy) + c);
+                    if (!dw) continue;
 #pragma unroll
                     for (int j = 0; j < J; ++j)
-                        if (p[j] >= 0) v[j] = __ldg(reinterpret_cast<const V*>(ys + p[j] * ldys) + c);
+                        if (p[j] >= 0) v[u][j] = __ldg(reinterpret_cast<const V*>(ys + p[j] * ldys) + c);
                 }
-                float g[R::N];
-                R::unpack(dv, g);
 #pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    if (p[j] < 0) continue;
-                    if (dys) {
-                        float o[R::N];
+                for (int u = 0; u < U; ++u) {
+                    const int c = c0 + u * tx;
+                    if (c >= a.nvec) break;
+                    float g[R::N];
+                    R::unpack(dv[u], g);
 #pragma unroll
-                        for (int i = 0; i < R::N; ++i) o[i] = wj[j] * g[i];
-                        reinterpret_cast<V*>(dys + p[j] * lddys)[c] = R::pack(o);
-                    }
-                    if (dw) {
-                        float f[R::N];
-                        R::unpack(v[j], f);
+                    for (int j = 0; j < J; ++j) {
+                        if (p[j] < 0) continue;
+                        if (dys) {
+                            float o[R::N];
 #pragma unroll
-                        for (int i = 0; i < R::N; ++i) dot[j] = fmaf(g[i], f[i], dot[j]);
+                            for (int i = 0; i < R::N; ++i) o[i] = wj[j] * g[i];
+                            reinterpret_cast<V*>(dys + p[j] * lddys)[c] = R::pack(o);
+                        }
+                        if (dw) {
+                            float f[R::N];
+                            R::unpack(v[u][j], f);
+#pragma unroll
+                            for (int i = 0; i < R::N; ++i) dot[j] = fmaf(g[i], f[i], dot[j]);
+                        }
                     }
                 }
             }
         }
         if (!dw) continue;
+        for (int d = min(tx, 32) / 2; d > 0; d /= 2) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-            for (int d = min(tx, 32) / 2; d > 0; d /= 2) dot[j] += __shfl_xor_sync(kFull, dot[j], d);
+            for (int j = 0; j < J; ++j) dot[j] += __shfl_xor_sync(kFull, dot[j], d);
+        }
         if (tx <= 32) {
             if (real && threadIdx.x == 0) {
 #pragma unroll
@@ -388,7 +399,7 @@ __global__ void __launch_bounds__(256)
 // sums and writes before it looks up the next token's. Lane j of the producer warp issues pair j's copies, its position read
 // a token ahead; the consumer warps share every stage (a warp that took only some of them could not tell one phase of a
 // stage's barrier from the one two later). 16384 tokens x 8
-// rows of 4 KB: 279 us by the kernel above (4.1 TB/s), 206 us streamed; the other two operators gain nothing by it
+// rows of 4 KB: 248 us by the kernel above (4.6 TB/s), 206 us streamed; the other two operators gain nothing by it
 // (gather 198 -> 215 us, combine 212 -> 207 us at 8 KB rows).
 
 constexpr int kRing = 196608;          // bytes of the ring
@@ -635,9 +646,14 @@ int combine_grad_launch(RouteArgs a, const void* dy, int64_t lddy, const void* y
     a.chunks = 1;
     unsigned grid = 0;
     SPMM_TRY(row_grid(a, block, &grid));
-    return launch_dependent(route_combine_grad_kernel<DT, VB, 8>, dim3(grid), block, 0, s, a, static_cast<const char*>(dy),
-                            static_cast<long long>(lddy), static_cast<const char*>(ys), static_cast<long long>(ldys), w,
-                            static_cast<char*>(dys), static_cast<long long>(lddys), dw);
+    // Eight 16-byte loads at a time, twice as many narrow ones (777 tokens x 4 rows of 4100 bytes: 13.1 us with 4 of them).
+    constexpr int kWide = VB == 16 ? 1 : 2;
+    auto* kernel = a.topk <= 2   ? route_combine_grad_kernel<DT, VB, 2, 4 * kWide>
+                   : a.topk <= 4 ? route_combine_grad_kernel<DT, VB, 4, 2 * kWide>
+                                 : route_combine_grad_kernel<DT, VB, 8, kWide>;
+    return launch_dependent(kernel, dim3(grid), block, 0, s, a, static_cast<const char*>(dy), static_cast<long long>(lddy),
+                            static_cast<const char*>(ys), static_cast<long long>(ldys), w, static_cast<char*>(dys),
+                            static_cast<long long>(lddys), dw);
 }
 
 template <int DT>
@@ -772,7 +788,7 @@ int spmm_route_combine_grad(const spmm_route_view* r, const void* dy, int64_t ld
     const int vb = al.vector_bytes();
     const RouteArgs a = make_args(r, H, dtype, vb, st);
     // Streamed: whole vectors, a stage's pairs, rows of a piece at least, and enough bytes that filling the ring pays.
-    // (32 MB of 4 KB rows: 19.1 us above, 16.8 us streamed, of 8 KB rows 14.6 and 16.8; 128 MB: 75 and 56, two pairs 140 and 77.)
+    // (32 MB of 4 KB rows: 15.8 us above, 16.8 us streamed, of 8 KB rows 12.7 and 16.8; 128 MB: 66 and 57, two pairs 93 and 77.)
     constexpr int64_t kLeast = INT64_C(64) << 20;
     if (vb == 16 && r->topk <= kMaxPairs && static_cast<int64_t>(H) * e >= 1024 && static_cast<int64_t>(r->tokens) * r->topk * H * e >= kLeast) {
         if (dtype == SPMM_DTYPE_BF16) return combine_grad_stream_launch<SPMM_DTYPE_BF16>(a, dy, lddy * e, ys, ldys * e, w, dys, lddys * e, dw, as_stream(stream), st);

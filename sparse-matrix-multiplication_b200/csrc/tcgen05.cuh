@@ -208,6 +208,16 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 
+// A box from shared memory; what lies past the tensor is not written. Source reads end with bulk_store_read_wait().
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src),
+                 "r"(x), "r"(y), "r"(z)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -253,16 +263,16 @@ inline int encode_2d(CUtensorMap* map, const void* ptr, uint64_t inner, uint64_t
     return r == CUDA_SUCCESS ? SPMM_OK : SPMM_ERR_INVALID_ARG;
 }
 
-// A 3-D tensor of 16-bit elements (strides in bytes of the two outer dimensions).
+// A 3-D tensor of 16- or 32-bit elements (strides in bytes of the two outer dimensions).
 inline int encode_3d(CUtensorMap* map, const void* ptr, const uint64_t (&dims)[3], const uint64_t (&strides)[2],
-                     const uint32_t (&box)[3], CUtensorMapSwizzle swz) {
+                     const uint32_t (&box)[3], CUtensorMapSwizzle swz, bool wide = false) {
     auto enc = tensor_map_encoder();
     if (!enc) return SPMM_ERR_UNSUPPORTED;
     const cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
     const cuuint64_t st[2] = {strides[0], strides[1]};
     const cuuint32_t b[3] = {box[0], box[1], box[2]};
     const cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(ptr), d, st, b, estr,
+    const CUresult r = enc(map, wide ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(ptr), d, st, b, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? SPMM_OK : SPMM_ERR_INVALID_ARG;
