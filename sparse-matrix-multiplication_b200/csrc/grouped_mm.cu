@@ -307,6 +307,31 @@ __device__ __forceinline__ const uint16_t* stage_line(const TcArgs& a, const Til
     return row + col;
 }
 
+// 32 consecutive results of a row, of which `cols` (a multiple of 8) exist, rounded once where the output has 16 bits.
+__device__ __forceinline__ void store_piece(const TcArgs& a, const uint32_t (&v)[32], char* out, int cols, bool sectors) {
+    if (a.out_f32) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = v[8 * c + i];
+            if (8 * c < cols) store_32(out + 32 * c, w, sectors);
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float lo = __uint_as_float(v[16 * c + 2 * i]), hi = __uint_as_float(v[16 * c + 2 * i + 1]);
+                w[i] = a.dtype == SPMM_DTYPE_BF16 ? pack_half2<SPMM_DTYPE_BF16>(lo, hi) : pack_half2<SPMM_DTYPE_F16>(lo, hi);
+            }
+            if (16 * c + 16 <= cols) store_32(out + 32 * c, w, sectors);
+            else if (16 * c < cols) *reinterpret_cast<uint4*>(out + 32 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
 // SINGLES (forward, FP32 out): groups of one row are left to eight warps more.
 template <int FORM, int TN, bool SINGLES, bool ANY>
 __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
@@ -629,29 +654,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
                             if (a.out_f32) *reinterpret_cast<float*>(o) = f;
                             else *reinterpret_cast<uint16_t*>(o) = a.dtype == SPMM_DTYPE_BF16 ? float_to_half_bits<SPMM_DTYPE_BF16>(f) : float_to_half_bits<SPMM_DTYPE_F16>(f);
                         }
-                    } else if (row >= rows) {
-                        // nothing to store
-                    } else if (a.out_f32) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t w[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) w[i] = v[8 * c + i];
-                            if (c0 + 8 * c < cols) store_32(out + (c0 + 8 * c) * 4, w, sectors);
-                        }
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t w[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const float lo = __uint_as_float(v[16 * c + 2 * i]), hi = __uint_as_float(v[16 * c + 2 * i + 1]);
-                                w[i] = a.dtype == SPMM_DTYPE_BF16 ? pack_half2<SPMM_DTYPE_BF16>(lo, hi) : pack_half2<SPMM_DTYPE_F16>(lo, hi);
-                            }
-                            const int col = c0 + 16 * c;
-                            if (col + 16 <= cols) store_32(out + col * 2, w, sectors);
-                            else if (col < cols) *reinterpret_cast<uint4*>(out + col * 2) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                    } else if (row < rows) {
+                        store_piece(a, v, out + c0 * size, cols - c0, sectors);
                     }
                     __syncwarp();
                 }
@@ -703,6 +707,231 @@ int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap
     return launch_dependent(grouped_tc_kernel<FORM, TN, SINGLES, ANY>, dim3(grid), dim3(tc_threads(SINGLES, ANY)), smem, s, ma, small, mb, wide, a);
 }
 
+// ------------------------------------------------------------------ tcgen05, pairs of blocks
+//
+// Forward and dx of long groups: two blocks of a cluster take a 256 x 256 tile with cta_group::2. Each loads its 128 rows of A
+// and half of B's 256 columns, and the MMA reads both halves, so a block fills 32 KB a step for the work that takes a block of
+// its own 48: kPairFigures. Half a row tile more of every group is wasted, hence for long groups only. dw stays on single
+// blocks: the rows past a group's end that it clears would have to be cleared in the other block as well.
+
+constexpr int kPairM = 256, kPairN = 256;
+
+struct PairLayout {
+    static constexpr int kA = 128 * kStepK * 2;
+    static constexpr int kStage = kA + 128 * kStepK * 2;
+    static constexpr int kStages = 6;
+    static constexpr int kBars = kStages * kStage;  // full[] (block 0's count), empty[], acc_full[2], acc_empty[2] (block 0's), drain
+    static constexpr int kTable = kBars + 8 * (2 * kStages + 5) + 16;
+    static constexpr int kFixed = kTable + 1024;
+};
+
+// Tile t: group, first row in it, first column.
+struct PairTile {
+    int g, m0, n0, begin, end;
+};
+
+__device__ __forceinline__ PairTile pair_tile(const TcArgs& a, const int* start, int t) {
+    constexpr int kPairBand = kBand / 2;
+    PairTile r;
+    r.g = tile_group(start, a.groups, t / a.ntiles);
+    int local = t - start[r.g] * a.ntiles;
+    const int band = local / (kPairBand * a.ntiles), high = min(kPairBand, start[r.g + 1] - start[r.g] - band * kPairBand);
+    local -= band * kPairBand * a.ntiles;
+    r.m0 = (band * kPairBand + local % high) * kPairM;
+    r.n0 = local / high * kPairN;
+    const GroupRange range = group_range(a.offsets, r.g, a.rows, nullptr);
+    r.begin = range.begin;
+    r.end = range.end;
+    return r;
+}
+
+template <int FORM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue, 1)
+    grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TcArgs a) {
+    using L = PairLayout;
+    constexpr int kStages = L::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_addr(smem_raw);
+    uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // the same offset in both blocks
+    const uint32_t sbase = smem_addr(base);
+    const uint32_t full0 = sbase + L::kBars, empty0 = full0 + 8 * kStages, acc_full0 = empty0 + 8 * kStages, acc_empty0 = acc_full0 + 16,
+                   drain = acc_empty0 + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kBars + 8 * (2 * kStages + 5));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* start = reinterpret_cast<int*>(base + L::kTable);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = static_cast<int>(cluster_rank()), pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(acc_full0 + 8 * s, 1);
+            mbar_init(acc_empty0 + 8 * s, 2 * kEpilogue);
+        }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_tensormap(&map_a);
+        prefetch_tensormap(&map_b);
+    }
+    if (warp == 1) tmem_alloc_pair(smem_addr(tmem_slot), 2 * kPairN);
+    grid_dependency_wait();
+    allow_dependent_launch();
+    build_tile_table(start, a.offsets, a.groups, a.rows, kPairM, blockIdx.x == 0 ? a.err : nullptr);
+    const int tiles = start[a.groups] * a.ntiles, steps = (a.sum + kStepK - 1) / kStepK;
+    tc_fence_before();
+    cluster_sync();  // the barriers of both blocks are set up, both have their TMEM
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        // ---------------- producer: this block's rows of A and half of B; block 0's barrier counts the bytes of both
+        if (elect_one()) {
+            int it = 0, s = 0;
+            uint32_t phase = 1;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs) {
+                const PairTile r = pair_tile(a, start, t);
+                const int row = r.begin + r.m0 + 128 * rank, col = r.n0 + 128 * rank;
+                for (int ks = 0; ks < steps; ++ks, ++it) {
+                    const uint32_t sa = sbase + s * L::kStage, sb = sa + L::kA, bar = cluster_addr(full0 + 8 * s, 0);
+                    if (!mbar_wait(empty0 + 8 * s, phase, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * L::kStage);
+                    if (++s == kStages) s = 0, phase ^= 1u;
+                    tma_load_2d_pair(sa, &map_a, bar, ks * kStepK, row);
+                    if constexpr (FORM == kForward) {
+                        tma_load_3d_pair(sb, &map_b, bar, ks * kStepK, col, r.g);
+                    } else {
+                        tma_load_3d_pair(sb, &map_b, bar, col, ks * kStepK, r.g);
+                        tma_load_3d_pair(sb + 8192, &map_b, bar, col + 64, ks * kStepK, r.g);
+                    }
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                record_device_error(a.err, SPMM_ERR_TIMEOUT, 41);
+                // Block 0's barrier, which may be what did not move, is the only one that sees this block's copies land: a
+                // while, far longer than a copy takes.
+                const unsigned long long t0 = global_ns();
+                while (global_ns() - t0 < 10ull * 1000 * 1000) {
+                }
+            }
+            // The stages' last MMAs are done, and so the copies into them.
+            for (int i = max(0, it - kStages); ok && i < it; ++i) mbar_wait(empty0 + 8 * (i % kStages), (i / kStages) & 1u, abort_flag);
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer, in block 0
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc = instr_desc_f16(a.dtype, kPairN, false, FORM != kForward, kPairM);
+            constexpr uint64_t kNextB = FORM == kForward ? 2 : 128;
+            int s = 0, n = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair; ok && t < tiles; t += pairs, ++n) {
+                const int buf = n & 1;
+                ok = mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + buf * kPairN;
+                for (int ks = 0; ks < steps; ++ks) {
+                    ok = mbar_wait(full0 + 8 * s, phase, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t sa = sbase + s * L::kStage, sb = sa + L::kA;
+                    const uint64_t da = smem_desc(sa, 16, 1024, kSwizzle128);
+                    const uint64_t db = FORM == kForward ? smem_desc(sb, 16, 1024, kSwizzle128) : smem_desc(sb, 8192, 1024, kSwizzle128);
+                    umma_f16_pair(acc, da, db, idesc, ks > 0 ? 1u : 0u);
+#pragma unroll
+                    for (int j = 1; j < 4; ++j) umma_f16_pair(acc, da + 2 * j, db + j * kNextB, idesc, 1u);  // past the sum: zeros
+                    umma_commit_pair(empty0 + 8 * s);
+                    if (++s == kStages) s = 0, phase ^= 1u;
+                }
+                umma_commit_pair(acc_full0 + 8 * buf);
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                record_device_error(a.err, SPMM_ERR_TIMEOUT, 42);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------- epilogue: this block's 128 rows
+        const int q = warp & 3, part = (warp - 2) >> 2;
+        const int size = a.out_f32 ? 4 : 2;
+        const bool sectors = (reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) % 32 == 0;
+        int n = 0;
+        bool ok = true;
+        for (int t = pair; t < tiles; t += pairs, ++n) {
+            const PairTile r = pair_tile(a, start, t);
+            const int buf = n & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const int first = r.m0 + 128 * rank + q * 32, rows = r.end - r.begin, cols = min(kPairN, a.outs - r.n0);
+            char* out = static_cast<char*>(a.out) + (static_cast<long long>(r.begin + first + lane) * a.ldo + r.n0) * size;
+            for (int c0 = part * 32; first < rows && c0 < cols; c0 += 8 * kEpilogue) {
+                uint32_t v[32];
+                tmem_ld32(tmem + buf * kPairN + c0 + (static_cast<uint32_t>(q * 32) << 16), v);
+                if (first + lane < rows) store_piece(a, v, out + c0 * size, cols - c0, sectors);
+                __syncwarp();
+            }
+            __syncwarp();
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty0 + 8 * buf, 0));
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_device_error(a.err, SPMM_ERR_TIMEOUT, 43);
+        }
+    }
+
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync();  // neither block's shared memory or TMEM goes while the other may use it
+    if (warp == 1) {
+        tc_fence_after();
+        if (rank == 0 && *abort_flag) {
+            // MMAs still in flight end before their accumulators are given back.
+            if (elect_one()) {
+                umma_commit_pair(drain);
+                const unsigned long long t0 = global_ns();
+                while (!mbar_try_wait(drain, 0) && global_ns() - t0 < kWaitNs) {
+                }
+            }
+            __syncwarp();
+        }
+        tmem_dealloc_pair(tmem, 2 * kPairN);
+    }
+    cluster_sync();
+}
+
+template <int FORM>
+int pair_launch(const GroupedArgs& g, TcArgs a, cudaStream_t s, DeviceState* st) {
+    static std::atomic<unsigned long long> attr_set{0};
+    const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
+    if (!bit || !(attr_set.load(std::memory_order_acquire) & bit)) {
+        SPMM_CUDA_TRY(cudaFuncSetAttribute(grouped_pair_kernel<FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           PairLayout::kFixed + 4 * (SPMM_MAX_GROUPS + 1)));
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    a.ntiles = (a.outs + kPairN - 1) / kPairN;
+    CUtensorMap ma, mb;
+    const uint64_t rows = g.rows, N = g.N, K = g.K;
+    SPMM_TRY(encode_2d(&ma, g.a, FORM == kForward ? K : N, rows, g.lda * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B));
+    SPMM_TRY(encode_3d(&mb, g.b, {K, N, static_cast<uint64_t>(g.groups)}, {K * 2, N * K * 2}, {64, FORM == kForward ? 128u : 64u, 1},
+                       CU_TENSOR_MAP_SWIZZLE_128B));
+    const size_t smem = PairLayout::kFixed + 4 * (static_cast<size_t>(a.groups) + 1);
+    return launch_dependent(grouped_pair_kernel<FORM>, dim3(static_cast<unsigned>(st->sm_count / 2 * 2)), dim3(64 + 32 * kEpilogue), smem, s, ma, mb, a);
+}
+
 bool fits16(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
 
 // Whether TMA and stores of 16 bytes can address the operands.
@@ -737,6 +966,12 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     t.err = a.err;
     // Row tiles: exact for dw, else as many as the groups can have (how many they do have is on the device).
     const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * t.mtiles : a.rows / kTileM + std::min(a.groups, a.rows);
+    if constexpr (FORM != kDw) {
+        // Pairs of blocks where the groups are 2048 rows long on average (a row tile of 256 then wastes 6 % of the rows at most
+        // where one of 128 wastes 3) and every pair has four tiles.
+        const int64_t pair_tiles = static_cast<int64_t>(a.rows / kPairM) * ((t.outs + kPairN - 1) / kPairN);
+        if (!any && t.outs >= kPairN && a.rows / a.groups >= 2048 && pair_tiles >= 2 * st->sm_count) return pair_launch<FORM>(a, t, s, st);
+    }
     // The widest tile that still gives every SM one: a wide tile reads A less often, narrow ones spread few rows.
     int tn = 256;
     if (any) tn = 128;

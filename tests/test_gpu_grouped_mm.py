@@ -94,6 +94,27 @@ def test_strides_and_rows_in_no_group(cuda, out):
     check_all([40, 0, 200, 9], 192, 96, BF16, out=out, pad=24, shift=8, first=11, tail=150)
 
 
+@pytest.mark.parametrize("sizes,first,tail,dtype,out", [
+    ([4000, 130], 0, 0, BF16, BF16), ([1, 4199], 3, 40, F16, F32), ([2304, 2305], 0, 5, F16, F16), ([4096], 0, 0, BF16, F32)])
+@pytest.mark.parametrize("wide,narrow", [(5120, 72), (5000, 200)])
+def test_long_groups(cuda, sizes, first, tail, dtype, out, wide, narrow):
+    """Groups long enough for a pair of blocks a tile, with ragged ends, columns that end inside a tile, and sums that end
+    inside a step: wide outputs of the forward product, then of dx."""
+    off = offsets(sizes, first)
+    n = int(off[-1])
+    o = off.cuda()
+    for forward in (True, False):
+        rows_in = values((n + tail, narrow), dtype, 1)
+        rows_in[:first], rows_in[n:] = float("nan"), float("inf")
+        w = values((len(sizes), wide, narrow) if forward else (len(sizes), narrow, wide), dtype, 2)
+        got = torch.full((n + tail, wide), 7.0, dtype=out, device="cuda")
+        (S.grouped_mm if forward else S.grouped_mm_dx)(o, rows_in, w, got, stream=stream())
+        clean()
+        want, mag = (R.grouped if forward else R.grouped_dx)(off, rows_in, w)
+        R.close(got[first:n], want[first:n], mag[first:n], narrow, out, "forward" if forward else "dx")
+        assert (got[:first] == 7).all() and (got[n:] == 7).all()
+
+
 def test_no_rows_and_empty_sums(cuda):
     check_all([0, 0], 64, 64, BF16, tail=5)
     x, w = torch.zeros((4, 0), dtype=BF16, device="cuda"), torch.zeros((1, 16, 0), dtype=BF16, device="cuda")
