@@ -332,6 +332,46 @@ __device__ __forceinline__ void store_piece(const TcArgs& a, const uint32_t (&v)
     }
 }
 
+// dw's tiles end where the operand does, which TMA knows: a warp's 32 rows in boxes of 128 bytes a row through shared memory,
+// for which nothing waits. (Each lane its row's sectors, as above, is one line a lane: 64 groups of 8 rows, 1024 x 1024 in
+// FP32, took 95 us where this takes 58.)
+__device__ __forceinline__ void store_boxes(const TcArgs& a, uint32_t acc, uint8_t* box, const CUtensorMap* map, bool zero, int part, int cols, int n0,
+                                            int row, int g) {
+    const int lane = threadIdx.x & 31, per = a.out_f32 ? 32 : 64;  // columns of a box
+    for (int c0 = part * per; c0 < cols; c0 += 2 * per) {
+        if (lane == 0) bulk_store_read_wait();
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (h && a.out_f32) break;
+            uint32_t v[32];
+            tmem_ld32(acc + c0 + 32 * h, v);
+            if (zero) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0u;
+            }
+            if (a.out_f32) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) *swizzled_piece(box, lane, c) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float lo = __uint_as_float(v[8 * c + 2 * i]), hi = __uint_as_float(v[8 * c + 2 * i + 1]);
+                        w[i] = a.dtype == SPMM_DTYPE_BF16 ? pack_half2<SPMM_DTYPE_BF16>(lo, hi) : pack_half2<SPMM_DTYPE_F16>(lo, hi);
+                    }
+                    *swizzled_piece(box, lane, 4 * h + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tma_store_3d(map, smem_addr(box), n0 + c0, row, g);
+    }
+}
+
 // SINGLES (forward, FP32 out): groups of one row are left to eight warps more.
 template <int FORM, int TN, bool SINGLES, bool ANY>
 __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
@@ -595,42 +635,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
             char* out = static_cast<char*>(a.out) + (at * a.ldo + r.n0 + r.split * a.split_stride) * size;
             const int cols = r.cols;
             if (FORM == kDw && !ANY && r.m0 + q * 32 < rows) {
-                // dw's tiles end where the operand does, which TMA knows: whole boxes through shared memory, nothing waits for
-                // them. (Each lane its row's sectors, as below, is one line a lane: 2.2 us for a tile of 128 x 256 in FP32.)
-                uint8_t* box = base + L::kOut + (warp - 2) * kStoreBox;
-                const int per = 128 / size;  // columns of a box
-                for (int c0 = part * per; c0 < cols; c0 += 2 * per) {
-                    if (lane == 0) bulk_store_read_wait();
-                    __syncwarp();
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h && a.out_f32) break;
-                        uint32_t v[32];
-                        tmem_ld32(acc + c0 + 32 * h, v);
-                        if (r.steps == 0) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = 0u;
-                        }
-                        if (a.out_f32) {
-#pragma unroll
-                            for (int c = 0; c < 8; ++c) *swizzled_piece(box, lane, c) = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const float lo = __uint_as_float(v[8 * c + 2 * i]), hi = __uint_as_float(v[8 * c + 2 * i + 1]);
-                                    w[i] = a.dtype == SPMM_DTYPE_BF16 ? pack_half2<SPMM_DTYPE_BF16>(lo, hi) : pack_half2<SPMM_DTYPE_F16>(lo, hi);
-                                }
-                                *swizzled_piece(box, lane, 4 * h + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                        }
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) tma_store_3d(&map_b_wide, smem_addr(box), r.n0 + c0, r.m0 + q * 32, r.g);
-                }
+                store_boxes(a, acc, base + L::kOut + (warp - 2) * kStoreBox, &map_b_wide, r.steps == 0, part, cols, r.n0, r.m0 + q * 32, r.g);
             } else if (r.m0 + q * 32 < rows) {
                 for (int c0 = part * 32; c0 < cols; c0 += 8 * kEpilogue) {
                     uint32_t v[32];
@@ -709,54 +714,84 @@ int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap
 
 // ------------------------------------------------------------------ tcgen05, pairs of blocks
 //
-// Forward and dx of long groups: two blocks of a cluster take a 256 x 256 tile with cta_group::2. Each loads its 128 rows of A
-// and half of B's 256 columns, and the MMA reads both halves, so a block fills 32 KB a step for the work that takes a block of
-// its own 48: kPairFigures. Half a row tile more of every group is wasted, hence for long groups only. dw stays on single
-// blocks: the rows past a group's end that it clears would have to be cleared in the other block as well.
+// Long groups: two blocks of a cluster take a 256 x 256 tile with cta_group::2. Each loads its 128 rows of A and half of B's
+// 256 columns, and the MMA reads both halves, so a block fills 32 KB a step for the work that takes a block of its own 48. That
+// fill bounds the single blocks' kernel (70 bytes a clock and SM from L2 at 80 % of the tensor rate) and costs it clock under
+// the power cap: 32768 rows x 4096 x 4096 over 8 groups, 921 -> 756 us back to back. In dw each block clears its own rows past
+// a group's end: such a last step completes on a barrier of the block itself, and both blocks tell block 0 when they are done.
 
 constexpr int kPairM = 256, kPairN = 256;
 
+template <int FORM>
 struct PairLayout {
     static constexpr int kA = 128 * kStepK * 2;
     static constexpr int kStage = kA + 128 * kStepK * 2;
     static constexpr int kStages = 6;
-    static constexpr int kBars = kStages * kStage;  // full[] (block 0's count), empty[], acc_full[2], acc_empty[2] (block 0's), drain
-    static constexpr int kTable = kBars + 8 * (2 * kStages + 5) + 16;
+    static constexpr int kOut = kStages * kStage;
+    // full[] (block 0's count), empty[], acc_full[2], acc_empty[2] (block 0's), drain, tail_full, tail_empty,
+    // tail_ready (block 0's)
+    static constexpr int kBars = kOut + (FORM == kDw ? kEpilogue * kStoreBox : 0);
+    static constexpr int kSlot = kBars + 8 * (2 * kStages + 8);
+    static constexpr int kTable = kSlot + 16;
     static constexpr int kFixed = kTable + 1024;
 };
 
-// Tile t: group, first row in it, first column.
+// Tile t: group, first row and column of D, the group's rows, steps of its sum.
 struct PairTile {
-    int g, m0, n0, begin, end;
+    int g, m0, n0, begin, end, steps;
 };
 
+template <int FORM>
 __device__ __forceinline__ PairTile pair_tile(const TcArgs& a, const int* start, int t) {
     constexpr int kPairBand = kBand / 2;
     PairTile r;
-    r.g = tile_group(start, a.groups, t / a.ntiles);
-    int local = t - start[r.g] * a.ntiles;
-    const int band = local / (kPairBand * a.ntiles), high = min(kPairBand, start[r.g + 1] - start[r.g] - band * kPairBand);
+    int local, mtiles;
+    if constexpr (FORM == kDw) {
+        const int per = a.mtiles * a.ntiles;
+        r.g = t / per;
+        local = t - r.g * per;
+        mtiles = a.mtiles;
+    } else {
+        r.g = tile_group(start, a.groups, t / a.ntiles);
+        local = t - start[r.g] * a.ntiles;
+        mtiles = start[r.g + 1] - start[r.g];
+    }
+    const int band = local / (kPairBand * a.ntiles), high = min(kPairBand, mtiles - band * kPairBand);
     local -= band * kPairBand * a.ntiles;
     r.m0 = (band * kPairBand + local % high) * kPairM;
     r.n0 = local / high * kPairN;
     const GroupRange range = group_range(a.offsets, r.g, a.rows, nullptr);
     r.begin = range.begin;
     r.end = range.end;
+    r.steps = ((FORM == kDw ? r.end - r.begin : a.sum) + kStepK - 1) / kStepK;
     return r;
 }
 
 template <int FORM>
+__device__ __forceinline__ void pair_step(uint32_t acc, uint32_t stage, uint32_t idesc, int slices, bool add) {
+    constexpr uint64_t kNextA = FORM == kDw ? 128 : 2, kNextB = FORM == kForward ? 2 : 128;
+    const uint64_t da = FORM == kDw ? smem_desc(stage, 8192, 1024, kSwizzle128) : smem_desc(stage, 16, 1024, kSwizzle128);
+    const uint32_t sb = stage + PairLayout<FORM>::kA;
+    const uint64_t db = FORM == kForward ? smem_desc(sb, 16, 1024, kSwizzle128) : smem_desc(sb, 8192, 1024, kSwizzle128);
+    umma_f16_pair(acc, da, db, idesc, add ? 1u : 0u);
+#pragma unroll
+    for (int j = 1; j < 4; ++j)
+        if (j < slices) umma_f16_pair(acc, da + j * kNextA, db + j * kNextB, idesc, 1u);
+}
+
+template <int FORM>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue, 1)
-    grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, TcArgs a) {
-    using L = PairLayout;
+    grouped_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                        const __grid_constant__ CUtensorMap map_out /* dw */, TcArgs a) {
+    using L = PairLayout<FORM>;
     constexpr int kStages = L::kStages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     uint8_t* base = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // the same offset in both blocks
     const uint32_t sbase = smem_addr(base);
     const uint32_t full0 = sbase + L::kBars, empty0 = full0 + 8 * kStages, acc_full0 = empty0 + 8 * kStages, acc_empty0 = acc_full0 + 16,
-                   drain = acc_empty0 + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kBars + 8 * (2 * kStages + 5));
+                   drain = acc_empty0 + 16, tail_full = drain + 8, tail_empty = tail_full + 8, tail_ready = tail_empty + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kSlot);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* start = reinterpret_cast<int*>(base + L::kTable);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -773,6 +808,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
             mbar_init(acc_empty0 + 8 * s, 2 * kEpilogue);
         }
         mbar_init(drain, 1);
+        mbar_init(tail_full, 1);
+        mbar_init(tail_empty, 1);
+        mbar_init(tail_ready, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_tensormap(&map_a);
         prefetch_tensormap(&map_b);
@@ -780,8 +818,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
     if (warp == 1) tmem_alloc_pair(smem_addr(tmem_slot), 2 * kPairN);
     grid_dependency_wait();
     allow_dependent_launch();
-    build_tile_table(start, a.offsets, a.groups, a.rows, kPairM, blockIdx.x == 0 ? a.err : nullptr);
-    const int tiles = start[a.groups] * a.ntiles, steps = (a.sum + kStepK - 1) / kStepK;
+    int tiles;
+    if constexpr (FORM == kDw) {
+        if (blockIdx.x == 0)
+            for (int g = threadIdx.x; g < a.groups; g += blockDim.x) group_range(a.offsets, g, a.rows, a.err);  // records bad ones
+        tiles = a.groups * a.mtiles * a.ntiles;
+    } else {
+        build_tile_table(start, a.offsets, a.groups, a.rows, kPairM, blockIdx.x == 0 ? a.err : nullptr);
+        tiles = start[a.groups] * a.ntiles;
+    }
     tc_fence_before();
     cluster_sync();  // the barriers of both blocks are set up, both have their TMEM
     tc_fence_after();
@@ -790,21 +835,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
     if (warp == 0) {
         // ---------------- producer: this block's rows of A and half of B; block 0's barrier counts the bytes of both
         if (elect_one()) {
-            int it = 0, s = 0;
+            int it = 0, s = 0, tails = 0;
             uint32_t phase = 1;
             bool ok = true;
             for (int t = pair; ok && t < tiles; t += pairs) {
-                const PairTile r = pair_tile(a, start, t);
-                const int row = r.begin + r.m0 + 128 * rank, col = r.n0 + 128 * rank;
-                for (int ks = 0; ks < steps; ++ks, ++it) {
-                    const uint32_t sa = sbase + s * L::kStage, sb = sa + L::kA, bar = cluster_addr(full0 + 8 * s, 0);
-                    if (!mbar_wait(empty0 + 8 * s, phase, abort_flag)) {
-                        ok = false;
-                        break;
+                const PairTile r = pair_tile<FORM>(a, start, t);
+                const int m = r.m0 + 128 * rank, col = r.n0 + 128 * rank;
+                for (int ks = 0; ks < r.steps; ++ks, ++it) {
+                    const bool tail = FORM == kDw && ks == r.steps - 1 && (r.end - r.begin) % 16 != 0;
+                    const uint32_t sa = sbase + s * L::kStage, sb = sa + L::kA;
+                    const uint32_t bar = tail ? cluster_addr(tail_full, rank) : cluster_addr(full0 + 8 * s, 0);
+                    ok = mbar_wait(empty0 + 8 * s, phase, abort_flag);
+                    // One step that completes on tail_full at a time: its MMAs are done before the next begins.
+                    if (tail && tails > 0) ok = ok && mbar_wait(tail_empty, (tails - 1) & 1u, abort_flag);
+                    if (!ok) break;
+                    if (tail) {
+                        mbar_arrive_expect_tx(tail_full, L::kStage);
+                        ++tails;
                     }
-                    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, 2 * L::kStage);
+                    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, tail ? 0 : 2 * L::kStage);
                     if (++s == kStages) s = 0, phase ^= 1u;
-                    tma_load_2d_pair(sa, &map_a, bar, ks * kStepK, row);
+                    if constexpr (FORM == kDw) {
+                        for (int j = 0; j < 2; ++j) {
+                            tma_load_2d_pair(sa + 8192 * j, &map_a, bar, m + 64 * j, r.begin + ks * kStepK);
+                            tma_load_2d_pair(sb + 8192 * j, &map_b, bar, col + 64 * j, r.begin + ks * kStepK);
+                        }
+                        continue;
+                    }
+                    tma_load_2d_pair(sa, &map_a, bar, ks * kStepK, r.begin + m);
                     if constexpr (FORM == kForward) {
                         tma_load_3d_pair(sb, &map_b, bar, ks * kStepK, col, r.g);
                     } else {
@@ -824,42 +882,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
             }
             // The stages' last MMAs are done, and so the copies into them.
             for (int i = max(0, it - kStages); ok && i < it; ++i) mbar_wait(empty0 + 8 * (i % kStages), (i / kStages) & 1u, abort_flag);
+            if (ok && tails > 0) mbar_wait(tail_empty, (tails - 1) & 1u, abort_flag);
         }
     } else if (warp == 1) {
-        // ---------------- MMA issuer, in block 0
-        if (rank == 0 && elect_one()) {
-            const uint32_t idesc = instr_desc_f16(a.dtype, kPairN, false, FORM != kForward, kPairM);
-            constexpr uint64_t kNextB = FORM == kForward ? 2 : 128;
-            int s = 0, n = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int t = pair; ok && t < tiles; t += pairs, ++n) {
-                const int buf = n & 1;
+        // ---------------- MMA issuer, one lane in block 0; in dw the warp of either block clears rows past a group's end
+        const uint32_t idesc = instr_desc_f16(a.dtype, kPairN, FORM == kDw, FORM != kForward, kPairM);
+        int it = 0, n = 0, tails = 0;
+        bool ok = true;
+        for (int t = pair; ok && t < tiles; t += pairs, ++n) {
+            const PairTile r = pair_tile<FORM>(a, start, t);
+            const int buf = n & 1, left = (r.end - r.begin) - (r.steps - 1) * kStepK;  // dw: rows of the last step
+            const int clear = FORM == kDw && left % 16 != 0;  // 0 of an empty group too
+            const uint32_t acc = tmem + buf * kPairN;
+            if (rank == 0 && elect_one()) {
                 ok = mbar_wait(acc_empty0 + 8 * buf, ((n >> 1) & 1u) ^ 1u, abort_flag);
-                if (!ok) break;
                 tc_fence_after();
-                const uint32_t acc = tmem + buf * kPairN;
-                for (int ks = 0; ks < steps; ++ks) {
+                int s = it % kStages;
+                uint32_t phase = (it / kStages) & 1u;
+                for (int ks = 0; ok && ks < r.steps - clear; ++ks) {
                     ok = mbar_wait(full0 + 8 * s, phase, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = sbase + s * L::kStage, sb = sa + L::kA;
-                    const uint64_t da = smem_desc(sa, 16, 1024, kSwizzle128);
-                    const uint64_t db = FORM == kForward ? smem_desc(sb, 16, 1024, kSwizzle128) : smem_desc(sb, 8192, 1024, kSwizzle128);
-                    umma_f16_pair(acc, da, db, idesc, ks > 0 ? 1u : 0u);
-#pragma unroll
-                    for (int j = 1; j < 4; ++j) umma_f16_pair(acc, da + 2 * j, db + j * kNextB, idesc, 1u);  // past the sum: zeros
+                    // Forward, dx: past the sum there are zeros; dw: whole slices of 16 rows.
+                    pair_step<FORM>(acc, sbase + s * L::kStage, idesc, FORM == kDw && ks == r.steps - 1 ? left / 16 : 4, ks > 0);
                     umma_commit_pair(empty0 + 8 * s);
                     if (++s == kStages) s = 0, phase ^= 1u;
                 }
-                umma_commit_pair(acc_full0 + 8 * buf);
             }
-            if (!ok) {
-                *abort_flag = 1;
-                record_device_error(a.err, SPMM_ERR_TIMEOUT, 42);
+            ok = __all_sync(0xffffffffu, ok);
+            it += r.steps;
+            if (FORM == kDw && clear && ok) {
+                const int s = (it - 1) % kStages, slices = (left + 15) / 16;
+                ok = __all_sync(0xffffffffu, mbar_wait(tail_full, tails & 1u, abort_flag));
+                if (ok) {
+                    const int pieces = (slices * 16 - left) * 8;  // 16-byte pieces of a box's rows to clear
+                    for (int b = 0; b < 4; ++b) {
+                        uint4* rows = reinterpret_cast<uint4*>(base + s * L::kStage + b * 8192 + left * 128);
+                        for (int i = lane; i < pieces; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(cluster_addr(tail_ready, 0));
+                    if (rank == 0 && elect_one()) {
+                        ok = mbar_wait_cluster(tail_ready, tails & 1u, abort_flag) && mbar_wait(full0 + 8 * s, ((it - 1) / kStages) & 1u, abort_flag);
+                        if (ok) {
+                            tc_fence_after();
+                            pair_step<FORM>(acc, sbase + s * L::kStage, idesc, slices, r.steps > 1);
+                            umma_commit_pair(tail_empty);
+                            umma_commit_pair(empty0 + 8 * s);
+                        }
+                    }
+                    ok = __all_sync(0xffffffffu, ok);
+                }
+                ++tails;
             }
+            if (rank == 0 && ok && elect_one()) umma_commit_pair(acc_full0 + 8 * buf);
+            __syncwarp();
         }
-        __syncwarp();
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            record_device_error(a.err, SPMM_ERR_TIMEOUT, 42);
+        }
     } else {
         // ---------------- epilogue: this block's 128 rows
         const int q = warp & 3, part = (warp - 2) >> 2;
@@ -868,14 +951,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
         int n = 0;
         bool ok = true;
         for (int t = pair; t < tiles; t += pairs, ++n) {
-            const PairTile r = pair_tile(a, start, t);
+            const PairTile r = pair_tile<FORM>(a, start, t);
             const int buf = n & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag))) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            const int first = r.m0 + 128 * rank + q * 32, rows = r.end - r.begin, cols = min(kPairN, a.outs - r.n0);
+            const int first = r.m0 + 128 * rank + q * 32, rows = FORM == kDw ? a.ms : r.end - r.begin, cols = min(kPairN, a.outs - r.n0);
+            if constexpr (FORM == kDw) {
+                if (first < rows)
+                    store_boxes(a, tmem + buf * kPairN + (static_cast<uint32_t>(q * 32) << 16), base + L::kOut + (warp - 2) * kStoreBox, &map_out, r.steps == 0,
+                                part, cols, r.n0, first, r.g);
+                __syncwarp();
+                tc_fence_before();
+                if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty0 + 8 * buf, 0));
+                continue;
+            }
             char* out = static_cast<char*>(a.out) + (static_cast<long long>(r.begin + first + lane) * a.ldo + r.n0) * size;
             for (int c0 = part * 32; first < rows && c0 < cols; c0 += 8 * kEpilogue) {
                 uint32_t v[32];
@@ -887,6 +979,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
             tc_fence_before();
             if (lane == 0) mbar_arrive_cluster(cluster_addr(acc_empty0 + 8 * buf, 0));
         }
+        if (FORM == kDw && lane == 0) bulk_store_wait();
         if (!ok && lane == 0) {
             *abort_flag = 1;
             record_device_error(a.err, SPMM_ERR_TIMEOUT, 43);
@@ -919,17 +1012,22 @@ int pair_launch(const GroupedArgs& g, TcArgs a, cudaStream_t s, DeviceState* st)
     const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
     if (!bit || !(attr_set.load(std::memory_order_acquire) & bit)) {
         SPMM_CUDA_TRY(cudaFuncSetAttribute(grouped_pair_kernel<FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           PairLayout::kFixed + 4 * (SPMM_MAX_GROUPS + 1)));
+                                           PairLayout<FORM>::kFixed + (FORM == kDw ? 0 : 4 * (SPMM_MAX_GROUPS + 1))));
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     a.ntiles = (a.outs + kPairN - 1) / kPairN;
-    CUtensorMap ma, mb;
-    const uint64_t rows = g.rows, N = g.N, K = g.K;
-    SPMM_TRY(encode_2d(&ma, g.a, FORM == kForward ? K : N, rows, g.lda * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B));
-    SPMM_TRY(encode_3d(&mb, g.b, {K, N, static_cast<uint64_t>(g.groups)}, {K * 2, N * K * 2}, {64, FORM == kForward ? 128u : 64u, 1},
-                       CU_TENSOR_MAP_SWIZZLE_128B));
-    const size_t smem = PairLayout::kFixed + 4 * (static_cast<size_t>(a.groups) + 1);
-    return launch_dependent(grouped_pair_kernel<FORM>, dim3(static_cast<unsigned>(st->sm_count / 2 * 2)), dim3(64 + 32 * kEpilogue), smem, s, ma, mb, a);
+    a.mtiles = (g.N + kPairM - 1) / kPairM;
+    CUtensorMap ma, mb, out{};
+    const uint64_t rows = g.rows, N = g.N, K = g.K, groups = g.groups, size = g.out_f32 ? 4 : 2;
+    SPMM_TRY(encode_2d(&ma, g.a, FORM == kForward ? K : N, rows, g.lda * 2, 64, FORM == kDw ? 64 : 128, CU_TENSOR_MAP_SWIZZLE_128B));
+    if constexpr (FORM == kDw) {
+        SPMM_TRY(encode_2d(&mb, g.b, K, rows, g.ldb * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+        SPMM_TRY(encode_3d(&out, g.out, {K, N, groups}, {K * size, N * K * size}, {static_cast<uint32_t>(128 / size), 32, 1}, CU_TENSOR_MAP_SWIZZLE_128B, g.out_f32));
+    } else {
+        SPMM_TRY(encode_3d(&mb, g.b, {K, N, groups}, {K * 2, N * K * 2}, {64, FORM == kForward ? 128u : 64u, 1}, CU_TENSOR_MAP_SWIZZLE_128B));
+    }
+    const size_t smem = PairLayout<FORM>::kFixed + (FORM == kDw ? 0 : 4 * (static_cast<size_t>(a.groups) + 1));
+    return launch_dependent(grouped_pair_kernel<FORM>, dim3(static_cast<unsigned>(st->sm_count / 2 * 2)), dim3(64 + 32 * kEpilogue), smem, s, ma, mb, out, a);
 }
 
 bool fits16(const void* p, int64_t ld, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0; }
@@ -966,12 +1064,13 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     t.err = a.err;
     // Row tiles: exact for dw, else as many as the groups can have (how many they do have is on the device).
     const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * t.mtiles : a.rows / kTileM + std::min(a.groups, a.rows);
-    if constexpr (FORM != kDw) {
-        // Pairs of blocks where the groups are 2048 rows long on average (a row tile of 256 then wastes 6 % of the rows at most
-        // where one of 128 wastes 3) and every pair has four tiles.
-        const int64_t pair_tiles = static_cast<int64_t>(a.rows / kPairM) * ((t.outs + kPairN - 1) / kPairN);
-        if (!any && t.outs >= kPairN && a.rows / a.groups >= 2048 && pair_tiles >= 2 * st->sm_count) return pair_launch<FORM>(a, t, s, st);
-    }
+    // Pairs of blocks where every pair has about four tiles (with three their coarser rounds cost what they gain: 0.92 to 1.13
+    // of the single blocks' rate) and the groups are long: a row tile of 256 wastes 128 rows of a group on average, in dw a tile
+    // has that much more to store. Measured at 16384 rows, 2048 x 2048, pairs against single blocks: 192 rows a group 1.07
+    // (forward), 1.05 (dx), 0.76 (dw); 384: 1.10, 1.13, 1.06; 1024: 1.20, 1.16, 1.12.
+    const int64_t pair_tiles = (FORM == kDw ? static_cast<int64_t>(a.groups) * ((a.N + kPairM - 1) / kPairM) : a.rows / kPairM) * ((t.outs + kPairN - 1) / kPairN);
+    if (!any && t.outs >= kPairN && (FORM != kDw || a.N >= kPairM) && a.rows / a.groups >= (FORM == kDw ? 384 : 192) && pair_tiles >= 2 * st->sm_count)
+        return pair_launch<FORM>(a, t, s, st);
     // The widest tile that still gives every SM one: a wide tile reads A less often, narrow ones spread few rows.
     int tn = 256;
     if (any) tn = 128;

@@ -95,7 +95,8 @@ def test_strides_and_rows_in_no_group(cuda, out):
 
 
 @pytest.mark.parametrize("sizes,first,tail,dtype,out", [
-    ([4000, 130], 0, 0, BF16, BF16), ([1, 4199], 3, 40, F16, F32), ([2304, 2305], 0, 5, F16, F16), ([4096], 0, 0, BF16, F32)])
+    ([4000, 130], 0, 0, BF16, BF16), ([1, 4199], 3, 40, F16, F32), ([2304, 2305], 0, 5, F16, F16), ([4096], 0, 0, BF16, F32),
+    ([257, 100, 0, 511, 256, 255, 400, 2, 1900, 300], 0, 1, BF16, BF16)])
 @pytest.mark.parametrize("wide,narrow", [(5120, 72), (5000, 200)])
 def test_long_groups(cuda, sizes, first, tail, dtype, out, wide, narrow):
     """Groups long enough for a pair of blocks a tile, with ragged ends, columns that end inside a tile, and sums that end
@@ -113,6 +114,56 @@ def test_long_groups(cuda, sizes, first, tail, dtype, out, wide, narrow):
         want, mag = (R.grouped if forward else R.grouped_dx)(off, rows_in, w)
         R.close(got[first:n], want[first:n], mag[first:n], narrow, out, "forward" if forward else "dx")
         assert (got[:first] == 7).all() and (got[n:] == 7).all()
+
+
+@pytest.mark.parametrize("sizes,first,tail,dtype,out", [
+    ([4000, 137], 0, 0, BF16, BF16), ([1, 4198], 3, 40, F16, F32), ([2304, 2320], 0, 5, F16, F16), ([0, 6200, 0], 1, 1, BF16, F32),
+    ([2049, 2063, 2050, 2034, 2048], 0, 0, BF16, F32)])
+@pytest.mark.parametrize("N,K", [(4608, 4352), (264, 38400), (4360, 4424)])
+def test_long_groups_dw(cuda, sizes, first, tail, dtype, out, N, K):
+    """The weights' gradient of long groups (pairs of blocks a tile): sums that end anywhere in a step, empty groups, edges.
+    Checked on some rows and columns of every group and all of its corners."""
+    off = offsets(sizes, first)
+    n = int(off[-1])
+    dy, x = values((n + tail, N), dtype, 1), values((n + tail, K), dtype, 2)
+    for t in (dy, x):
+        t[:first], t[n:] = float("nan"), float("inf")
+    dw = torch.full((len(sizes), N, K), float("nan"), dtype=out, device="cuda")
+    S.grouped_mm_dw(off.cuda(), dy, x, dw, stream=stream())
+    clean()
+    assert not torch.isnan(dw).any()
+    g = torch.Generator().manual_seed(7)
+    ns = torch.cat([torch.randint(0, N, (40,), generator=g), torch.tensor([0, 127, 128, 255, 256, N - 1])]).cuda()
+    ks = torch.cat([torch.randint(0, K, (60,), generator=g), torch.tensor([0, 127, 128, 255, 256, K - 1])]).cuda()
+    want, mag = R.grouped_dw(off, dy[:, ns], x[:, ks])
+    R.close(dw[:, ns][:, :, ks], want, mag, max(sizes), out, "dw")
+
+
+def test_long_groups_in_a_graph_between_other_kernels(cuda):
+    """The clusters' launches captured, behind and before kernels of single blocks, give the eager bits again and again."""
+    off = offsets([2500, 0, 3647]).cuda()
+    x, dy, w = values((6147, 2048), BF16, 1), values((6147, 2304), BF16, 2), values((3, 2304, 2048), BF16, 3)
+
+    def run():
+        y, dx, dw = torch.zeros_like(dy), torch.zeros_like(x), torch.zeros(w.shape, device="cuda")
+        small = torch.zeros((40, 2304), dtype=BF16, device="cuda")
+        s = stream()
+        S.grouped_mm(off, x, w, y, stream=s)
+        S.grouped_mm_dx(off, y, w, dx, stream=s)
+        S.grouped_mm_dw(off, y, x, dw, stream=s)
+        S.grouped_mm(few, x[:40], w, small, stream=s)
+        S.grouped_mm_dw(off, dy, dx, dw, stream=s)
+        return y, dx, dw, small
+
+    few = offsets([40, 0, 0]).cuda()
+    eager = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+    for _ in range(3):
+        graph.replay()
+    clean()
+    assert all(torch.equal(a, b) for a, b in zip(eager, captured))
 
 
 def test_no_rows_and_empty_sums(cuda):
