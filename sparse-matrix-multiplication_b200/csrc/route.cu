@@ -31,6 +31,7 @@ constexpr int kMaxSortThreads = 1024;
 constexpr int kOneBlock = 4096;       // pairs that one block takes alone: a second launch costs more than they do
 constexpr int kPairsPerBlock = 2048;
 constexpr int kMaxSortBlocks = 128;   // blocks grow beyond kPairsPerBlock instead
+constexpr int kMaxSortSmem = 4 * (10 * SPMM_MAX_GROUPS + 33);  // 8 histograms, totals and prefixes of the most groups: 160 KiB
 
 struct SortShape {
     int warps;      // warps with a histogram of their own
@@ -717,8 +718,16 @@ int spmm_route_build(const int32_t* ids, int32_t tokens, int32_t topk, int32_t g
     const cudaStream_t s = as_stream(stream);
     const int pairs = tokens * topk;
     const SortShape h = sort_shape(pairs, groups);
-    if (h.smem > 48 * 1024)
-        SPMM_CUDA_TRY(cudaFuncSetAttribute(route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(h.smem)));
+    if (h.smem > 48 * 1024) {
+        // Once a device, for the largest of all calls: each call its own size would take it from a larger call's launch under
+        // way in another thread.
+        static std::atomic<unsigned long long> attr_set{0};
+        const unsigned long long bit = st->device < 64 ? 1ull << st->device : 0ull;
+        if (!bit || !(attr_set.load(std::memory_order_acquire) & bit)) {
+            SPMM_CUDA_TRY(cudaFuncSetAttribute(route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSortSmem));
+            attr_set.fetch_or(bit, std::memory_order_acq_rel);
+        }
+    }
     int* counts = static_cast<int*>(ws);
     // More threads than the warps with histograms only where there are groups for them.
     const int threads = std::max(h.warps * 32, std::min(kMaxSortThreads, (groups + 31) / 32 * 32));

@@ -1,6 +1,8 @@
 """Tokens routed to groups and back on the GPU, against plain 64-bit forms."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -293,3 +295,31 @@ def test_binding_refuses_other_shapes_types_and_strides(cuda):
         S.route_combine(pos, xs, x, torch.zeros((4, 1), device="cuda"))
     with pytest.raises(ValueError):
         S.route_combine_grad(pos, x, xs, None, None, None)
+
+
+def test_builds_of_different_sizes_from_two_threads(cuda):
+    """Each on its own stream, with numbers of groups that take different amounts of shared memory."""
+    wants, errors = {}, []
+
+    def work(groups):
+        try:
+            ids = make_ids(600, 2, groups, 0.1, seed=groups)
+            want = R.sort_pairs(ids, groups)[2]
+            with torch.cuda.stream(torch.cuda.Stream()):
+                on_gpu = ids.cuda()
+                off = torch.zeros(groups + 1, dtype=torch.int32, device="cuda")
+                pos = [torch.zeros((600, 2), dtype=torch.int32, device="cuda") for _ in range(300)]
+                for p in pos:
+                    S.route_build(on_gpu, groups, off, None, p, stream=stream())
+                stream().synchronize()
+                wants[groups] = all(torch.equal(p.cpu(), want) for p in pos)
+        except Exception as e:  # noqa: BLE001 - shown below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(groups,)) for groups in (4096, 2500, 1500)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    clean()
+    assert not errors and wants == {4096: True, 2500: True, 1500: True}, errors
