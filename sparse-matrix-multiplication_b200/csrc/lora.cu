@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <cstdint>
 
 #include "groups.cuh"
@@ -308,11 +309,14 @@ __device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8
                 f[4] += hi4.x, f[5] += hi4.y, f[6] += hi4.z, f[7] += hi4.w;
             }
         }
-        const uint4 top = RowVec<DT, 16>::pack(f);
+        // A finite u is kept past FP16's range (hi at its end); an infinity or NaN is hi's alone, or lo would undo it.
         float g[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = DT == SPMM_DTYPE_F16 && fabsf(f[j]) < INFINITY ? fminf(fmaxf(f[j], -65504.f), 65504.f) : f[j];
+        const uint4 top = RowVec<DT, 16>::pack(g);
         RowVec<DT, 16>::unpack(top, g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = f[j] - g[j];
+        for (int j = 0; j < 8; ++j) g[j] = fabsf(g[j]) < INFINITY ? f[j] - g[j] : 0.f;
         const int at = row * 128 + piece / 8 * 16384 + (((piece % 8) ^ (row & 7)) << 4);
         *reinterpret_cast<uint4*>(hi + at) = top;
         *reinterpret_cast<uint4*>(hi + RB * 16384 + at) = RowVec<DT, 16>::pack(g);

@@ -199,3 +199,35 @@ def test_sorted_requests_of_one_adapter_give_the_same_rows(cuda):
     want, real, err = R.lora(None, ad.flatten(), x, a, b, None, None)
     close(one, want, real, err, BF16, 0.0)
     close(two, want, real, err, BF16, 0.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sizes", [[1, 1], [40, 1]])
+def test_infinite_intermediates_give_infinities_not_nan(cuda, sizes, dtype):
+    rows = sum(sizes)
+    x, a, b = values((rows, 64), dtype, 1), values((2, 16, 64), dtype, 2).abs() + 1, values((2, 72, 16), dtype, 3).abs() + 1
+    b[:, ::2] = -b[:, ::2]
+    x[0, 5] = float("inf")
+    out = torch.zeros((rows, 72), dtype=dtype, device="cuda")
+    S.lora(offsets(sizes).cuda(), torch.zeros(2, dtype=torch.int32, device="cuda"), x, a, b, out, stream=stream())
+    clean()
+    want, _, _ = R.lora(offsets(sizes), torch.zeros(2, dtype=torch.int32), x, a, b, None, None)
+    assert torch.isinf(want[0]).all() and torch.equal(R.d(out[0]), want[0])
+    assert torch.isfinite(out[1:]).all()
+
+
+@pytest.mark.parametrize("sizes", [[1, 1], [40, 1]])
+def test_intermediates_past_the_range_of_fp16(cuda, sizes):
+    """|u| is 64 * 64 or 80 times 16 and a little: kept to 2^-13 of itself, beside the bounds of the others."""
+    rows = sum(sizes)
+    x, b = torch.full((rows, 64), 16.0, dtype=F16, device="cuda"), values((2, 72, 16), F16, 3) * 2.0**-10
+    x += torch.arange(64, device="cuda").to(F16) / 64
+    a = torch.full((2, 16, 64), 64.0, dtype=F16, device="cuda")
+    a[:, 1::2] = -80.0
+    out = torch.zeros((rows, 72), dtype=F16, device="cuda")
+    S.lora(offsets(sizes).cuda(), torch.zeros(2, dtype=torch.int32, device="cuda"), x, a, b, out, stream=stream())
+    clean()
+    want, real, err = R.lora(offsets(sizes), torch.zeros(2, dtype=torch.int32), x, a, b, None, None)
+    u = R.d(x) @ R.d(a[0]).T
+    assert (u.abs() > 65520).all() and (u.abs() < 131008).all() and want.abs().max() < 60000
+    close(out, want, real, err + 2.0**-13 * (u.abs() @ R.d(b[0]).abs().T), F16, 0.0)
