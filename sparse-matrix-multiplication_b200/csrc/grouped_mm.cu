@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
         } else {
             build_tile_table(start, a.offsets, a.groups, a.rows, kTileM, err);
         }
-        tiles = start[a.groups] * a.ntiles;
+        tiles = min(start[a.groups], most_tiles(a.groups, a.rows, kTileM)) * a.ntiles;
     }
     tc_fence_before();
     __syncthreads();
@@ -825,7 +825,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
         tiles = a.groups * a.mtiles * a.ntiles;
     } else {
         build_tile_table(start, a.offsets, a.groups, a.rows, kPairM, blockIdx.x == 0 ? a.err : nullptr);
-        tiles = start[a.groups] * a.ntiles;
+        tiles = min(start[a.groups], most_tiles(a.groups, a.rows, kPairM)) * a.ntiles;
     }
     tc_fence_before();
     cluster_sync();  // the barriers of both blocks are set up, both have their TMEM
@@ -1063,7 +1063,8 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     t.ldb = a.ldb;
     t.err = a.err;
     // Row tiles: exact for dw, else as many as the groups can have (how many they do have is on the device).
-    const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * t.mtiles : a.rows / kTileM + std::min(a.groups, a.rows);
+    const int64_t mtiles = FORM == kDw ? static_cast<int64_t>(a.groups) * t.mtiles : most_tiles(a.groups, a.rows, kTileM);
+    if (mtiles * ((t.outs + 63) / 64) > INT32_MAX) return SPMM_ERR_TOO_LARGE;  // of the narrowest kind
     // Pairs of blocks where every pair has about four tiles (with three their coarser rounds cost what they gain: 0.92 to 1.13
     // of the single blocks' rate) and the groups are long: a row tile of 256 wastes 128 rows of a group on average, in dw a tile
     // has that much more to store. Measured at 16384 rows, 2048 x 2048, pairs against single blocks: 192 rows a group 1.07
@@ -1077,7 +1078,6 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     while (!any && tn > 64 && (mtiles * ((t.outs + tn - 1) / tn) < st->sm_count || t.outs <= tn / 2)) tn /= 2;
     t.ntiles = (t.outs + tn - 1) / tn;
     const int64_t tiles = mtiles * t.ntiles;
-    if (tiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
 
     CUtensorMap ma{}, small{}, mb{}, wide{};
     if (any) return tc_launch<FORM, 128, false, true>(ma, small, mb, wide, t, tiles, s, st);
@@ -1141,7 +1141,7 @@ int partial_products(const PartialProducts& p, cudaStream_t s, DeviceState* st) 
     t.singles = p.singles;
     t.err = st->err;
     const int tn = p.rank <= 64 ? 64 : (p.rank <= 128 ? 128 : 256);
-    const int64_t tiles = (p.rows / kTileM + std::min<int64_t>(p.groups, p.rows)) * p.most_splits;
+    const int64_t tiles = static_cast<int64_t>(most_tiles(p.groups, p.rows, kTileM)) * p.most_splits;
     if (tiles > INT32_MAX) return SPMM_ERR_TOO_LARGE;
     CUtensorMap ma, small, mb, wide;
     const uint64_t rows = p.rows, K = p.K, rank = p.rank;

@@ -26,8 +26,9 @@ __device__ __forceinline__ int group_matrix(const int* __restrict__ which, int g
     return i < 0 || i >= matrices ? -1 : i;
 }
 
-// start[g] = sum of count(0) .. count(g - 1), start[groups] = all of them. Called by every thread of the block; ends with
-// a barrier.
+// start[g] = sum of count(0) .. count(g - 1), start[groups] = all of them; counts are at most 2^24. Offsets out of order can
+// overlap and so count rows more than once: sums past 2^30 stay above it without being exact, and callers take no more
+// entries than groups without overlap have (most_tiles). Called by every thread of the block; ends with a barrier.
 template <class Count>
 __device__ __forceinline__ void build_table(int* start, int groups, Count count) {
     for (int g = threadIdx.x; g < groups; g += blockDim.x) start[g + 1] = count(g);
@@ -44,7 +45,7 @@ __device__ __forceinline__ void build_table(int* start, int groups, Count count)
                 if (static_cast<int>(threadIdx.x) >= d) v += u;
             }
             if (g < groups) start[g + 1] = run + v;
-            run += __shfl_sync(0xffffffffu, v, 31);
+            run = min(run + __shfl_sync(0xffffffffu, v, 31), 1 << 30);
         }
     }
     __syncthreads();
@@ -58,6 +59,9 @@ __device__ __forceinline__ void build_tile_table(int* start, const int* __restri
         return (r.end - r.begin + tile - 1) / tile;
     });
 }
+
+// Row tiles (of `tile` rows) that groups in order have at most.
+__host__ __device__ __forceinline__ int most_tiles(int groups, int rows, int tile) { return rows / tile + (groups < rows ? groups : rows); }
 
 // The group of entry m, 0 <= m < start[groups].
 __device__ __forceinline__ int tile_group(const int* start, int groups, int m) {

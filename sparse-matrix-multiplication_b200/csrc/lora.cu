@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         const GroupRange g = group_range(a.offsets, r, a.rows, blockIdx.x == 0 ? a.err : nullptr);
         return is_single(g) ? 0 : (g.end - g.begin + kTileM - 1) / kTileM;
     });
-    const long long pairs = static_cast<long long>(start[a.requests]) * e.ntiles;
+    const long long pairs = static_cast<long long>(min(start[a.requests], most_tiles(a.requests, a.rows, kTileM))) * e.ntiles;
     const int begin = static_cast<int>(pairs * blockIdx.x / gridDim.x), end = static_cast<int>(pairs * (blockIdx.x + 1) / gridDim.x);
     tc_fence_before();
     __syncthreads();
@@ -711,7 +711,7 @@ struct Shape {
 Shape shape_of(int32_t requests, int32_t rows, int32_t K) {
     Shape h{};
     h.rows = rows <= 4 * static_cast<int64_t>(requests);
-    h.mtiles = rows / kTileM + std::min(requests, rows);
+    h.mtiles = most_tiles(requests, rows, kTileM);
     // Ranges of the sum over K, from which the shrink chooses: enough that few tiles fill the GPU, each at least 4 steps of 64.
     h.most_splits = h.rows ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 1184 / std::max<int64_t>(1, h.mtiles), K / 256})));
     return h;

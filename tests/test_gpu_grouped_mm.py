@@ -359,3 +359,17 @@ def test_binding_refuses_other_shapes_and_types(cuda):
             S.grouped_mm(**{**dict(offsets=o, x=x, w=w, y=y), **bad})
     with pytest.raises(S.SpmmError):
         S.grouped_mm(o, x, w, y.half())  # out is neither x's type nor float32
+
+
+def test_offsets_that_count_rows_thousands_of_times(cuda):
+    """4096 groups that alternate between all 2^27 rows and none (out of order): 2^31 row tiles if each were taken."""
+    rows, i32 = 1 << 27, dict(dtype=torch.int32, device="cuda")
+    x, w = torch.zeros((rows, 8), dtype=BF16, device="cuda"), torch.zeros((4096, 8, 8), dtype=BF16, device="cuda")
+    guard = torch.full((rows + 64, 8), 5.0, dtype=BF16, device="cuda")
+    off = torch.tensor([0, rows] * 2048 + [0], **i32)
+    for run in (lambda y: S.grouped_mm(off, x, w, y, stream=stream()), lambda y: S.grouped_mm_dx(off, x, w, y, stream=stream()),
+                lambda y: S.lora(off, torch.zeros(4096, **i32), x, w, w, y, stream=stream())):
+        run(guard[32:32 + rows])
+        torch.cuda.synchronize()
+        assert S.device_error(0)[0] == -8
+        assert (guard[:32] == 5).all() and (guard[-32:] == 5).all()
