@@ -341,8 +341,8 @@ typedef struct spmm_route_view {
 } spmm_route_view;
 
 /* Tokens to their groups: xs[pos[t, j], :] = x[t, :] for every pair that has a row. Other rows of xs are left
- * as they were. H columns; dtype F16, BF16 or F32 (bits are copied). The gradient of x is
- * spmm_route_combine of the gradient of xs with w = NULL. */
+ * as they were. H columns, at most 2^24 (SPMM_ERR_TOO_LARGE above; here and below); dtype F16, BF16 or F32 (bits
+ * are copied). The gradient of x is spmm_route_combine of the gradient of xs with w = NULL. */
 int spmm_route_gather(const spmm_route_view* r, const void* x, int64_t ldx, void* xs, int64_t ldxs, int32_t H,
                       int32_t dtype, void* stream);
 

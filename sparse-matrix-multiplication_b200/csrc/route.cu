@@ -580,7 +580,8 @@ int route_args(const spmm_route_view* r, int32_t H, int32_t dtype) {
     if (!r || r->tokens < 0 || r->topk < 1 || r->rows < 0 || H < 0) return SPMM_ERR_INVALID_ARG;
     if (dtype != SPMM_DTYPE_F16 && dtype != SPMM_DTYPE_BF16 && dtype != SPMM_DTYPE_F32) return SPMM_ERR_INVALID_ARG;
     if (r->tokens > 0 && !r->pos) return SPMM_ERR_INVALID_ARG;
-    if (static_cast<int64_t>(r->tokens) * r->topk > INT32_MAX - 4095) return SPMM_ERR_TOO_LARGE;
+    // Vectors and bytes of a row are counted in ints.
+    if (static_cast<int64_t>(r->tokens) * r->topk > INT32_MAX - 4095 || H > (1 << 24)) return SPMM_ERR_TOO_LARGE;
     return SPMM_OK;
 }
 

@@ -110,3 +110,10 @@ def test_binding_refuses_tensors_off_the_gpu():
         S.grouped_mm(torch.zeros(2, dtype=torch.int32), x, torch.zeros((1, 8, 8), dtype=torch.bfloat16), x)
     with pytest.raises(ValueError):
         S.grouped_mm(torch.zeros(2, dtype=torch.int32), x.double(), torch.zeros((1, 8, 8)), x)
+
+
+@pytest.mark.parametrize("call", [lambda **k: gather(ldx=1 << 26, ldxs=1 << 26, **k), lambda **k: combine(ldys=1 << 26, ldy=1 << 26, **k),
+                                  lambda **k: combine_grad(lddy=1 << 26, ldys=1 << 26, lddys=1 << 26, **k)])
+def test_rows_too_long_to_count_are_refused(call):
+    assert call(H=(1 << 24) + 1) == TOO_LARGE
+    assert call(H=1 << 24) != TOO_LARGE
