@@ -395,9 +395,9 @@ typedef struct spmm_lora_view {
  * in spmm_grouped_mm; NULL = every row is a request of its own (requests == rows, single tokens). base: rows x N
  * (the shared projection's output), NULL = 0; out may be base itself (same stride). Rows in no request are left as
  * they were. One rounding of the result; the rank-wide intermediate is held in FP32 or as a sum of two 16-bit
- * terms (F16: |a * x| up to 131008, beyond 65504 to 2^-13 of it, and to 2^-25 where it is smallest). rank <= 256, requests <= 4096 (SPMM_ERR_TOO_LARGE above). A workspace of
- * spmm_lora_workspace_size bytes (any contents, 256-byte aligned) belongs to the call until it has run: calls that
- * overlap on the GPU need one each. */
+ * terms (F16: |a * x| up to 131008, beyond 65504 to 2^-13 of it, and to 2^-25 where it is smallest). rank <= 256,
+ * requests <= 4096 (SPMM_ERR_TOO_LARGE above). A workspace of spmm_lora_workspace_size bytes (any contents, 256-byte
+ * aligned) belongs to the call until it has run: calls that overlap on the GPU need one each. */
 int spmm_lora_workspace_size(const spmm_lora_view* l, int32_t requests, int32_t rows, size_t* bytes);
 int spmm_lora(const spmm_lora_view* l, const int32_t* offsets, const int32_t* adapter, int32_t requests, int32_t rows,
               const void* x, int64_t ldx, const void* base, int64_t ldbase, void* out, int64_t ldout, void* ws,
