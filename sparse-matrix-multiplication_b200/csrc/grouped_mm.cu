@@ -77,6 +77,7 @@ struct TcArgs {
     int sum;           // not dw: length of the sum
     int mtiles;        // dw: row tiles of a group
     int ntiles;
+    int blocks;        // that run at a time
     void* out;
     long long ldo;     // row stride of out
     int out_f32, dtype;
@@ -103,9 +104,9 @@ struct Tile {
     int steps;         // k steps
 };
 
-// The tiles in the order that blocks take them, block b those at b, b + grid, ... The last round, if it does not give every
-// block a tile, is cut into narrower ones (TN / parts columns) while that gives no block two: a block streams a tile no
-// faster for the others' being idle.
+// The tiles in the order that blocks take them: block b those at b, b + blocks, ..., in dw each the next that none has. The
+// last round, if it does not give every block a tile, is cut into narrower ones (TN / parts columns) while that gives no
+// block two: a block streams a tile no faster for the others' being idle.
 struct Rounds {
     int tiles;         // all of them, full width
     int whole;         // those of the full rounds
@@ -133,9 +134,8 @@ __device__ __forceinline__ void choose_splits(Rounds& r, int tiles, int steps, i
 }
 
 template <int TN>
-__device__ __forceinline__ Rounds rounds_of(int tiles) {
-    Rounds r;
-    const int grid = gridDim.x;
+__host__ __device__ __forceinline__ Rounds rounds_of(int tiles, int grid) {
+    Rounds r{};
     r.tiles = tiles;
     r.whole = tiles / grid * grid;
     const int rest = tiles - r.whole;
@@ -145,8 +145,61 @@ __device__ __forceinline__ Rounds rounds_of(int tiles) {
     return r;
 }
 
+// dw's tiles differ in length as the groups do, so they are taken one by one as blocks become free, those of the longest groups
+// first: the grid has a block for every tile, and the blocks that run take over those that have not started. Against equal
+// numbers of tiles in the groups' order: 16384 rows over 8 groups that fall like 1 / i, 512 x 512: 33.6 -> 24.5 us; 3001 over 16,
+// 520 x 776 in FP32: 19.2 -> 15.7; 8192 over 64 that fall like i^-1/2, 1024 x 1024: 39.7 -> 40.7 (short tiles, more of them at
+// once at the stores). The pairs' rounds keep the groups' order: sorted, they found less of each other's operands in L2
+// (65536 rows over 128 groups, 1024 x 2048: 324 -> 343 us).
+constexpr int kMostSorted = 128;  // groups; with more they come as they lie
+
+// The groups by falling length, equal ones as they lie. Called by every thread of the block; ends with a barrier.
+__device__ __forceinline__ void sort_groups(const TcArgs& a, int* length, uint8_t* order) {
+    const int g = threadIdx.x;
+    if (g < a.groups) {
+        const GroupRange r = group_range(a.offsets, g, a.rows, a.err);  // records bad ones
+        length[g] = r.end - r.begin;
+    }
+    __syncthreads();
+    if (g < a.groups) {
+        int before = 0;
+        for (int h = 0; h < a.groups; ++h) before += length[h] > length[g] || (length[h] == length[g] && h < g);
+        order[before] = static_cast<uint8_t>(g);
+    }
+    __syncthreads();
+}
+
+// Answers to the block's requests for tiles, four of them: from the producer, which asks, to the other warps.
+struct TileQueue {
+    static constexpr int kAnswers = 4;
+    uint32_t answers, full, empty;  // 16 bytes each, barriers
+
+    // Request n, once answer n - kAnswers has been read by all.
+    __device__ __forceinline__ bool ask(int n, volatile int* abort_flag) const {
+        const uint32_t s = n % kAnswers;
+        if (!mbar_wait(empty + 8 * s, ((n / kAnswers) & 1u) ^ 1u, abort_flag)) return false;
+        mbar_arrive_expect_tx(full + 8 * s, 16);
+        take_block(answers + 16 * s, full + 8 * s);
+        return true;
+    }
+    // Its answer. The reader then arrives on its `empty`, unless it is the one that asks.
+    __device__ __forceinline__ bool answer(int n, volatile int* abort_flag, int* t) const {
+        const uint32_t s = n % kAnswers;
+        if (!mbar_wait(full + 8 * s, (n / kAnswers) & 1u, abort_flag)) return false;
+        *t = taken_block(answers + 16 * s);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next answer comes by the asynchronous proxy
+        return true;
+    }
+    // By a whole warp.
+    __device__ __forceinline__ bool next(int n, volatile int* abort_flag, int* t) const {
+        const bool ok = __all_sync(0xffffffffu, answer(n, abort_flag, t));
+        if (ok && (threadIdx.x & 31) == 0) mbar_arrive_count(empty + 8 * (n % kAnswers), 1);
+        return ok;
+    }
+};
+
 template <int FORM, int TN, bool SINGLES>
-__device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, const Rounds& rounds, int t) {
+__device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, const uint8_t* order, const Rounds& rounds, int t) {
     Tile r;
     int g, local, mtiles, width = TN, part = 0;
     if (t >= rounds.whole && rounds.parts > 1) {
@@ -165,6 +218,7 @@ __device__ __forceinline__ Tile tile_of(const TcArgs& a, const int* start, const
         g = t / per;
         local = t - g * per;
         mtiles = a.mtiles;
+        if (order) g = order[g];
     } else {
         g = tile_group(start, a.groups, t / a.ntiles);
         local = t - start[g] * a.ntiles;
@@ -391,9 +445,23 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ int singles;
     __shared__ uint16_t single[SINGLES ? SPMM_MAX_GROUPS : 1];
+    constexpr bool kQueue = FORM == kDw && !ANY;
+    __shared__ alignas(16) uint4 answers[kQueue ? TileQueue::kAnswers : 1];
+    __shared__ unsigned long long answer_bars[kQueue ? 2 * TileQueue::kAnswers : 1];  // full[], empty[]
+    __shared__ int lengths[kQueue ? kMostSorted : 1];
+    __shared__ uint8_t sorted[kQueue ? kMostSorted : 1];
+    const TileQueue queue{smem_addr(answers), smem_addr(answer_bars), smem_addr(answer_bars) + 8 * TileQueue::kAnswers};
+    const bool queued = kQueue && gridDim.x > static_cast<unsigned>(a.blocks);  // else a tile a block
+    const uint8_t* order = queued && a.groups <= kMostSorted ? sorted : nullptr;
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
+        if constexpr (kQueue) {
+            for (int s = 0; s < TileQueue::kAnswers; ++s) {
+                mbar_init(queue.full + 8 * s, 1);
+                mbar_init(queue.empty + 8 * s, 1 + kEpilogue);
+            }
+        }
         for (int s = 0; s < kStages; ++s) {
             mbar_init(full0 + 8 * s, ANY ? kLoaders : 1);
             mbar_init(empty0 + 8 * s, 1);
@@ -414,7 +482,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
     allow_dependent_launch();
     int tiles;
     if constexpr (FORM == kDw) {
-        if (blockIdx.x == 0)
+        if (order) sort_groups(a, lengths, sorted);
+        else if (queued || blockIdx.x == 0)  // any block may be the one that others take over
             for (int g = threadIdx.x; g < a.groups; g += blockDim.x) group_range(a.offsets, g, a.rows, a.err);  // records bad ones
         tiles = a.groups * a.mtiles * a.ntiles;
     } else {
@@ -447,7 +516,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    Rounds rounds = rounds_of<TN>(tiles);
+    Rounds rounds = rounds_of<TN>(tiles, a.blocks);
     if constexpr (SINGLES) {
         choose_splits(rounds, tiles, (a.sum + kStepK - 1) / kStepK, a.most_splits);
         rounds.units = rounds.whole = tiles * rounds.splits;  // cut along the sum, not the columns
@@ -459,8 +528,15 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
             int it = 0, s = 0;
             uint32_t phase = 1;
             bool ok = true;
-            for (int t = blockIdx.x; ok && t < rounds.units; t += gridDim.x) {
-                const Tile r = tile_of<FORM, TN, SINGLES>(a, start, rounds, t);
+            int asked = 0;
+            const auto next = [&](int t, int n) {  // the tile behind the block's n-th, t
+                if (!queued) return t + static_cast<int>(gridDim.x);
+                if (ok && asked == n) ok = queue.ask(asked, abort_flag), asked += ok;
+                if (ok) ok = queue.answer(n, abort_flag, &t);
+                return t;
+            };
+            for (int t = blockIdx.x, n = 0; ok && t < rounds.units; t = next(t, n++)) {
+                const Tile r = tile_of<FORM, TN, SINGLES>(a, start, order, rounds, t);
                 const bool small = FORM != kDw && r.end - r.begin - r.m0 <= kSmallRows;
                 // Boxes of 64 columns that lie wholly past the operand are not loaded; their part of D is not stored.
                 if (r.cols == 0) continue;
@@ -480,6 +556,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
                     if constexpr (FORM == kDw) {
                         for (int j = 0; j < na; ++j) tma_load_2d(sa + j * 8192, &map_a, bar, r.m0 + 64 * j, r.begin + k0);
                         for (int j = 0; j < nb; ++j) tma_load_2d(sb + j * 8192, &map_b, bar, r.n0 + 64 * j, r.begin + k0);
+                        // Not before the tile's last loads: a tile taken earlier would wait here while other blocks are free.
+                        if (queued && ks == r.steps - 1) ok = queue.ask(asked, abort_flag), asked += ok;
                     } else {
                         tma_load_2d(sa, small ? &map_a_small : &map_a, bar, k0, r.begin + r.m0);
                         if (FORM == kForward && wide) {
@@ -496,6 +574,12 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
                 record_device_error(a.err, SPMM_ERR_TIMEOUT, 11);
             }
             // The block's shared memory outlives every copy into it and every arrival on its barriers.
+            if (!ok && asked > 0) {
+                const unsigned long long t0 = global_ns();
+                while (!mbar_try_wait(queue.full + 8 * ((asked - 1) % TileQueue::kAnswers), ((asked - 1) / TileQueue::kAnswers) & 1u) &&
+                       global_ns() - t0 < kWaitNs) {
+                }
+            }
             for (int i = max(0, it - kStages); i < it; ++i) {
                 const unsigned long long t0 = global_ns();
                 while (!mbar_try_wait(full0 + 8 * (i % kStages), (i / kStages) & 1u) && global_ns() - t0 < kWaitNs) {
@@ -505,10 +589,15 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer: one lane; in dw the whole warp clears the rows past a group's end
-        int it = 0, n = 0;
+        int it = 0, n = 0, taken = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < rounds.units; t += gridDim.x) {
-            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, rounds, t);
+        const auto next = [&](int t) {
+            if (!queued) return t + static_cast<int>(gridDim.x);
+            ok = ok && queue.next(taken++, abort_flag, &t);
+            return t;
+        };
+        for (int t = blockIdx.x; ok && t < rounds.units; t = next(t)) {
+            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, order, rounds, t);
             if (r.cols == 0) continue;
             const int buf = n & 1;
             const uint32_t acc = tmem + buf * TN;
@@ -582,7 +671,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
         uint32_t phase = 1;
         bool ok = true;
         for (int t = blockIdx.x; ok && t < rounds.units; t += gridDim.x) {
-            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, rounds, t);
+            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, order, rounds, t);
             if (r.cols == 0) continue;
             for (int ks = 0; ks < r.steps; ++ks) {
                 ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, phase, abort_flag));
@@ -618,10 +707,15 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
         const int q = warp & 3, part = (warp - 2) >> 2;  // warps q and q + 4 may access TMEM lanes 32 q ..
         const int size = a.out_f32 ? 4 : 2;
         const bool sectors = (reinterpret_cast<uintptr_t>(a.out) | static_cast<uintptr_t>(a.ldo * size)) % 32 == 0;
-        int n = 0;
+        int n = 0, taken = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < rounds.units; t += gridDim.x) {
-            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, rounds, t);
+        const auto next = [&](int t) {
+            if (!queued) return t + static_cast<int>(gridDim.x);
+            ok = queue.next(taken++, abort_flag, &t);
+            return t;
+        };
+        for (int t = blockIdx.x; ok && t < rounds.units; t = next(t)) {
+            const Tile r = tile_of<FORM, TN, SINGLES>(a, start, order, rounds, t);
             if (r.cols == 0) continue;
             const int buf = n & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag))) {
@@ -708,8 +802,12 @@ int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     const size_t smem = L::kFixed + (FORM == kDw ? 0 : 4 * (static_cast<size_t>(a.groups) + 1));
-    const unsigned grid = static_cast<unsigned>(SINGLES ? st->sm_count : std::min<long long>(tiles * (TN / 64), st->sm_count));
-    return launch_dependent(grouped_tc_kernel<FORM, TN, SINGLES, ANY>, dim3(grid), dim3(tc_threads(SINGLES, ANY)), smem, s, ma, small, mb, wide, a);
+    const bool queue = FORM == kDw && !ANY;  // a block for every unit, those that run take the others'
+    const long long units = queue ? rounds_of<TN>(static_cast<int>(tiles), st->sm_count).units : std::min<long long>(tiles * (TN / 64), st->sm_count);
+    const unsigned grid = static_cast<unsigned>(SINGLES ? st->sm_count : units);
+    TcArgs args = a;
+    args.blocks = queue ? st->sm_count : static_cast<int>(grid);
+    return launch_dependent(grouped_tc_kernel<FORM, TN, SINGLES, ANY>, dim3(grid), dim3(tc_threads(SINGLES, ANY)), smem, s, ma, small, mb, wide, args);
 }
 
 // ------------------------------------------------------------------ tcgen05, pairs of blocks

@@ -58,6 +58,26 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
+// Asks for a block of the grid that has not started, to do its work here instead: 16 bytes of answer (16-byte aligned), counted
+// by the barrier. Not to be asked again after an answer of none.
+__device__ __forceinline__ void take_block(uint32_t answer, uint32_t bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+
+// Its index along x, or INT_MAX for none.
+__device__ __forceinline__ int taken_block(uint32_t answer) {
+    uint32_t x = 0x7fffffffu;
+    asm volatile(
+        "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 r, [%1];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, r;\n\t}"
+        : "+r"(x)
+        : "r"(answer)
+        : "memory");
+    return static_cast<int>(x);
+}
+
 // Non-blocking test of a phase.
 __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;

@@ -373,3 +373,48 @@ def test_offsets_that_count_rows_thousands_of_times(cuda):
         torch.cuda.synchronize()
         assert S.device_error(0)[0] == -8
         assert (guard[:32] == 5).all() and (guard[-32:] == 5).all()
+
+
+@pytest.mark.parametrize("out", [F16, F32])
+@pytest.mark.parametrize("sizes", [[700] + [3] * 30 + [0, 0, 350, 64, 1, 129], [0] * 60 + [200, 15, 33] + [1] * 70, [5, 0, 90] * 60, [40] * 128])
+def test_weights_gradients_of_many_tiles(cuda, sizes, out):
+    """More tiles than blocks, of up to 128 groups (sorted) and of more: each computed once, whoever takes it."""
+    off = offsets(sizes, 4)
+    rows = int(off[-1]) + 70
+    dy, x = values((rows, 520), F16, 1), values((rows, 328), F16, 2)
+    dy[:4], x[int(off[-1]):] = float("nan"), float("inf")
+    want, mag = R.grouped_dw(off, dy, x)
+    runs = []
+    for _ in range(3):
+        dw = torch.full((len(sizes), 520, 328), float("nan"), dtype=out, device="cuda")
+        S.grouped_mm_dw(off.cuda(), dy, x, dw, stream=stream())
+        runs.append(dw)
+    clean()
+    R.close(runs[0], want, mag, max(sizes), out, "dw")
+    assert all(torch.equal(runs[0], t) for t in runs[1:])
+
+
+def test_weights_gradients_on_two_streams_at_once_and_replayed(cuda):
+    """Kernels that take each other's place on the GPU keep to their own tiles."""
+    sizes = [900, 0] + [60] * 38
+    off = offsets(sizes).cuda()
+    n = sum(sizes)
+    ops = [(values((n, 520), BF16, 10 * i), values((n, 776), BF16, 10 * i + 1)) for i in range(2)]
+    wants = []
+    for dy, x in ops:
+        wants.append(torch.zeros((40, 520, 776), device="cuda"))
+        S.grouped_mm_dw(off, dy, x, wants[-1], stream=stream())
+    torch.cuda.synchronize()
+    gots, graphs, streams = [torch.zeros_like(w) for w in wants], [], [torch.cuda.Stream() for _ in wants]
+    for (dy, x), got in zip(ops, gots):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(10):
+                S.grouped_mm_dw(off, dy, x, got, stream=stream())
+        graphs.append(graph)
+    for _ in range(3):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    clean()
+    assert all(torch.equal(w, g) for w, g in zip(wants, gots))
