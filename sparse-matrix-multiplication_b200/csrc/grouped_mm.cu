@@ -149,8 +149,8 @@ __host__ __device__ __forceinline__ Rounds rounds_of(int tiles, int grid) {
 // first: the grid has a block for every tile, and the blocks that run take over those that have not started. Against equal
 // numbers of tiles in the groups' order: 16384 rows over 8 groups that fall like 1 / i, 512 x 512: 33.6 -> 24.5 us; 3001 over 16,
 // 520 x 776 in FP32: 19.2 -> 15.7; 8192 over 64 that fall like i^-1/2, 1024 x 1024: 39.7 -> 40.7 (short tiles, more of them at
-// once at the stores). The pairs' rounds keep the groups' order: sorted, they found less of each other's operands in L2
-// (65536 rows over 128 groups, 1024 x 2048: 324 -> 343 us).
+// once at the stores). The pairs of blocks keep to equal numbers in the groups' order: they read less from L2 when they run in
+// step (65536 rows over 128 groups, 1024 x 2048: 324 us, sorted 343; 16384 over 8, 4096 x 2048: 200 us, as they become free 228).
 constexpr int kMostSorted = 128;  // groups; with more they come as they lie
 
 // The groups by falling length, equal ones as they lie. Called by every thread of the block; ends with a barrier.
