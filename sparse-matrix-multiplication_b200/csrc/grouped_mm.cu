@@ -104,8 +104,8 @@ struct Tile {
     int steps;         // k steps
 };
 
-// The tiles in the order that blocks take them: block b those at b, b + blocks, ..., in dw each the next that none has. The
-// last round, if it does not give every block a tile, is cut into narrower ones (TN / parts columns) while that gives no
+// The tiles in the order that blocks take them: block b those at b, b + blocks, ..., with a queue each the next that none has.
+// The last round, if it does not give every block a tile, is cut into narrower ones (TN / parts columns) while that gives no
 // block two: a block streams a tile no faster for the others' being idle.
 struct Rounds {
     int tiles;         // all of them, full width
@@ -146,7 +146,7 @@ __host__ __device__ __forceinline__ Rounds rounds_of(int tiles, int grid) {
 }
 
 // dw's tiles differ in length as the groups do, so they are taken one by one as blocks become free, those of the longest groups
-// first: the grid has a block for every tile, and the blocks that run take over those that have not started. Against equal
+// first (the other forms': tc_launch): the grid has a block for every tile, and the blocks that run take over those that have not started. Against equal
 // numbers of tiles in the groups' order: 16384 rows over 8 groups that fall like 1 / i, 512 x 512: 33.6 -> 24.5 us; 3001 over 16,
 // 520 x 776 in FP32: 19.2 -> 15.7; 8192 over 64 that fall like i^-1/2, 1024 x 1024: 39.7 -> 40.7 (short tiles, more of them at
 // once at the stores). The pairs of blocks keep to equal numbers in the groups' order: they read less from L2 when they run in
@@ -445,14 +445,14 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ int singles;
     __shared__ uint16_t single[SINGLES ? SPMM_MAX_GROUPS : 1];
-    constexpr bool kQueue = FORM == kDw && !ANY;
+    constexpr bool kQueue = !ANY && !SINGLES;
     __shared__ alignas(16) uint4 answers[kQueue ? TileQueue::kAnswers : 1];
     __shared__ unsigned long long answer_bars[kQueue ? 2 * TileQueue::kAnswers : 1];  // full[], empty[]
-    __shared__ int lengths[kQueue ? kMostSorted : 1];
-    __shared__ uint8_t sorted[kQueue ? kMostSorted : 1];
+    __shared__ int lengths[FORM == kDw ? kMostSorted : 1];
+    __shared__ uint8_t sorted[FORM == kDw ? kMostSorted : 1];
     const TileQueue queue{smem_addr(answers), smem_addr(answer_bars), smem_addr(answer_bars) + 8 * TileQueue::kAnswers};
     const bool queued = kQueue && gridDim.x > static_cast<unsigned>(a.blocks);  // else a tile a block
-    const uint8_t* order = queued && a.groups <= kMostSorted ? sorted : nullptr;
+    const uint8_t* order = FORM == kDw && queued && a.groups <= kMostSorted ? sorted : nullptr;
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -522,6 +522,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
         rounds.units = rounds.whole = tiles * rounds.splits;  // cut along the sum, not the columns
     }
 
+    // The grid may have more blocks than there are tiles, which only the device knows: queued, they are all taken over.
+    const int end = queued ? INT_MAX : rounds.units;
     if (warp == 0) {
         // ---------------- producer
         if (!ANY && elect_one()) {
@@ -535,7 +537,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
                 if (ok) ok = queue.answer(n, abort_flag, &t);
                 return t;
             };
-            for (int t = blockIdx.x, n = 0; ok && t < rounds.units; t = next(t, n++)) {
+            for (int t = blockIdx.x, n = 0; ok && t < end; t = next(t, n++)) {
+                if (t >= rounds.units) continue;
                 const Tile r = tile_of<FORM, TN, SINGLES>(a, start, order, rounds, t);
                 const bool small = FORM != kDw && r.end - r.begin - r.m0 <= kSmallRows;
                 // Boxes of 64 columns that lie wholly past the operand are not loaded; their part of D is not stored.
@@ -556,8 +559,6 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
                     if constexpr (FORM == kDw) {
                         for (int j = 0; j < na; ++j) tma_load_2d(sa + j * 8192, &map_a, bar, r.m0 + 64 * j, r.begin + k0);
                         for (int j = 0; j < nb; ++j) tma_load_2d(sb + j * 8192, &map_b, bar, r.n0 + 64 * j, r.begin + k0);
-                        // Not before the tile's last loads: a tile taken earlier would wait here while other blocks are free.
-                        if (queued && ks == r.steps - 1) ok = queue.ask(asked, abort_flag), asked += ok;
                     } else {
                         tma_load_2d(sa, small ? &map_a_small : &map_a, bar, k0, r.begin + r.m0);
                         if (FORM == kForward && wide) {
@@ -567,6 +568,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
                                 tma_load_3d(sb + j * 8192, &map_b, bar, FORM == kForward ? k0 : r.n0 + 64 * j, FORM == kForward ? r.n0 + 64 * j : k0, r.g);
                         }
                     }
+                    // Not before the tile's last loads: a tile taken earlier would wait here while other blocks are free.
+                    if (queued && ks == r.steps - 1) ok = queue.ask(asked, abort_flag), asked += ok;
                 }
             }
             if (!ok) {
@@ -596,7 +599,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
             ok = ok && queue.next(taken++, abort_flag, &t);
             return t;
         };
-        for (int t = blockIdx.x; ok && t < rounds.units; t = next(t)) {
+        for (int t = blockIdx.x; ok && t < end; t = next(t)) {
+            if (t >= rounds.units) continue;
             const Tile r = tile_of<FORM, TN, SINGLES>(a, start, order, rounds, t);
             if (r.cols == 0) continue;
             const int buf = n & 1;
@@ -714,7 +718,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
             ok = queue.next(taken++, abort_flag, &t);
             return t;
         };
-        for (int t = blockIdx.x; ok && t < rounds.units; t = next(t)) {
+        for (int t = blockIdx.x; ok && t < end; t = next(t)) {
+            if (t >= rounds.units) continue;
             const Tile r = tile_of<FORM, TN, SINGLES>(a, start, order, rounds, t);
             if (r.cols == 0) continue;
             const int buf = n & 1;
@@ -802,8 +807,14 @@ int tc_launch(const CUtensorMap& ma, const CUtensorMap& small, const CUtensorMap
         attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
     const size_t smem = L::kFixed + (FORM == kDw ? 0 : 4 * (static_cast<size_t>(a.groups) + 1));
-    const bool queue = FORM == kDw && !ANY;  // a block for every unit, those that run take the others'
-    const long long units = queue ? rounds_of<TN>(static_cast<int>(tiles), st->sm_count).units : std::min<long long>(tiles * (TN / 64), st->sm_count);
+    // With a queue a block for every unit, those that run take the others'. dw's are known here; of the other two there are as
+    // many as there can be, and a queue where rows of w lie across 128-byte lines: there blocks stream at unequal rates
+    // (20000 rows over 128 groups, 1400 x 2040: 234 -> 209 us; 5003 over 60, 1000 x 1960: 79 -> 72; 6000 over 40, dx of
+    // 1288 x 2568: 84 -> 80). Elsewhere they keep step, and the same read of each other's operands in L2 (20000 over 128,
+    // 1408 x 2048: 189 us, 193 queued).
+    const bool queue = !ANY && !SINGLES && (FORM == kDw || (tiles > 2 * st->sm_count && (FORM == kForward ? a.sum : a.outs) % 64 != 0));
+    long long units = std::min<long long>(tiles * (TN / 64), st->sm_count);
+    if (queue) units = FORM == kDw ? rounds_of<TN>(static_cast<int>(tiles), st->sm_count).units : std::min<long long>(tiles * (TN / 64), tiles + st->sm_count);
     const unsigned grid = static_cast<unsigned>(SINGLES ? st->sm_count : units);
     TcArgs args = a;
     args.blocks = queue ? st->sm_count : static_cast<int>(grid);

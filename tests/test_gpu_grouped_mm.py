@@ -418,3 +418,11 @@ def test_weights_gradients_on_two_streams_at_once_and_replayed(cuda):
                 graph.replay()
     clean()
     assert all(torch.equal(w, g) for w, g in zip(wants, gots))
+
+
+@pytest.mark.parametrize("out", [F16, F32])
+@pytest.mark.parametrize("sizes", [[0] * 150 + [200, 30] + [1] * 60, [3] * 100 + [0, 600, 129], [64] * 200, [1, 128] * 50])
+def test_products_of_many_tiles(cuda, sizes, out):
+    """More tiles than blocks, fewer than the groups could have, rows of 464 and of 1040 bytes."""
+    check_all(sizes, 520, 232, F16, out=out, first=5, tail=77)
+    check_all(sizes, 232, 520, F16, out=out)
