@@ -64,7 +64,8 @@ struct TcLayout {
     static constexpr int kStage = kA + kB;
     static constexpr int kStages = ANY ? 4 : (TN == 256 ? 4 : (TN == 128 ? 6 : 8));  // 192 KB, 128 with ANY
     static constexpr int kOut = kStages * kStage;
-    static constexpr int kBars = kOut + (ANY ? kEpilogue * kTransposed : (FORM == kDw ? kEpilogue * kStoreBox : 0));  // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
+    // full[], empty[], acc_full[2], acc_empty[2], drain, tmem slot, abort
+    static constexpr int kBars = kOut + (ANY ? kEpilogue * kTransposed : (FORM == kDw ? kEpilogue * kStoreBox : 0));
     static constexpr int kTable = kBars + 8 * (2 * kStages + 5) + 16;
     static constexpr int kFixed = kTable + 1024;     // room to align the base to 1 KB; then int[groups + 1]
 };
@@ -756,7 +757,8 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
                             const float f = tile[i * 33 + lane];
                             char* o = corner + i * a.ldo * size;
                             if (a.out_f32) *reinterpret_cast<float*>(o) = f;
-                            else *reinterpret_cast<uint16_t*>(o) = a.dtype == SPMM_DTYPE_BF16 ? float_to_half_bits<SPMM_DTYPE_BF16>(f) : float_to_half_bits<SPMM_DTYPE_F16>(f);
+                            else if (a.dtype == SPMM_DTYPE_BF16) *reinterpret_cast<uint16_t*>(o) = float_to_half_bits<SPMM_DTYPE_BF16>(f);
+                            else *reinterpret_cast<uint16_t*>(o) = float_to_half_bits<SPMM_DTYPE_F16>(f);
                         }
                     } else if (row < rows) {
                         store_piece(a, v, out + c0 * size, cols - c0, sectors);
@@ -1131,7 +1133,8 @@ int pair_launch(const GroupedArgs& g, TcArgs a, cudaStream_t s, DeviceState* st)
     SPMM_TRY(encode_2d(&ma, g.a, FORM == kForward ? K : N, rows, g.lda * 2, 64, FORM == kDw ? 64 : 128, CU_TENSOR_MAP_SWIZZLE_128B));
     if constexpr (FORM == kDw) {
         SPMM_TRY(encode_2d(&mb, g.b, K, rows, g.ldb * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B));
-        SPMM_TRY(encode_3d(&out, g.out, {K, N, groups}, {K * size, N * K * size}, {static_cast<uint32_t>(128 / size), 32, 1}, CU_TENSOR_MAP_SWIZZLE_128B, g.out_f32));
+        SPMM_TRY(encode_3d(&out, g.out, {K, N, groups}, {K * size, N * K * size}, {static_cast<uint32_t>(128 / size), 32, 1},
+                           CU_TENSOR_MAP_SWIZZLE_128B, g.out_f32));
     } else {
         SPMM_TRY(encode_3d(&mb, g.b, {K, N, groups}, {K * 2, N * K * 2}, {64, FORM == kForward ? 128u : 64u, 1}, CU_TENSOR_MAP_SWIZZLE_128B));
     }
@@ -1178,7 +1181,8 @@ int grouped_launch(const GroupedArgs& a, int dtype, cudaStream_t s, DeviceState*
     // of the single blocks' rate) and the groups are long: a row tile of 256 wastes 128 rows of a group on average, in dw a tile
     // has that much more to store. Measured at 16384 rows, 2048 x 2048, pairs against single blocks: 192 rows a group 1.07
     // (forward), 1.05 (dx), 0.76 (dw); 384: 1.10, 1.13, 1.06; 1024: 1.20, 1.16, 1.12.
-    const int64_t pair_tiles = (FORM == kDw ? static_cast<int64_t>(a.groups) * ((a.N + kPairM - 1) / kPairM) : a.rows / kPairM) * ((t.outs + kPairN - 1) / kPairN);
+    const int64_t pair_rows = FORM == kDw ? static_cast<int64_t>(a.groups) * ((a.N + kPairM - 1) / kPairM) : a.rows / kPairM;
+    const int64_t pair_tiles = pair_rows * ((t.outs + kPairN - 1) / kPairN);
     if (!any && t.outs >= kPairN && (FORM != kDw || a.N >= kPairM) && a.rows / a.groups >= (FORM == kDw ? 384 : 192) && pair_tiles >= 2 * st->sm_count)
         return pair_launch<FORM>(a, t, s, st);
     // The widest tile that still gives every SM one: a wide tile reads A less often, narrow ones spread few rows.
