@@ -220,8 +220,10 @@ __global__ void __launch_bounds__(256) lora_expand_rows_kernel(LoraArgs a, int c
 // Requests of one row come behind the tiles through the same ring: a stage is then as many of b's column tiles as it
 // holds, and the epilogue warps take the dot products with u from it on CUDA cores (lanes loading b themselves took 17 us
 // where the 100 single rows of a mixed batch now take 4).
-// The MMA needs 16-bit u; one term would cost half a step of 16 bits in every product (2^-8 in bf16), two leave 2^-16
-// for twice the MMAs, which still run under the copies.
+// The MMA needs 16-bit u; one term would cost half a step of 16 bits in every product (2^-8 in bf16), two leave half a step of
+// a half step (2^-16 in bf16, 2^-22 in fp16) for twice the MMAs, which still run under the copies. FP16's terms have
+// neither the range nor the small steps of FP32, so a row of u is held with a power of two taken out, its largest element in
+// [2^14, 2^15); the epilogue puts it back.
 
 constexpr int kTileM = 128;
 constexpr int kSetWarps = 8;
@@ -244,7 +246,11 @@ struct ExpandLayout {
     static constexpr int kStage0 = kUs * kU;
     static constexpr int kBars = kStage0 + kStages * kStage;  // full[], empty[], u_full[2], u_empty[2], acc_full[2], acc_empty[2], drain, u_first
     static constexpr int kInfo = kBars + 8 * (2 * kStages + 10);  // StageInfo[kStages]
-    static constexpr int kSlot = kInfo + 32 * kStages;
+    // Powers of two taken out of u's rows, of kUs + 2 units: u of a unit is made once the MMAs of the unit kUs before it are
+    // done, when the epilogue may still be at the last tile of that one and, if it has a single tile, of the one before it.
+    static constexpr int kScales = 4;
+    static constexpr int kExp = kInfo + 32 * kStages;  // int8_t[kScales][kTileM]
+    static constexpr int kSlot = kExp + kScales * kTileM;
     static constexpr int kTable = kSlot + 8;
     static constexpr int kFixed = kTable + 1024;
 };
@@ -270,7 +276,7 @@ struct StageInfo {
     int row, i, nt;
     float scale;
     int16_t first, last;  // tile of its unit
-    int tile;          // 1: a tile for the tensor cores
+    int tile;          // a tile for the tensor cores: 1 + the place of its unit's powers of two; else 0
     int singles;       // column tiles from nt on of a request of one row, else 0
 };
 
@@ -288,19 +294,22 @@ __device__ __forceinline__ Unit unit_of(const ExpandArgs& e, const int* start, i
     return x;
 }
 
-// u of one unit into shared memory, by `warps` warps of which this is the `w`-th: the parts' sum, hi and lo. Pieces of 8
-// ranks to consecutive threads; the parts' loads of a piece are in flight together.
+// u of one unit into shared memory, by `warps` warps of which this is the `w`-th: the parts' sum, hi and lo. A row's pieces of 8
+// ranks to consecutive lanes; the parts' loads of a piece are in flight together.
 template <int DT, int RB>
-__device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8_t* hi, int w, int warps) {
+__device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8_t* hi, int8_t* exponents, int w, int warps) {
     const LoraArgs& a = e.l;
     const int pieces = (a.rank + 15) / 16 * 2;  // the last may lie past the rank and is zero
+    int lanes = 2;                              // that a row takes
+    while (lanes < pieces) lanes *= 2;
+    const int lane = threadIdx.x & 31, piece = lane & (lanes - 1), per_warp = 32 / lanes;
     const int splits = e.singles[1];
     const float* parts = a.u + static_cast<long long>(x.row) * a.rank;
     const long long stride = static_cast<long long>(a.rows) * a.rank;
-    for (int k = w * 32 + (threadIdx.x & 31); k < x.rows * pieces; k += warps * 32) {
-        const int row = k / pieces, piece = k - row * pieces;
+    for (int row0 = w * per_warp; row0 < x.rows; row0 += warps * per_warp) {
+        const int row = row0 + lane / lanes;
         float f[8] = {};
-        if (8 * piece < a.rank) {
+        if (row < x.rows && 8 * piece < a.rank) {
             const float* src = parts + static_cast<long long>(row) * a.rank + 8 * piece;
 #pragma unroll 4
             for (int s = 0; s < splits; ++s) {
@@ -309,12 +318,23 @@ __device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8
                 f[4] += hi4.x, f[5] += hi4.y, f[6] += hi4.z, f[7] += hi4.w;
             }
         }
-        // A finite u is kept past FP16's range (hi at its end); an infinity or NaN is hi's alone, or lo would undo it.
-        float g[8];
+        if constexpr (DT == SPMM_DTYPE_F16) {
+            float most = 0.f;  // of the finite ones
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[j] = DT == SPMM_DTYPE_F16 && fabsf(f[j]) < INFINITY ? fminf(fmaxf(f[j], -65504.f), 65504.f) : f[j];
-        const uint4 top = RowVec<DT, 16>::pack(g);
+            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
+            for (int d = lanes / 2; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            // Sums of products of FP16 values are 0 or between 2^-48 and 2^56: -62 <= exponent <= 42.
+            const int exponent = most > 0.f ? static_cast<int>(__float_as_uint(most) >> 23) - 127 - 14 : 0;
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - exponent) << 23);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] *= down;
+            if (piece == 0 && row < x.rows) exponents[row] = static_cast<int8_t>(exponent);
+        }
+        if (row >= x.rows || piece >= pieces) continue;
+        const uint4 top = RowVec<DT, 16>::pack(f);
+        float g[8];
         RowVec<DT, 16>::unpack(top, g);
+        // An infinity or NaN is hi's alone, or lo would undo it.
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = fabsf(g[j]) < INFINITY ? f[j] - g[j] : 0.f;
         const int at = row * 128 + piece / 8 * 16384 + (((piece % 8) ^ (row & 7)) << 4);
@@ -389,6 +409,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base + L::kSlot);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     StageInfo* infos = reinterpret_cast<StageInfo*>(base + L::kInfo);
+    int8_t* exponents = reinterpret_cast<int8_t*>(base + L::kExp);
     int* start = reinterpret_cast<int*>(base + L::kTable);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -432,7 +453,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             const Unit x = unit_of(e, start, t, end);
             t += x.nt1 - x.nt0;
             if (x.i < 0) continue;
-            make_u<DT, RB>(e, x, base, warp - 2, kExpandThreads / 32 - 2);
+            make_u<DT, RB>(e, x, base, exponents, warp - 2, kExpandThreads / 32 - 2);
             if (lane == 0) mbar_arrive_count(u_first, 1);
             break;
         }
@@ -441,7 +462,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     if (warp == 0) {
         // ---------------- producer
         if (elect_one()) {
-            int it = 0;
+            int it = 0, nu = 0;
             bool ok = true;
             // The next stage, once it is free, with its description; its copies follow.
             const auto claim = [&](const StageInfo& info) {
@@ -458,8 +479,9 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                 t += x.nt1 - x.nt0;
                 const bool small = x.rows <= kSmallRows;
                 const float scale = x.i >= 0 && a.scale ? __ldg(a.scale + x.i) : 1.f;
+                const int tile = x.i >= 0 ? 1 + nu++ % L::kScales : 0;
                 for (int nt = x.nt0; nt < x.nt1; ++nt) {
-                    const int s = claim({x.rows, x.row, x.i, nt, scale, nt == x.nt0, nt == x.nt1 - 1, x.i >= 0, 0});
+                    const int s = claim({x.rows, x.row, x.i, nt, scale, nt == x.nt0, nt == x.nt1 - 1, tile, 0});
                     if (!ok) break;
                     const uint32_t bar = full0 + 8 * s, sb = sbase + L::kStage0 + s * L::kStage, sbs = sb + L::kB;
                     const int n0 = nt * kTn, blocks = min(kTn / 64, (a.N - n0 + 63) / 64);
@@ -578,6 +600,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             }
             const int cols = min(kTn, a.N - x.nt * kTn), row = q * 32 + lane;
             uint16_t* out = a.out + (x.row + row) * a.ldout + x.nt * kTn;
+            float up = 1.f;
+            if (DT == SPMM_DTYPE_F16 && x.tile) up = __uint_as_float(static_cast<uint32_t>(127 + exponents[(x.tile - 1) * kTileM + row]) << 23);
             if (q * 32 < x.rows) {
                 // 32 columns at a time, half of a 64-column block (16 KB of the stage).
                 for (int c0 = half * 32; c0 < cols; c0 += 64) {
@@ -594,7 +618,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                             float f[8];
                             RowVec<DT, 16>::unpack(o[c], f);
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) f[k] = fmaf(__uint_as_float(v[8 * c + k]), x.scale, f[k]);
+                            for (int k = 0; k < 8; ++k) f[k] = fmaf(DT == SPMM_DTYPE_F16 ? __uint_as_float(v[8 * c + k]) * up : __uint_as_float(v[8 * c + k]), x.scale, f[k]);
                             o[c] = RowVec<DT, 16>::pack(f);
                         }
                     }
@@ -636,7 +660,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             if (nu > 0) {
                 ok = __all_sync(0xffffffffu, mbar_wait(u_empty0 + 8 * ub, ((nu / kUs) & 1u) ^ 1u, abort_flag));
                 if (!ok) break;
-                make_u<DT, RB>(e, x, base + ub * L::kU, warp - 2 - kEpilogueWarps, 4);
+                make_u<DT, RB>(e, x, base + ub * L::kU, exponents + nu % L::kScales * kTileM, warp - 2 - kEpilogueWarps, 4);
                 if (lane == 0) mbar_arrive_count(u_full0 + 8 * ub, 1);
             }
             ++nu;

@@ -1,0 +1,135 @@
+"""What the adapters' intermediate u = a x keeps: FP16 values of any size, small terms behind a large base, long batches.
+
+Bound: u is a sum of K terms in 32 bits (K * 2^-23 of the sum of their magnitudes) and may then be two 16-bit terms, half a step of a
+half step of itself (2^-16 in bf16, 2^-22 in fp16), in fp16 with a power of two taken out of each row so that its largest element
+lies in [2^14, 2^15): elements far below that one keep 2^-25 of the smallest step, 2^-39 of the largest. The product with b is
+at most 2 * rank additions in 32 bits more, scale and base one rounding each."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import _rows as R
+import spmm_b200 as S
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def stream():
+    return torch.cuda.current_stream()
+
+
+def offsets(sizes):
+    return torch.tensor([0] + sizes, dtype=torch.int64).cumsum(0).to(torch.int32)
+
+
+def normal(shape, seed):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
+
+
+def exact(sizes, adapter, x, a, b, base, scale):
+    """out in 64 bits and a bound on its error before the last rounding (sizes None: a request a row)."""
+    at = offsets(sizes if sizes is not None else [1] * x.shape[0]).tolist()
+    out = torch.zeros((x.shape[0], b.shape[1]), dtype=torch.float64) if base is None else R.d(base)
+    err = torch.zeros_like(out)
+    K, rank = x.shape[1], a.shape[1]
+    for e, i, j in zip(adapter.tolist(), at, at[1:]):
+        if e < 0 or i == j:
+            continue
+        s = 1.0 if scale is None else float(scale[e])
+        u, um = R.d(x[i:j]) @ R.d(a[e]).T, R.d(x[i:j]).abs() @ R.d(a[e]).abs().T
+        kept = K * 2.0**-23 * um + R.STEP[x.dtype] ** 2 * u.abs()
+        if x.dtype == F16:
+            kept = kept + 2.0**-39 * u.abs().amax(1, keepdim=True)
+        bm, delta = R.d(b[e]).abs().T, s * (u @ R.d(b[e]).T)
+        err[i:j] = abs(s) * (kept @ bm + 2 * rank * 2.0**-23 * (um @ bm)) + 2.0**-22 * (out[i:j].abs() + delta.abs())
+        out[i:j] += delta
+    return out, err
+
+
+def check(sizes, adapter, x, a, b, base=None, scale=None, want_finite=True):
+    """Both ways to say it: packed requests, and (where every request is a row) single tokens."""
+    adapter = torch.tensor(adapter, dtype=torch.int32)
+    out = torch.full((x.shape[0], b.shape[1]), 7.0, dtype=x.dtype, device="cuda")
+    S.lora(None if sizes is None else offsets(sizes).cuda(), adapter.cuda(), x, a, b, out, base=base, scale=scale, stream=stream())
+    torch.cuda.synchronize()
+    code, detail = S.device_error(0)
+    assert code == 0, f"device error {code} ({detail})"
+    want, err = exact(sizes, adapter, x, a, b, base, scale)
+    assert not want_finite or want.abs().max() < 65504
+    bound = err + R.STEP[x.dtype] * (want.abs() + err) + R.TINY[x.dtype]
+    off = (R.d(out) - want).abs()
+    bad = ~(off <= bound)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {float((off / bound)[bad].max()):.3g} times the bound"
+    return out
+
+
+SIZES = [None, [1] * 64, [64], [1, 40, 0, 22, 1]]  # single tokens, short requests, tensor-core tiles, both in a batch
+
+
+def ads(sizes):
+    return [0] * (64 if sizes is None else len(sizes))
+
+
+@pytest.mark.parametrize("rank", [8, 48, 72, 256])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_large_intermediates_in_fp16(cuda, sizes, rank):
+    """|u| around 2^22, which the scale brings back: finite in every form, whatever batch the row is in."""
+    x = (normal((64, 64), 1) * 500 + 1000).to(F16).cuda()
+    a = (normal((1, rank, 64), 2) * 20 + 60).to(F16).cuda()
+    b = (normal((1, 72, rank), 3) * 2.0**-8).to(F16).cuda()
+    b[:, :, 1::3] = 0
+    assert (R.d(x) @ R.d(a[0]).T).abs().min() > 131008
+    check(sizes, ads(sizes), x, a, b, scale=torch.full((1,), 2.0**-10, device="cuda"))
+
+
+@pytest.mark.parametrize("rank", [8, 48, 72, 256])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_small_intermediates_in_fp16(cuda, sizes, rank):
+    """|u| around 2^-20, which b and the scale bring back."""
+    x = (normal((64, 64), 1) * 2.0**-10).to(F16).cuda()
+    a = (normal((1, rank, 64), 2) * 2.0**-13).to(F16).cuda()
+    b = (normal((1, 72, rank), 3) * 64).to(F16).cuda()
+    assert (R.d(x) @ R.d(a[0]).T).abs().max() < 2.0**-14
+    check(sizes, ads(sizes), x, a, b, scale=torch.full((1,), 4096.0, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_rows_and_ranks_of_unlike_sizes(cuda, sizes, dtype):
+    """Neighbouring rows, and elements of one row, that are powers of two apart; a row of zeros; one of the largest values."""
+    x = normal((64, 96), 1) * torch.exp2(torch.arange(64) % 23 - 11.0)[:, None]
+    x[7], x[9] = 0, 65504 * x[9].sign()
+    a = normal((1, 48, 96), 2) * torch.exp2(-(torch.arange(48) % 13.0))[None, :, None]
+    x, a, b = x.to(dtype).cuda(), a.to(dtype).cuda(), (normal((1, 136, 48), 3) * 2.0**-11).to(dtype).cuda()
+    check(sizes, ads(sizes), x, a, b)
+    assert (check(sizes, ads(sizes), x, a, b)[7] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_base_that_cancels(cuda, sizes, dtype):
+    """base = -delta to 16 bits: what is left shows the intermediate's own error, which no rounding hides."""
+    x, a, b = (normal(s, k).to(dtype).cuda() for k, s in ((1, (64, 256)), (2, (1, 32, 256)), (3, (1, 136, 32))))
+    want, _ = exact([64], torch.zeros(1, dtype=torch.int32), x, a, b, None, None)
+    check(sizes, ads(sizes), x, a, b, base=(-want).to(dtype).cuda())
+
+
+@pytest.mark.parametrize("dtype,rank", [(F16, 16), (BF16, 64), (F16, 96), (BF16, 256), (F16, 256)])
+@pytest.mark.parametrize("N", [8, 200])
+def test_many_row_tiles_a_block(cuda, dtype, rank, N):
+    """Long enough that a block makes u for several row tiles, with and without an adapter between them, into the same memory."""
+    sizes = [30000, 1, 0, 129, 41000, 128, 1, 17000, 640, 1]
+    adapter = [0, 2, 1, -1, 1, 2, 0, -1, 2, -1]
+    rows = sum(sizes)
+    x = (normal((rows, 64), 1) * torch.exp2(torch.arange(rows) % 5 - 2.0)[:, None]).to(dtype).cuda()
+    a, b = normal((3, rank, 64), 2).to(dtype).cuda(), (normal((3, N, rank), 3) / 16).to(dtype).cuda()
+    base = normal((rows, N), 4).to(dtype).cuda()
+    scale = torch.tensor([0.5, 2.0, -1.0], device="cuda")
+    first = check(sizes, adapter, x, a, b, base=base, scale=scale)
+    again = base.clone()
+    S.lora(offsets(sizes).cuda(), torch.tensor(adapter, dtype=torch.int32).cuda(), x, a, b, again, base=again, scale=scale, stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(first, again)
