@@ -724,7 +724,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
             const Tile r = tile_of<FORM, TN, SINGLES>(a, start, order, rounds, t);
             if (r.cols == 0) continue;
             const int buf = n & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag))) {
+            if (!__all_sync(0xffffffffu, mbar_wait_sum(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag, r.steps))) {
                 ok = false;
                 break;
             }
@@ -999,9 +999,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
         // ---------------- MMA issuer, one lane in block 0; in dw the warp of either block clears rows past a group's end
         const uint32_t idesc = instr_desc_f16(a.dtype, kPairN, FORM == kDw, FORM != kForward, kPairM);
         int it = 0, n = 0, tails = 0;
+        int since = 0;  // steps since the last that ended in a cleared one
         bool ok = true;
         for (int t = pair; ok && t < tiles; t += pairs, ++n) {
             const PairTile r = pair_tile<FORM>(a, start, t);
+            since = min(since, 1 << 30) + min(r.steps, 1 << 30);
             const int buf = n & 1, left = (r.end - r.begin) - (r.steps - 1) * kStepK;  // dw: rows of the last step
             const int clear = FORM == kDw && left % 16 != 0;  // 0 of an empty group too
             const uint32_t acc = tmem + buf * kPairN;
@@ -1024,7 +1026,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
             it += r.steps;
             if (FORM == kDw && clear && ok) {
                 const int s = (it - 1) % kStages, slices = (left + 15) / 16;
-                ok = __all_sync(0xffffffffu, mbar_wait(tail_full, tails & 1u, abort_flag));
+                // The other block's warp has nothing to do before this: it waits for all of the tiles since the last.
+                ok = __all_sync(0xffffffffu, mbar_wait_sum(tail_full, tails & 1u, abort_flag, since));
+                since = 0;
                 if (ok) {
                     const int pieces = (slices * 16 - left) * 8;  // 16-byte pieces of a box's rows to clear
                     for (int b = 0; b < 4; ++b) {
@@ -1064,7 +1068,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * kEpilogue,
         for (int t = pair; t < tiles; t += pairs, ++n) {
             const PairTile r = pair_tile<FORM>(a, start, t);
             const int buf = n & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag))) {
+            if (!__all_sync(0xffffffffu, mbar_wait_sum(acc_full0 + 8 * buf, (n >> 1) & 1u, abort_flag, r.steps))) {
                 ok = false;
                 break;
             }

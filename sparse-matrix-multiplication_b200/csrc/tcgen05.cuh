@@ -115,6 +115,16 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return mbar_wait_slow(bar, parity, abort_flag);
 }
 
+// mbar_wait for a whole sum of `steps` stages: as long again for every 25000 of them, 20 us a stage, of which the slowest loads
+// take 1.5. A stage that does not come ends the waits for single stages first, and they raise the abort flag.
+__device__ __forceinline__ bool mbar_wait_sum(uint32_t bar, uint32_t parity, volatile int* abort_flag, int steps) {
+    while (!mbar_wait(bar, parity, abort_flag)) {
+        if (steps <= 0 || *abort_flag) return false;
+        steps -= 25000;
+    }
+    return true;
+}
+
 __device__ __forceinline__ void mbar_arrive_count(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
