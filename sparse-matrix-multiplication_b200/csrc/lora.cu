@@ -432,8 +432,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         if (a.base) prefetch_tensormap(&map_base);
     }
     if (warp == 1) tmem_alloc(smem_addr(tmem_slot), 2 * kTn);
-    // Only the warps that read the shrink's parts wait for it (every block has them, so none ends before it): the shrink
-    // itself waited for everything before it, and writes nothing else.
+    // The shrink itself waited for everything before it, and writes nothing but the parts: the first stages' b and base are
+    // loaded while it runs. Every role waits for its end before a bounded wait that could cover it.
     allow_dependent_launch();
     build_table(start, a.requests, [&](int r) {
         const GroupRange g = group_range(a.offsets, r, a.rows, blockIdx.x == 0 ? a.err : nullptr);
@@ -467,6 +467,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             // The next stage, once it is free, with its description; its copies follow.
             const auto claim = [&](const StageInfo& info) {
                 const int s = it % kStages;
+                if (it == kStages) grid_dependency_wait();
                 ok = mbar_wait(empty0 + 8 * s, ((it / kStages) & 1u) ^ 1u, abort_flag);
                 if (ok) {
                     infos[s] = info;
@@ -544,6 +545,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             const int slices = (a.rank + 15) / 16;
             int nu = 0;
             bool ok = true;
+            grid_dependency_wait();
             // Stage `it` goes to epilogue set it & 1 with accumulator it & 1, whether or not it is a tile: so a set sees every
             // phase of its barriers, in order.
             for (int it = 0, ends = 0; ends < 2; ++it) {
@@ -658,7 +660,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             if (x.i < 0) continue;
             const int ub = nu % kUs;
             if (nu > 0) {
-                ok = __all_sync(0xffffffffu, mbar_wait(u_empty0 + 8 * ub, ((nu / kUs) & 1u) ^ 1u, abort_flag));
+                ok = __all_sync(0xffffffffu, mbar_wait_sum(u_empty0 + 8 * ub, ((nu / kUs) & 1u) ^ 1u, abort_flag, kUs * e.ntiles));
                 if (!ok) break;
                 make_u<DT, RB>(e, x, base + ub * L::kU, exponents + nu % L::kScales * kTileM, warp - 2 - kEpilogueWarps, 4);
                 if (lane == 0) mbar_arrive_count(u_full0 + 8 * ub, 1);
