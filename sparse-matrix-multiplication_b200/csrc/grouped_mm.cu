@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(tc_threads(SINGLES, ANY), 1)
             for (int g = threadIdx.x; g < a.groups; g += blockDim.x) group_range(a.offsets, g, a.rows, a.err);  // records bad ones
         tiles = a.groups * a.mtiles * a.ntiles;
     } else {
-        DeviceErrorRecord* err = blockIdx.x == 0 ? a.err : nullptr;
+        DeviceErrorRecord* err = queued || blockIdx.x == 0 ? a.err : nullptr;  // likewise
         if constexpr (SINGLES) {
             build_table(start, a.groups, [&](int g) {
                 const GroupRange r = group_range(a.offsets, g, a.rows, err);
