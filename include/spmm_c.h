@@ -315,7 +315,8 @@ int spmm_device_error(int32_t device, int32_t* code, int64_t* detail, int32_t cl
  * low-rank adapters of many requests. None has a counterpart in the reference. All pointers are
  * device pointers on the current device; calls are asynchronous on `stream`, allocate nothing,
  * use no atomics on results (the same inputs give the same bits) and can be captured in a CUDA
- * graph (after a first call on the device, which sets up the library's device state). Row strides
+ * graph (after a first call on the device, which sets up the library's device state). Index arrays, weights
+ * and scales lie on 4-byte boundaries, elements on their own (SPMM_ERR_MISALIGNED otherwise). Row strides
  * (ld*) count elements and are at least the row's length; outputs must not overlap inputs except
  * where said. Index arrays are read on the device: a bad entry never leads out of a buffer, is
  * recorded (SPMM_ERR_BAD_INDEX, spmm_device_error) and its row is left as described below. */

@@ -1224,6 +1224,7 @@ int check_common(const int32_t* offsets, int32_t groups, int32_t rows, int32_t N
     if (groups < 1 || rows < 0 || N < 0 || K < 0 || !offsets) return SPMM_ERR_INVALID_ARG;
     if (dtype != SPMM_DTYPE_F16 && dtype != SPMM_DTYPE_BF16) return SPMM_ERR_INVALID_ARG;
     if (out_dtype != dtype && out_dtype != SPMM_DTYPE_F32) return SPMM_ERR_INVALID_ARG;
+    if (!words_fit(offsets)) return SPMM_ERR_MISALIGNED;
     // Tile and row numbers are ints; the sizes of any operand that fits a GPU are far below this.
     if (groups > SPMM_MAX_GROUPS || rows > INT32_MAX - 256 || N > (1 << 24) || K > (1 << 24)) return SPMM_ERR_TOO_LARGE;
     return SPMM_OK;

@@ -782,6 +782,7 @@ int spmm_lora(const spmm_lora_view* l, const int32_t* offsets, const int32_t* ad
     const bool adds = some && l->adapters > 0 && l->rank > 0;
     if (some) {
         if (!adapter) return SPMM_ERR_INVALID_ARG;
+        if (!words_fit(offsets, adapter, l->scale)) return SPMM_ERR_MISALIGNED;
         SPMM_TRY(check_operand(out, ldout, l->N));
         if (base) SPMM_TRY(check_operand(base, ldbase, l->N));
         if (base == out && ldbase != ldout) return SPMM_ERR_INVALID_ARG;
@@ -792,7 +793,6 @@ int spmm_lora(const spmm_lora_view* l, const int32_t* offsets, const int32_t* ad
             SPMM_TRY(check_operand(l->a, l->K, l->K));
             SPMM_TRY(check_operand(x, ldx, l->K));
         }
-        if (reinterpret_cast<uintptr_t>(l->scale) % 4) return SPMM_ERR_MISALIGNED;
         if (need > 0 && (!ws || ws_bytes < need)) return SPMM_ERR_INVALID_ARG;
         if (reinterpret_cast<uintptr_t>(ws) % 256) return SPMM_ERR_MISALIGNED;
     }

@@ -580,6 +580,7 @@ int route_args(const spmm_route_view* r, int32_t H, int32_t dtype) {
     if (!r || r->tokens < 0 || r->topk < 1 || r->rows < 0 || H < 0) return SPMM_ERR_INVALID_ARG;
     if (dtype != SPMM_DTYPE_F16 && dtype != SPMM_DTYPE_BF16 && dtype != SPMM_DTYPE_F32) return SPMM_ERR_INVALID_ARG;
     if (r->tokens > 0 && !r->pos) return SPMM_ERR_INVALID_ARG;
+    if (!words_fit(r->pos)) return SPMM_ERR_MISALIGNED;
     // Vectors and bytes of a row are counted in ints.
     if (static_cast<int64_t>(r->tokens) * r->topk > INT32_MAX - 4095 || H > (1 << 24)) return SPMM_ERR_TOO_LARGE;
     return SPMM_OK;
@@ -713,7 +714,7 @@ int spmm_route_build(const int32_t* ids, int32_t tokens, int32_t topk, int32_t g
     size_t need = 0;
     SPMM_TRY(spmm_route_workspace_size(tokens, topk, groups, &need));
     if (!offsets || (tokens > 0 && (!ids || !pos)) || (need > 0 && (!ws || ws_bytes < need))) return SPMM_ERR_INVALID_ARG;
-    if (reinterpret_cast<uintptr_t>(ws) % 4) return SPMM_ERR_MISALIGNED;
+    if (!words_fit(ids, offsets, order, pos, static_cast<const int*>(ws))) return SPMM_ERR_MISALIGNED;
     DeviceState* st = nullptr;
     SPMM_TRY(current_device_state(&st));
     const cudaStream_t s = as_stream(stream);
@@ -764,7 +765,7 @@ int spmm_route_combine(const spmm_route_view* r, const void* ys, int64_t ldys, c
     SPMM_TRY(route_args(r, H, dtype));
     SPMM_TRY(check_rows(ys, ldys, r->rows, H, dtype));
     SPMM_TRY(check_rows(y, ldy, r->tokens, H, dtype));
-    if (reinterpret_cast<uintptr_t>(w) % 4) return SPMM_ERR_MISALIGNED;
+    if (!words_fit(w)) return SPMM_ERR_MISALIGNED;
     DeviceState* st = nullptr;
     SPMM_TRY(current_device_state(&st));
     if (r->tokens == 0 || H == 0) return SPMM_OK;
@@ -785,7 +786,7 @@ int spmm_route_combine_grad(const spmm_route_view* r, const void* dy, int64_t ld
     SPMM_TRY(check_rows(dy, lddy, r->tokens, H, dtype));
     if (dw) SPMM_TRY(check_rows(ys, ldys, r->rows, H, dtype));
     if (dys) SPMM_TRY(check_rows(dys, lddys, r->rows, H, dtype));
-    if (reinterpret_cast<uintptr_t>(w) % 4 || reinterpret_cast<uintptr_t>(dw) % 4) return SPMM_ERR_MISALIGNED;
+    if (!words_fit(w, dw)) return SPMM_ERR_MISALIGNED;
     DeviceState* st = nullptr;
     SPMM_TRY(current_device_state(&st));
     if (r->tokens == 0 || (H == 0 && !dw)) return SPMM_OK;

@@ -12,6 +12,12 @@
 
 namespace spmm_b200 {
 
+// Index arrays, weights and scales: 4-byte elements on their own boundaries.
+template <typename... P>
+inline bool words_fit(const P*... p) {
+    return ((reinterpret_cast<uintptr_t>(p) | ...)) % 4 == 0;
+}
+
 inline int dtype_bytes(int dtype) { return dtype == SPMM_DTYPE_F32 ? 4 : 2; }
 
 // The widest vector (16, 4 or 2 bytes) that row r + column c of every operand fits: base pointers and row
