@@ -56,6 +56,14 @@ __device__ __forceinline__ int adapter_of(const LoraArgs& a, int r, DeviceErrorR
     return i < 0 || i >= a.adapters ? -1 : i;
 }
 
+// Bad offsets and adapters of all requests, those without rows too, to the record: by one block.
+__device__ __forceinline__ void record_bad_requests(const LoraArgs& a) {
+    for (int r = threadIdx.x; r < a.requests; r += blockDim.x) {
+        if (a.offsets) group_range(a.offsets, r, a.rows, a.err);
+        adapter_of(a, r, a.err);
+    }
+}
+
 // ------------------------------------------------------------------ any alignment: one block a row
 
 template <int DT>
@@ -65,7 +73,7 @@ __global__ void __launch_bounds__(256) lora_shrink_any_kernel(LoraArgs a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int p = blockIdx.x; p < a.rows; p += gridDim.x) {
         const int r = request_of(a, p);
-        const int i = r < 0 ? -1 : adapter_of(a, r, threadIdx.x == 0 ? a.err : nullptr);
+        const int i = r < 0 ? -1 : adapter_of(a, r, nullptr);
         if (i < 0) continue;
         for (int q = warp; q < a.rank; q += 8) {
             const uint16_t* row = a.a + (static_cast<long long>(i) * a.rank + q) * a.K;
@@ -84,8 +92,7 @@ __global__ void __launch_bounds__(256) lora_expand_any_kernel(LoraArgs a) {
     __shared__ float u[kMaxRank];
     grid_dependency_wait();
     allow_dependent_launch();
-    if (blockIdx.x == 0 && a.offsets)
-        for (int r = threadIdx.x; r < a.requests; r += 256) group_range(a.offsets, r, a.rows, a.err);  // records bad ones
+    if (blockIdx.x == 0) record_bad_requests(a);
     for (int p = blockIdx.x; p < a.rows; p += gridDim.x) {
         const int r = request_of(a, p);
         if (r < 0) continue;
@@ -127,7 +134,7 @@ __global__ void __launch_bounds__(256) lora_shrink_rows_kernel(LoraArgs a, int r
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int p = blockIdx.x / rank_blocks, q0 = (blockIdx.x - p * rank_blocks) * kRanksPerBlock;
     const int r = request_of(a, p);
-    const int i = r < 0 ? -1 : adapter_of(a, r, threadIdx.x == 0 && q0 == 0 ? a.err : nullptr);
+    const int i = r < 0 ? -1 : adapter_of(a, r, nullptr);
     if (i < 0) return;
     const uint4* x = reinterpret_cast<const uint4*>(a.x + p * a.ldx);
     const uint4* rows = reinterpret_cast<const uint4*>(a.a + (static_cast<long long>(i) * a.rank + q0) * a.K);
@@ -164,8 +171,7 @@ __global__ void __launch_bounds__(256) lora_expand_rows_kernel(LoraArgs a, int c
     // Reached only behind the shrink of the same call, which has itself waited for everything before it and writes
     // nothing but u: the rest may be read before this kernel's own wait.
     allow_dependent_launch();
-    if (blockIdx.x == 0 && a.offsets)
-        for (int k = threadIdx.x; k < a.requests; k += 256) group_range(a.offsets, k, a.rows, a.err);  // records bad ones
+    if (blockIdx.x == 0) record_bad_requests(a);
     const int p = blockIdx.x / col_blocks, n = (blockIdx.x - p * col_blocks) * 256 + threadIdx.x;
     const int r = request_of(a, p);
     const int i = r < 0 ? -1 : adapter_of(a, r, nullptr);

@@ -1,4 +1,5 @@
-"""What the adapters' intermediate u = a x keeps: FP16 values of any size, small terms behind a large base, long batches.
+"""What the adapters' intermediate u = a x keeps: FP16 values of any size, small terms behind a large base, long batches;
+and the adapters that are recorded.
 
 Bound: u is a sum of K terms in 32 bits (K * 2^-23 of the sum of their magnitudes) and may then be two 16-bit terms, half a step of a
 half step of itself (2^-16 in bf16, 2^-22 in fp16), in fp16 with a power of two taken out of each row so that its largest element
@@ -133,3 +134,22 @@ def test_many_row_tiles_a_block(cuda, dtype, rank, N):
     S.lora(offsets(sizes).cuda(), torch.tensor(adapter, dtype=torch.int32).cuda(), x, a, b, again, base=again, scale=scale, stream=stream())
     torch.cuda.synchronize()
     assert torch.equal(first, again)
+
+
+@pytest.mark.parametrize("adapters,rank,N,sizes,adapter,detail", [
+    (2, 0, 64, [4, 2], [0, 2], 1),        # nothing to add
+    (0, 8, 64, [4, 2], [-1, 0], 1),       # no adapters at all
+    (2, 8, 64, [1, 0, 1], [0, 5, 1], 1),  # a request without rows: few rows a request
+    (2, 8, 65, [1, 0, 1], [0, 5, 1], 1),  # off 16-byte boundaries
+    (2, 8, 64, [40, 0, 1], [0, 5, 1], 1),  # tensor-core tiles
+])
+def test_adapters_past_the_last_are_recorded(cuda, adapters, rank, N, sizes, adapter, detail):
+    rows = sum(sizes)
+    x, a, b = (normal(s, k).to(BF16).cuda() for k, s in ((1, (rows, 64)), (2, (adapters, rank, 64)), (3, (adapters, N, rank))))
+    base = normal((rows, N), 4).to(BF16).cuda()
+    out = torch.zeros_like(base)
+    S.lora(offsets(sizes).cuda(), torch.tensor(adapter, dtype=torch.int32).cuda(), x, a, b, out, base=base, stream=stream())
+    torch.cuda.synchronize()
+    assert S.device_error(0) == (-8, detail)
+    if rank == 0 or adapters == 0:
+        assert torch.equal(out, base)
