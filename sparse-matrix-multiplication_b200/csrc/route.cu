@@ -28,7 +28,11 @@ constexpr unsigned kFull = 0xffffffffu;
 // adds up what it needs (blocks x groups ints from L2), so there is no wait between blocks.
 
 constexpr int kMaxSortThreads = 1024;
-constexpr int kOneBlock = 4096;       // pairs that one block takes alone: a second launch costs more than they do
+// Pairs that one block takes alone, without a workspace. 2048 of them: 3.8 / 5.3 / 9.6 us for 8 / 256 / 4096 groups, in two launches
+// 5.7 / 6.8 / 11.4; 4096: 5.3 / 8.8 / 13.5, in two launches 5.9 / 7.6 / 13.5.
+constexpr int kOneBlock = 4096;
+// 131072 pairs, 8 / 256 / 4096 groups: 6.8 / 9.8 / 30.5 us; 1024 a block 7.2 / 26.2 / 48.3 (128 histograms for every block to add
+// up); 4096 a block 7.8 / 12.6 / 27.9. The histograms and the order within a block bound it, not the 1.6 MB.
 constexpr int kPairsPerBlock = 2048;
 constexpr int kMaxSortBlocks = 128;   // blocks grow beyond kPairsPerBlock instead
 constexpr int kMaxSortSmem = 4 * (10 * SPMM_MAX_GROUPS + 33);  // 8 histograms, totals and prefixes of the most groups: 160 KiB
@@ -635,10 +639,10 @@ int combine_launch_ju(RouteArgs a, const void* ys, int64_t ldys, const float* w,
 
 template <int DT, int VB>
 int combine_launch(const RouteArgs& a, const void* ys, int64_t ldys, const float* w, void* y, int64_t ldy, cudaStream_t s) {
-    // Few pairs leave loads for more vectors; only where there are blocks enough without splitting a row so finely.
-    const bool many = static_cast<int64_t>(a.tokens) * a.nvec >= 512 * 1024;
-    if (many && a.topk <= 2) return combine_launch_ju<DT, VB, 2, 4>(a, ys, ldys, w, y, ldy, s);
-    if (many && a.topk <= 4) return combine_launch_ju<DT, VB, 4, 2>(a, ys, ldys, w, y, ldy, s);
+    // Few pairs leave loads for more vectors. Against 8 x 1, BF16: one token of 2 x 1001 1.8 -> 1.6 us, 2048 of 2 x 512 3.3 -> 2.5,
+    // 4096 of 4 x 2048 18.6 -> 10.9, 16384 of 1 x 4096 132 -> 54; behind by 0.2 us at most (rows of 128 bytes).
+    if (a.topk <= 2) return combine_launch_ju<DT, VB, 2, 4>(a, ys, ldys, w, y, ldy, s);
+    if (a.topk <= 4) return combine_launch_ju<DT, VB, 4, 2>(a, ys, ldys, w, y, ldy, s);
     return combine_launch_ju<DT, VB, 8, 1>(a, ys, ldys, w, y, ldy, s);
 }
 

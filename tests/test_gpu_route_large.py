@@ -1,4 +1,4 @@
-"""Routing at the sizes from which its streamed gradient and its wider sums run, against 64-bit forms on the GPU."""
+"""Routing of large batches (its streamed gradient, sums of few pairs) against 64-bit forms on the GPU."""
 from __future__ import annotations
 
 import pytest
@@ -124,7 +124,7 @@ def test_bad_positions_of_a_large_batch_are_recorded_and_skipped(cuda):
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("topk,H", [(1, 1024), (1, 3001), (2, 1000), (2, 333), (2, 4104), (3, 520), (3, 2050), (4, 2048), (4, 1001), (4, 72)])
 def test_combine_of_large_batches(cuda, topk, H, dtype):
-    """At most four pairs in batches large enough for several vectors a thread, of every vector width."""
+    """At most four pairs, several vectors a thread, of every vector width."""
     row = H * SIZE[dtype]
     width = 16 if row % 16 == 0 else (4 if row % 4 == 0 else 2)
     tokens = (512 * 1024) // (row // width) + 37
