@@ -740,9 +740,19 @@ struct Shape {
     int64_t mtiles;
 };
 
-Shape shape_of(int32_t requests, int32_t rows, int32_t K) {
+Shape shape_of(const spmm_lora_view& l, int32_t requests, int32_t rows) {
     Shape h{};
-    h.rows = rows <= 4 * static_cast<int64_t>(requests);
+    const int64_t K = l.K;
+    // Few rows a request, and the form with the smaller estimate in ns: rows, each with its adapter through L2 (5.2 TB/s) and its
+    // blocks' share, or tiles, a start and each request's column tiles (half of one where no request has more than one row).
+    // Four rows a request at most: beyond them the requests are rarely all short, and a long one costs the row form most.
+    // Measured, us, rows and tiles, BF16, N = K = 4096: 32 single rows, rank 16 4.9, 16.4; 256 single rows, rank 16 20, 31, rank 64
+    // 58, 42; 256 requests of 2, rank 16 35, 81, rank 64 109, 87; a prompt of 380 and 128 single rows, rank 16 33, 27, rank 64 106, 34;
+    // 2000 single rows, rank 8 117, 249, rank 64 430, 256.
+    const int64_t vectors = static_cast<int64_t>(l.rank) * (static_cast<int64_t>(l.N) + K);
+    const int64_t rows_ns = rows * (vectors / 2600 + l.rank / 4 + l.N / 256);
+    const int64_t tiles_ns = 12000 + requests * ((static_cast<int64_t>(l.N) + 127) / 128) * (rows <= requests ? 4 : 8);
+    h.rows = rows <= 4 * static_cast<int64_t>(requests) && rows_ns <= tiles_ns;
     h.mtiles = most_tiles(requests, rows, kTileM);
     // Ranges of the sum over K, from which the shrink chooses: enough that few tiles fill the GPU, each at least 4 steps of 64.
     h.most_splits = h.rows ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 1184 / std::max<int64_t>(1, h.mtiles), K / 256})));
@@ -774,7 +784,7 @@ extern "C" {
 int spmm_lora_workspace_size(const spmm_lora_view* l, int32_t requests, int32_t rows, size_t* bytes) {
     SPMM_TRY(check_view(l, requests, rows));
     if (!bytes) return SPMM_ERR_INVALID_ARG;
-    const Shape h = shape_of(requests, rows, l->K);
+    const Shape h = shape_of(*l, requests, rows);
     *bytes = sizeof(float) * static_cast<size_t>(rows) * l->rank * h.most_splits + (h.rows ? 0 : sizeof(int) * (2 + static_cast<size_t>(requests)));
     return SPMM_OK;
 }
@@ -829,7 +839,7 @@ int spmm_lora(const spmm_lora_view* l, const int32_t* offsets, const int32_t* ad
     const bool bf16 = l->dtype == SPMM_DTYPE_BF16;
     const bool fits = adds && st->cc_major == 10 && l->K > 0 && l->K % 8 == 0 && l->N % 8 == 0 && l->rank % 8 == 0 && fits16(x, ldx) &&
                       fits16(out, ldout) && (!base || fits16(base, ldbase)) && fits16(l->a, 8) && fits16(l->b, 8);
-    const Shape h = shape_of(requests, rows, l->K);
+    const Shape h = shape_of(*l, requests, rows);
     if (fits && h.rows) {
         const int rank_blocks = l->rank / kRanksPerBlock, col_blocks = (l->N + 255) / 256;
         const int64_t blocks = static_cast<int64_t>(rows) * std::max(rank_blocks, col_blocks);

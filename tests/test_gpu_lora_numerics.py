@@ -136,6 +136,17 @@ def test_many_row_tiles_a_block(cuda, dtype, rank, N):
     assert torch.equal(first, again)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("sizes,rank,width", [(None, 16, 4096), (None, 64, 4096), ([1] * 256, 64, 4096), ([380] + [1] * 128, 64, 2048), ([380] + [1] * 128, 8, 1024),
+                                              ([2] * 200, 128, 1024), ([2] * 200, 8, 1024), ([0] * 90 + [1, 2, 30] * 10, 128, 2048)])
+def test_few_rows_a_request_in_either_form(cuda, sizes, rank, width, dtype):
+    """At most four rows a request on average: the rank and the widths choose between rows and tiles."""
+    n = 256 if sizes is None else sum(sizes)
+    adapter = [(3 * r) % 5 - (r % 11 == 0) for r in range(n if sizes is None else len(sizes))]
+    x, a, b = normal((n, width), 1).to(dtype).cuda(), (normal((5, rank, width), 2) * width**-0.5).to(dtype).cuda(), normal((5, width, rank), 3).to(dtype).cuda()
+    check(sizes, adapter, x, a, b, base=normal((n, width), 4).to(dtype).cuda(), scale=torch.linspace(0.5, 2, 5, device="cuda"))
+
+
 @pytest.mark.parametrize("adapters,rank,N,sizes,adapter,detail", [
     (2, 0, 64, [4, 2], [0, 2], 1),        # nothing to add
     (0, 8, 64, [4, 2], [-1, 0], 1),       # no adapters at all
