@@ -226,10 +226,10 @@ __global__ void __launch_bounds__(256) lora_expand_rows_kernel(LoraArgs a, int c
 // Requests of one row come behind the tiles through the same ring: a stage is then as many of b's column tiles as it
 // holds, and the epilogue warps take the dot products with u from it on CUDA cores (lanes loading b themselves took 17 us
 // where the 100 single rows of a mixed batch now take 4).
-// The MMA needs 16-bit u; one term would cost half a step of 16 bits in every product (2^-8 in bf16), two leave half a step of
-// a half step (2^-16 in bf16, 2^-22 in fp16) for twice the MMAs, which still run under the copies. FP16's terms have
-// neither the range nor the small steps of FP32, so a row of u is held with a power of two taken out, its largest element in
-// [2^14, 2^15); the epilogue puts it back.
+// The MMA needs 16-bit u. In BF16 it takes three terms of eight bits each, which are u's FP32 value exactly: for three times
+// the MMAs of one, which still run under the copies. The third, for which shared memory has no room, is in TMEM. In FP16 two
+// terms leave 2^-22; they have neither the range nor the small steps of FP32, so a row of u is held with a power of two taken
+// out, its largest element in [2^14, 2^15), and the epilogue puts it back.
 
 constexpr int kTileM = 128;
 constexpr int kSetWarps = 8;
@@ -240,7 +240,8 @@ constexpr int kSmallRows = 32;  // tiles with no more rows load a base box of th
 template <int RB>  // rank in blocks of 64
 struct ExpandLayout {
     static constexpr int kTn = RB == 4 ? 64 : 128;
-    static constexpr int kU = 2 * RB * 16384;                 // hi blocks, lo blocks: 128 rows x 64 each
+    static constexpr int kU = 2 * RB * 16384;                 // first terms' blocks, second's: 128 rows x 64 each
+    static constexpr int kThird = RB * 32;                    // TMEM columns of the third terms (BF16), behind the accumulators
     static constexpr int kUs = RB == 1 ? 2 : 1;
     static constexpr int kB = RB * kTn * 128;
     static constexpr int kBase = kTn / 64 * 16384;            // 64-column blocks of 128 rows
@@ -259,6 +260,10 @@ struct ExpandLayout {
     static constexpr int kSlot = kExp + kScales * kTileM;
     static constexpr int kTable = kSlot + 8;
     static constexpr int kFixed = kTable + 1024;
+    static constexpr int tmem_columns(int dtype) {
+        const int used = 2 * kTn + (dtype == SPMM_DTYPE_BF16 ? kUs * kThird : 0);
+        return used <= 128 ? 128 : (used <= 256 ? 256 : 512);
+    }
 };
 
 struct ExpandArgs {
@@ -300,10 +305,75 @@ __device__ __forceinline__ Unit unit_of(const ExpandArgs& e, const int* start, i
     return x;
 }
 
-// u of one unit into shared memory, by `warps` warps of which this is the `w`-th: the parts' sum, hi and lo. A row's pieces of 8
-// ranks to consecutive lanes; the parts' loads of a piece are in flight together.
-template <int DT, int RB>
-__device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8_t* hi, int8_t* exponents, int w, int warps) {
+// u of one unit as three BF16 terms, by `warps` warps, a multiple of four, of which this is the `w`-th. A warp stores to its own
+// quarter of the TMEM lanes, 16 rows x 32 ranks at a time: four lanes read and write a row's pieces side by side.
+template <int RB>
+__device__ __forceinline__ void make_u_bf16(const ExpandArgs& e, const Unit& x, uint8_t* u, uint32_t third, int w, int warps) {
+    const LoraArgs& a = e.l;
+    const int lane = threadIdx.x & 31, q = (threadIdx.x >> 5) & 3;
+    const long long stride = static_cast<long long>(a.rows) * a.rank;
+    const int splits = e.singles[1], halves = (a.rank + 31) / 32 * 2;  // what lies past the rank is zero
+    tc_fence_after();  // the MMAs that read what was there before
+    for (int k = w / 4; k < halves; k += warps / 4) {
+        const int lane0 = 32 * q + 16 * (k & 1), row = lane0 + lane / 4, col = 32 * (k >> 1) + 4 * (lane & 3);
+        if (lane0 >= x.rows) continue;
+        float f[2][2][4] = {};  // of ranks col and col + 16, of rows row and row + 8
+        if (row < x.rows && col < a.rank) {
+            // All of a part's loads in flight together; what does not exist is the first again, and not used.
+            const float* src = a.u + static_cast<long long>(x.row + row) * a.rank + col;
+            const int right = col + 16 < a.rank ? 16 : 0, down = row + 8 < x.rows ? 8 * a.rank : 0;
+#pragma unroll 4
+            for (int s = 0; s < splits; ++s) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float4 v = *reinterpret_cast<const float4*>(src + s * stride + (c & 1) * down + (c >> 1) * right);
+                    float(&g)[4] = f[c >> 1][c & 1];
+                    g[0] += v.x, g[1] += v.y, g[2] += v.z, g[3] += v.w;
+                }
+            }
+            if (!right) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[1][i / 4][i % 4] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            uint32_t terms[3][2][2];
+#pragma unroll
+            for (int t = 0; t < 3; ++t) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // The upper halves of two words: what is cut off is exact in FP32, and nothing of an infinity or NaN.
+                    float &even = f[c][i / 2][2 * (i & 1)], &odd = f[c][i / 2][2 * (i & 1) + 1];
+                    const uint32_t lo = __float_as_uint(even), hi = __float_as_uint(odd);
+                    terms[t][i / 2][i & 1] = __byte_perm(lo, hi, 0x7632);
+                    even = fabsf(even) < INFINITY ? even - __uint_as_float(lo & 0xffff0000u) : 0.f;
+                    odd = fabsf(odd) < INFINITY ? odd - __uint_as_float(hi & 0xffff0000u) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint4* piece = swizzled_piece(u + (t * RB + col / 64) * 16384, row + 8 * h, col / 8 % 8 + 2 * c);
+                    reinterpret_cast<uint2*>(piece)[lane & 1] = make_uint2(terms[t][h][0], terms[t][h][1]);
+                }
+            }
+            __syncwarp();
+            tmem_st_16x8(third + 16 * (k >> 1) + 8 * c + (static_cast<uint32_t>(lane0) << 16), terms[2]);
+        }
+    }
+    tmem_st_wait();
+    tc_fence_before();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+
+// u of one unit as two FP16 terms, by `warps` warps of which this is the `w`-th. A row's pieces of 8 ranks to consecutive lanes; the
+// parts' loads of a piece are in flight together.
+template <int RB>
+__device__ __forceinline__ void make_u_f16(const ExpandArgs& e, const Unit& x, uint8_t* hi, int8_t* exponents, int w, int warps) {
+    constexpr int DT = SPMM_DTYPE_F16;
     const LoraArgs& a = e.l;
     const int pieces = (a.rank + 15) / 16 * 2;  // the last may lie past the rank and is zero
     int lanes = 2;                              // that a row takes
@@ -324,18 +394,16 @@ __device__ __forceinline__ void make_u(const ExpandArgs& e, const Unit& x, uint8
                 f[4] += hi4.x, f[5] += hi4.y, f[6] += hi4.z, f[7] += hi4.w;
             }
         }
-        if constexpr (DT == SPMM_DTYPE_F16) {
-            float most = 0.f;  // of the finite ones
+        float most = 0.f;  // of the finite ones
 #pragma unroll
-            for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
-            for (int d = lanes / 2; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            // Sums of products of FP16 values are 0 or between 2^-48 and 2^56: -62 <= exponent <= 42.
-            const int exponent = most > 0.f ? static_cast<int>(__float_as_uint(most) >> 23) - 127 - 14 : 0;
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - exponent) << 23);
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
+        for (int d = lanes / 2; d > 0; d /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        // Sums of products of FP16 values are 0 or between 2^-48 and 2^56: -62 <= exponent <= 42.
+        const int exponent = most > 0.f ? static_cast<int>(__float_as_uint(most) >> 23) - 127 - 14 : 0;
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - exponent) << 23);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] *= down;
-            if (piece == 0 && row < x.rows) exponents[row] = static_cast<int8_t>(exponent);
-        }
+        for (int j = 0; j < 8; ++j) f[j] *= down;
+        if (piece == 0 && row < x.rows) exponents[row] = static_cast<int8_t>(exponent);
         if (row >= x.rows || piece >= pieces) continue;
         const uint4 top = RowVec<DT, 16>::pack(f);
         float g[8];
@@ -437,7 +505,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         prefetch_tensormap(&map_b);
         if (a.base) prefetch_tensormap(&map_base);
     }
-    if (warp == 1) tmem_alloc(smem_addr(tmem_slot), 2 * kTn);
+    if (warp == 1) tmem_alloc(smem_addr(tmem_slot), L::tmem_columns(DT));
     // The shrink itself waited for everything before it, and writes nothing but the parts: the first stages' b and base are
     // loaded while it runs. Every role waits for its end before a bounded wait that could cover it.
     allow_dependent_launch();
@@ -452,6 +520,11 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    // u of a unit: into buffer `buf`, `order`-th of the block's units with an adapter.
+    const auto make_u = [&](const Unit& x, int buf, int order, int w, int warps) {
+        if constexpr (DT == SPMM_DTYPE_BF16) make_u_bf16<RB>(e, x, base + buf * L::kU, tmem + 2 * kTn + buf * L::kThird, w, warps);
+        else make_u_f16<RB>(e, x, base + buf * L::kU, exponents + order % L::kScales * kTileM, w, warps);
+    };
     // The first unit with an adapter has its u made by every warp but the first two: nothing else can begin without it.
     if (warp >= 2) {
         grid_dependency_wait();
@@ -459,7 +532,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             const Unit x = unit_of(e, start, t, end);
             t += x.nt1 - x.nt0;
             if (x.i < 0) continue;
-            make_u<DT, RB>(e, x, base, exponents, warp - 2, kExpandThreads / 32 - 2);
+            make_u(x, 0, 0, warp - 2, kExpandThreads / 32 - 2);
             if (lane == 0) mbar_arrive_count(u_first, 1);
             break;
         }
@@ -576,6 +649,10 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
                         const uint64_t db = smem_desc(sb + k / 4 * kTn * 128 + 32 * (k % 4), 16, 1024, kSwizzle128);
                         umma_f16(acc, da, db, idesc, t + k > 0 ? 1u : 0u);
                     }
+                if constexpr (DT == SPMM_DTYPE_BF16) {
+                    for (int k = 0; k < slices; ++k)
+                        umma_f16_tmem_a(acc, tmem + 2 * kTn + ub * L::kThird + 8 * k, smem_desc(sb + k / 4 * kTn * 128 + 32 * (k % 4), 16, 1024, kSwizzle128), idesc, 1u);
+                }
                 umma_commit(acc_full0 + 8 * buf);
                 if (x.last) {
                     umma_commit(u_empty0 + 8 * ub);
@@ -668,7 +745,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             if (nu > 0) {
                 ok = __all_sync(0xffffffffu, mbar_wait_sum(u_empty0 + 8 * ub, ((nu / kUs) & 1u) ^ 1u, abort_flag, kUs * e.ntiles));
                 if (!ok) break;
-                make_u<DT, RB>(e, x, base + ub * L::kU, exponents + nu % L::kScales * kTileM, warp - 2 - kEpilogueWarps, 4);
+                make_u(x, ub, nu, warp - 2 - kEpilogueWarps, 4);
                 if (lane == 0) mbar_arrive_count(u_full0 + 8 * ub, 1);
             }
             ++nu;
@@ -691,7 +768,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
             }
         }
         __syncwarp();
-        tmem_dealloc(tmem, 2 * kTn);
+        tmem_dealloc(tmem, L::tmem_columns(DT));
     }
 }
 
