@@ -363,8 +363,10 @@ int spmm_route_combine_grad(const spmm_route_view* r, const void* dy, int64_t ld
 /* Products of row groups with their own matrices, on the tensor cores: y[p, :] = w[g] * x[p, :] for
  * offsets[g] <= p < offsets[g+1], w = groups x N x K contiguous (a block-diagonal sparse matrix with dense N x K
  * blocks). x is rows x K, y rows x N; rows in no group are left as they were. offsets (groups + 1, non-decreasing,
- * within [0, rows]) stays on the device; an offset out of order is clamped to its neighbours and recorded.
- * dtype F16 or BF16 (x, w); out_dtype the same or F32; sums in FP32. 16-byte aligned pointers and rows (N and K
+ * within [0, rows]) stays on the device; one out of order is recorded: a group keeps those of its rows that exist, and
+ * rows that two groups then share hold the result of either (in dw they count in both).
+ * dtype F16 or BF16 (x, w); out_dtype the same or F32; sums in FP32, as the tensor cores add (which may cut off
+ * where an FMA rounds: at most 2^-23 of the magnitudes' sum an addition). 16-byte aligned pointers and rows (N and K
  * multiples of 8, ldx/ldy * size multiples of 16) are loaded by TMA, other operands by the kernel's own warps, at about a
  * fifth of the rate. groups <= 4096 (SPMM_ERR_TOO_LARGE above). */
 int spmm_grouped_mm(const int32_t* offsets, int32_t groups, int32_t rows, const void* x, int64_t ldx, const void* w,

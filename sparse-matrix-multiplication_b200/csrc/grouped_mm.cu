@@ -305,7 +305,8 @@ __device__ __forceinline__ Unaligned load_unaligned(const uint16_t* at, int coun
     v.shift = static_cast<int>(p & 15);
     v.count = min(count, 8);
     v.lo = v.hi = make_uint4(0, 0, 0, 0);
-    // A vector that holds a byte of the row lies in the row's allocation whole.
+    // Whole vectors: behind an operand that does not end on 16 bytes up to 14 bytes more are read, of the same 16 and so of the
+    // same page, and shifted out or cleared.
     if (v.count > 0) v.lo = __ldg(base);
     if (v.shift + 2 * v.count > 16) v.hi = __ldg(base + 1);
     return v;

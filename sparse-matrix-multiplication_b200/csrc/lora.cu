@@ -1,7 +1,8 @@
 // Low-rank adapters of many requests at once: out_p = base_p + s_i B_i (A_i x_p), i = the adapter of p's request.
 //
 // Two launches: shrink u_p = A_i x_p (rank values a row, FP32 in the workspace), expand out_p = base_p + s_i B_i u_p.
-// Three forms of each: a few rows a request (CUDA cores, latency), many (tcgen05, the rows' bytes), any alignment.
+// Three forms of each: a few rows a request (CUDA cores, latency), many (tcgen05, the rows' bytes), any alignment. The last shares
+// nothing between rows: 8200 mixed rows, N = K = 4096, rank 4 228 us (rank 8 by tcgen05 54), rank 64 and N = 4095 7.1 ms (65).
 
 #include <cuda_runtime.h>
 
