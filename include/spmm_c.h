@@ -399,7 +399,7 @@ typedef struct spmm_lora_view {
  * (the shared projection's output), NULL = 0; out may be base itself (same stride). Rows in no request are left as
  * they were. One rounding of the result; the rank-wide intermediate is an FP32 sum, which batches for the tensor cores
  * multiply by b as three BF16 terms, exactly, or as two F16 terms, to 2^-22 of itself and 2^-39 of the row's
- * largest, whatever its size. rank <= 256,
+ * largest, whatever its size (an infinity in b may give NaN there, whose terms it meets one by one). rank <= 256,
  * requests <= 4096 (SPMM_ERR_TOO_LARGE above). A workspace of spmm_lora_workspace_size bytes (any contents, 256-byte
  * aligned) belongs to the call until it has run: calls that overlap on the GPU need one each. */
 int spmm_lora_workspace_size(const spmm_lora_view* l, int32_t requests, int32_t rows, size_t* bytes);
